@@ -393,7 +393,7 @@ def _plain_select(s):
     q = _grouped(s["q"], c)
     top = q.abs().amax(-1, keepdim=True)
     e = top / torch.full_like(top, 127.0)
-    code = torch.where(e > 0, torch.round(q / e), torch.zeros_like(q)).double()
+    code = torch.where(e > 0, torch.round(q / e).clamp(-127, 127), torch.zeros_like(q)).double()
     code = torch.cat((code.clamp(min=0), code.clamp(max=0)), -1)                                 # [S][H][G][2 D]
     b = s["bounds"][table.clamp(min=0)].double().flatten(3).transpose(1, 2)                      # [S][H][MP][2 D]
     dot = torch.matmul(code, b.transpose(2, 3))                                                  # whole numbers: exact
