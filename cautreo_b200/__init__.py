@@ -25,6 +25,7 @@ CT_OK, CT_ERR_ARG, CT_ERR_CUDA, CT_ERR_NOMEM, CT_ERR_FULL, CT_ERR_UNMAPPED, CT_E
 # ct_kv_dtype_t
 CT_KV_BF16, CT_KV_F32, CT_KV_INT8, CT_KV_E4M3 = 0, 1, 2, 3
 CT_KV_Q8_0, CT_KV_Q4_0, CT_KV_Q2_0, CT_KV_Q1_0 = 4, 5, 6, 7      # block codecs of quant.h, 32 values per block
+CT_GQA_MODULO, CT_GQA_BLOCKED = 0, 1                              # ct_gqa_head_order_t
 BLOCK_BYTES = {CT_KV_Q8_0: 34, CT_KV_Q4_0: 18, CT_KV_Q2_0: 10, CT_KV_Q1_0: 6}
 
 
@@ -71,6 +72,17 @@ class MlaShape(C.Structure):
     _fields_ = [("n_heads", C.c_uint32), ("entry_dim", C.c_uint32), ("v_dim", C.c_uint32),
                 ("page_tokens", C.c_uint32), ("max_pages_per_seq", C.c_uint32), ("kv_dtype", C.c_uint32),
                 ("scale", C.c_float), ("n_pages", C.c_uint32)]
+
+
+class GqaLayout(C.Structure):
+    """ct_kv_gqa_layout_t: a paged cache with K and V per head."""
+    _fields_ = [("n_kv_heads", C.c_uint32), ("head_dim", C.c_uint32), ("page_tokens", C.c_uint32),
+                ("kv_dtype", C.c_uint32), ("n_pages", C.c_uint32), ("max_pages_per_seq", C.c_uint32)]
+
+
+class GqaShape(C.Structure):
+    _fields_ = [("kv", GqaLayout), ("n_q_heads", C.c_uint32), ("window_tokens", C.c_uint32),
+                ("head_order", C.c_uint32), ("scale", C.c_float)]
 
 
 class Scorecard(C.Structure):
@@ -141,6 +153,15 @@ SIGNATURES = {
     "ct_kv_paged_seq_lens_dev": (P, [P]),
     "ct_kv_paged_write_slots": (I, [P, P, U32, P, U32, P, U32, U32, P]),
     "ct_kv_paged_move_pages": (I, [P, P, P, P, P, U32, SZ, U32, P]),
+    "ct_kv_gqa_write_slots": (I, [C.POINTER(GqaLayout), P, P, P, P, U64, U64, U32, P, U32, P]),
+    "ct_kv_gqa_read_slots": (I, [C.POINTER(GqaLayout), P, P, P, U32, P, P, U64, U64, U32, P]),
+    "ct_kv_gqa_page_bounds": (I, [C.POINTER(GqaLayout), P, P, P, P, U32, P, P, P]),
+    "ct_kv_paged_create_gqa": (P, [C.POINTER(PagedConfig), U32, U32, I]),
+    "ct_kv_paged_append_kv": (I, [P, P, P, U32, P, P, U64, U64, U32]),
+    "ct_kv_paged_gather_kv": (I, [P, P, P, P, U32, P, P, U32]),
+    "ct_kv_paged_gqa_layout": (I, [P, C.POINTER(GqaLayout)]),
+    "ct_kv_paged_bounds": (P, [P]),
+    "ct_kv_paged_bound_scales": (P, [P]),
     # attention.h
     "ct_attn_forward": (B, [P, P, P, U32, U32, U32, F, P]),
     "ct_attn_forward_kv": (B, [P, P, P, U32, U32, U32, F, P]),
@@ -158,6 +179,13 @@ SIGNATURES = {
     "ct_attn_mla_decode_step_host": (I, [P, P, P, P, P, P, P, P, P, P]),
     "ct_attn_mla_decode_paged_noalloc": (I, [C.POINTER(MlaShape), P, U32, P, P, P, P, P, P, P, P]),
     "ct_mla_tc_error": (I, [I]),
+    "ct_gqa_plan_create": (P, [C.POINTER(GqaShape), U32, I]),
+    "ct_gqa_plan_destroy": (V, [P]),
+    "ct_gqa_plan_workers": (U32, [P]),
+    "ct_gqa_plan_scratch_bytes": (SZ, [P]),
+    "ct_attn_gqa_decode_paged": (I, [P, P, U64, P, P, P, P, P, P, P]),
+    "ct_attn_gqa_select_pages": (I, [P, P, U64, P, P, P, P, U32, U32, U32, P, P]),
+    "ct_attn_gqa_decode_selected": (I, [P, P, U64, P, P, P, P, P, U32, P, P, P]),
     # quant.h
     "ct_quant_q8_0": (V, [P, P, I64]),
     "ct_quant_q4_0": (V, [P, P, I64]),
@@ -436,6 +464,127 @@ class PagedKV:
     @property
     def seq_lens_dev(self):
         return lib().ct_kv_paged_seq_lens_dev(self.h)
+
+
+class GqaKV(PagedKV):
+    """ct_kv_paged_* handle of a cache with K and V per head (ct_kv_paged_create_gqa)."""
+
+    def __init__(self, n_seqs, max_pages_per_seq, n_pages, n_kv_heads, head_dim, page_tokens=64, window_tokens=0,
+                 dtype=CT_KV_BF16, keep_bounds=False, device=0, stream=None, _handle=None):
+        cfg = PagedConfig(n_seqs, max_pages_per_seq, n_pages, page_tokens, 2 * n_kv_heads * head_dim, window_tokens, dtype,
+                          device)
+        self.h = None
+        h = _handle if _handle is not None else lib().ct_kv_paged_create_gqa(C.byref(cfg), n_kv_heads, head_dim,
+                                                                            int(keep_bounds))
+        if not h:
+            raise RuntimeError("ct_kv_paged_create_gqa failed: " + lib().ct_hal_cuda_last_error().decode())
+        super().__init__(n_seqs, max_pages_per_seq, n_pages, page_tokens, cfg.entry_dim, window_tokens, dtype, device,
+                         stream, _handle=h)
+
+    @classmethod
+    def load(cls, path, device=0, stream=None):
+        h = lib().ct_kv_paged_load(str(path).encode(), device)
+        if not h:
+            raise RuntimeError("ct_kv_paged_load failed: " + lib().ct_hal_cuda_last_error().decode())
+        c = lib().ct_kv_paged_config(h).contents
+        lay = GqaLayout()
+        if lib().ct_kv_paged_gqa_layout(h, C.byref(lay)) != CT_OK:
+            lib().ct_kv_paged_destroy(h)
+            raise RuntimeError("ct_kv_paged_load: not a grouped-query cache")
+        return cls(c.n_seqs, c.max_pages_per_seq, c.n_pages, lay.n_kv_heads, lay.head_dim, c.page_tokens, c.window_tokens,
+                   c.dtype, device=device, stream=stream, _handle=h)
+
+    @property
+    def layout(self):
+        out = GqaLayout()
+        check(lib().ct_kv_paged_gqa_layout(self.h, C.byref(out)), "ct_kv_paged_gqa_layout")
+        return out
+
+    @property
+    def bounds(self):
+        return lib().ct_kv_paged_bounds(self.h)
+
+    @property
+    def bound_scales(self):
+        return lib().ct_kv_paged_bound_scales(self.h)
+
+    def append_kv(self, seq_ids, counts, k, v, src_dtype=CT_KV_BF16, k_stride=0, v_stride=0):
+        """Append tokens whose K and V rows are k and v (device; strides in values)."""
+        seq_ids = np.ascontiguousarray(seq_ids, np.uint32)
+        counts = np.ascontiguousarray(counts, np.uint32)
+        check(lib().ct_kv_paged_append_kv(self.h, ptr(seq_ids), ptr(counts), len(seq_ids), ptr(k), ptr(v), k_stride,
+                                          v_stride, src_dtype), "ct_kv_paged_append_kv")
+
+    def gather_kv(self, seqs, starts, counts, k_out, v_out, out_dtype=CT_KV_BF16):
+        """Several (seq, start, count) ranges, back to back, K and V apart."""
+        seqs, starts, counts = (np.ascontiguousarray(a, np.uint32) for a in (seqs, starts, counts))
+        check(lib().ct_kv_paged_gather_kv(self.h, ptr(seqs), ptr(starts), ptr(counts), len(seqs), ptr(k_out), ptr(v_out),
+                                          out_dtype), "ct_kv_paged_gather_kv")
+
+
+def gqa_write_slots(layout, pool, scales, k, v, dest_slot, n, src_dtype=CT_KV_BF16, k_stride=0, v_stride=0, stream=None):
+    """Write n tokens' K and V rows into a grouped-query pool (ct_kv_gqa_write_slots)."""
+    check(lib().ct_kv_gqa_write_slots(C.byref(layout), ptr(pool), ptr(scales), ptr(k), ptr(v), k_stride, v_stride, src_dtype,
+                                      ptr(dest_slot), n, stream), "ct_kv_gqa_write_slots")
+
+
+def gqa_read_slots(layout, pool, scales, src_slot, n, k_out, v_out, out_dtype=CT_KV_BF16, k_stride=0, v_stride=0,
+                   stream=None):
+    """Read n tokens' K and V rows back from a grouped-query pool (ct_kv_gqa_read_slots)."""
+    check(lib().ct_kv_gqa_read_slots(C.byref(layout), ptr(pool), ptr(scales), ptr(src_slot), n, ptr(k_out), ptr(v_out),
+                                     k_stride, v_stride, out_dtype, stream), "ct_kv_gqa_read_slots")
+
+
+def gqa_page_bounds(layout, pool, scales, pages, counts, n, bounds, bound_scales, stream=None):
+    """Bounds of the keys of n pages (ct_kv_gqa_page_bounds)."""
+    check(lib().ct_kv_gqa_page_bounds(C.byref(layout), ptr(pool), ptr(scales), ptr(pages), ptr(counts), n, ptr(bounds),
+                                      ptr(bound_scales), stream), "ct_kv_gqa_page_bounds")
+
+
+class GqaPlan:
+    """ct_gqa_plan_t: decode and page selection over a grouped-query cache."""
+
+    def __init__(self, layout, n_seq, n_q_heads, window_tokens=0, head_order=CT_GQA_MODULO, scale=0.0, device=0):
+        self.shape = GqaShape(layout, n_q_heads, window_tokens, head_order, scale)
+        self.n_seq = n_seq
+        self.h = lib().ct_gqa_plan_create(C.byref(self.shape), n_seq, device)
+        if not self.h:
+            raise RuntimeError("ct_gqa_plan_create failed: " + lib().ct_hal_cuda_last_error().decode())
+
+    def close(self):
+        if self.h:
+            lib().ct_gqa_plan_destroy(self.h)
+            self.h = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except (TypeError, AttributeError):   # interpreter shutdown: module globals already cleared
+            pass
+
+    @property
+    def workers(self):
+        return int(lib().ct_gqa_plan_workers(self.h))
+
+    @property
+    def scratch_bytes(self):
+        return int(lib().ct_gqa_plan_scratch_bytes(self.h))
+
+    def decode(self, q, pool, scales, block_table, seq_lens, out, lse=None, q_stride=0, stream=None):
+        check(lib().ct_attn_gqa_decode_paged(self.h, ptr(q), q_stride, ptr(pool), ptr(scales), ptr(block_table),
+                                             ptr(seq_lens), ptr(out), ptr(lse), stream), "ct_attn_gqa_decode_paged")
+
+    def select(self, q, bounds, bound_scales, block_table, seq_lens, pages, n_select, n_first=1, n_last=1, q_stride=0,
+               stream=None):
+        check(lib().ct_attn_gqa_select_pages(self.h, ptr(q), q_stride, ptr(bounds), ptr(bound_scales), ptr(block_table),
+                                             ptr(seq_lens), n_select, n_first, n_last, ptr(pages), stream),
+              "ct_attn_gqa_select_pages")
+
+    def decode_selected(self, q, pool, scales, block_table, seq_lens, pages, n_select, out, lse=None, q_stride=0,
+                        stream=None):
+        check(lib().ct_attn_gqa_decode_selected(self.h, ptr(q), q_stride, ptr(pool), ptr(scales), ptr(block_table),
+                                                ptr(seq_lens), ptr(pages), n_select, ptr(out), ptr(lse), stream),
+              "ct_attn_gqa_decode_selected")
 
 
 class MlaPlan:

@@ -1,0 +1,314 @@
+/*
+ * gqa_cache.cu -- the paged cache with K and V per head (pool
+ * [page][K, V][kv head][slot][dim]): quantise-on-write, read back, and the
+ * bounds of a page's keys that the page selection scores.
+ *
+ * A row is the D values of one token, K or V, and one head.  8-bit pools hold
+ * a scale per row, with the per-token codecs' arithmetic:
+ *   d = max|x| / 127 (int8) or / 448 (e4m3),  code = floor(x (1/d) + 1/2) or
+ *   e4m3(x (1/d)), every operation rounded once to fp32;
+ * a row that holds a NaN or an infinity has scale NaN and codes 0, so that
+ * what is read back says so instead of a finite value (and e4m3's NaN code is
+ * never stored, which the decode's widening relies on).
+ */
+#include <cuda_runtime.h>
+#include <float.h>
+#include <math.h>
+
+#include "../../include/hal.h"
+#include "../../include/kv_cache.h"
+#include "ct_internal.h"
+#include "gqa_internal.h"
+
+namespace {
+
+constexpr int kThreads = 256;
+
+/* Lanes that share a row, 8 values each: the power of two >= D / 8. */
+__host__ __device__ constexpr int lanes_of(int D) { return D <= 32 ? 4 : D <= 64 ? 8 : D <= 128 ? 16 : 32; }
+
+CT_DEV uint32_t pack2_bf16(float lo, float hi) {
+    __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<uint32_t *>(&h);
+}
+
+struct Where {
+    bool ok;
+    uint32_t token, kv, head;
+    size_t row;                  /* row of the pool */
+};
+
+/* Row r of the call, ordered (token, K / V, head). */
+CT_DEV Where where(size_t r, size_t n_rows, const int32_t *slots, uint32_t n_kv_heads, uint32_t page_tokens, uint32_t n_pages) {
+    Where w = {false, 0, 0, 0, 0};
+    if (r >= n_rows) return w;
+    w.token = (uint32_t)(r / (2 * n_kv_heads));
+    const uint32_t kh = (uint32_t)(r % (2 * n_kv_heads));
+    w.kv = kh / n_kv_heads;
+    w.head = kh % n_kv_heads;
+    const int32_t slot = slots[w.token];
+    if (slot < 0) return w;
+    const uint32_t page = (uint32_t)slot / page_tokens;
+    if (page >= n_pages) return w;
+    w.ok = true;
+    w.row = ((size_t)page * 2 * n_kv_heads + kh) * page_tokens + (uint32_t)slot % page_tokens;
+    return w;
+}
+
+template <int D, int DT, bool F32>
+__global__ void __launch_bounds__(kThreads) k_gqa_write(void *pool, float *scales, const void *ks, const void *vs, size_t k_stride,
+                                                        size_t v_stride, const int32_t *slots, uint32_t n, uint32_t n_kv_heads,
+                                                        uint32_t page_tokens, uint32_t n_pages) {
+    constexpr int L = lanes_of(D), U = D / 8;
+    const uint32_t u = threadIdx.x % L;
+    const size_t n_rows = (size_t)n * 2 * n_kv_heads;
+    const size_t r = (size_t)blockIdx.x * (kThreads / L) + threadIdx.x / L;
+    const Where w = where(r, n_rows, slots, n_kv_heads, page_tokens, n_pages);
+    const bool mine = w.ok && u < U;
+    float x[8];
+    #pragma unroll
+    for (int i = 0; i < 8; i++) x[i] = 0.0f;
+    if (mine) {
+        const size_t at = (size_t)w.token * (w.kv ? v_stride : k_stride) + (size_t)w.head * D + u * 8;
+        if (F32) {
+            const float4 *p = reinterpret_cast<const float4 *>(static_cast<const float *>(w.kv ? vs : ks) + at);
+            const float4 a = __ldg(p), b = __ldg(p + 1);
+            x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w; x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
+        } else {
+            const uint4 a = __ldg(reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(w.kv ? vs : ks) + at));
+            if (DT == CT_KV_BF16) {
+                *reinterpret_cast<uint4 *>(static_cast<uint16_t *>(pool) + w.row * D + u * 8) = a;
+                return;
+            }
+            const uint32_t ws[4] = {a.x, a.y, a.z, a.w};
+            #pragma unroll
+            for (int i = 0; i < 4; i++) { x[2 * i] = __uint_as_float(ws[i] << 16); x[2 * i + 1] = __uint_as_float(ws[i] & 0xFFFF0000u); }
+        }
+    }
+    if (DT == CT_KV_BF16) {
+        if (mine)
+            *reinterpret_cast<uint4 *>(static_cast<uint16_t *>(pool) + w.row * D + u * 8) =
+                make_uint4(pack2_bf16(x[0], x[1]), pack2_bf16(x[2], x[3]), pack2_bf16(x[4], x[5]), pack2_bf16(x[6], x[7]));
+        return;
+    }
+    uint32_t top = 0;                                        /* bits of max|x|: NaN above Inf above every finite value */
+    #pragma unroll
+    for (int i = 0; i < 8; i++) top = max(top, __float_as_uint(x[i]) & 0x7FFFFFFFu);
+    #pragma unroll
+    for (int o = 1; o < L; o <<= 1) top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
+    if (!mine) return;
+    const bool fine = top < 0x7F800000u;
+    const float d = __fdiv_rn(__uint_as_float(top), DT == CT_KV_INT8 ? 127.0f : 448.0f);
+    const float id = fine && d > 0.0f ? fminf(__fdiv_rn(1.0f, d), FLT_MAX) : 0.0f;
+    uint32_t c[2] = {0u, 0u};
+    if (fine) {
+        #pragma unroll
+        for (int k = 0; k < 2; k++) {
+            if (DT == CT_KV_INT8) {
+                uint32_t q[4];
+                #pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const int v = __float2int_rd(__fadd_rn(__fmul_rn(x[4 * k + e], id), 0.5f));
+                    q[e] = (uint32_t)max(-127, min(127, v));
+                }
+                c[k] = __byte_perm(__byte_perm(q[0], q[1], 0x0040), __byte_perm(q[2], q[3], 0x0040), 0x5410);
+            } else {
+                c[k] = (uint32_t)ct_e4m3x2_code(x[4 * k], x[4 * k + 1], id) |
+                       ((uint32_t)ct_e4m3x2_code(x[4 * k + 2], x[4 * k + 3], id) << 16);
+            }
+        }
+    }
+    *reinterpret_cast<uint2 *>(static_cast<uint8_t *>(pool) + w.row * D + u * 8) = make_uint2(c[0], c[1]);
+    if (u == 0) scales[w.row] = fine ? d : __uint_as_float(0x7FC00000u);
+}
+
+/* Eight stored values of a row in fp32. */
+template <int D, int DT>
+CT_DEV void load8(const void *pool, size_t row, uint32_t u, float sc, float *x) {
+    if (DT == CT_KV_BF16) {
+        const uint4 a = __ldg(reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(pool) + row * D + u * 8));
+        const uint32_t ws[4] = {a.x, a.y, a.z, a.w};
+        #pragma unroll
+        for (int i = 0; i < 4; i++) { x[2 * i] = __uint_as_float(ws[i] << 16); x[2 * i + 1] = __uint_as_float(ws[i] & 0xFFFF0000u); }
+    } else {
+        const uint2 a = __ldg(reinterpret_cast<const uint2 *>(static_cast<const uint8_t *>(pool) + row * D + u * 8));
+        const uint32_t ws[2] = {a.x, a.y};
+        #pragma unroll
+        for (int i = 0; i < 8; i += 2) {
+            const uint32_t w = ws[i >> 2] >> (8 * (i & 3));
+            if (DT == CT_KV_INT8) {
+                x[i] = __fmul_rn((float)(int8_t)(uint8_t)w, sc);
+                x[i + 1] = __fmul_rn((float)(int8_t)(uint8_t)(w >> 8), sc);
+            } else {
+                const float2 f = ct_e4m3x2_to_f32x2((uint16_t)w);
+                x[i] = __fmul_rn(f.x, sc);
+                x[i + 1] = __fmul_rn(f.y, sc);
+            }
+        }
+    }
+}
+
+template <int D, int DT, bool F32>
+__global__ void __launch_bounds__(kThreads) k_gqa_read(const void *pool, const float *scales, const int32_t *slots, uint32_t n,
+                                                       uint32_t n_kv_heads, uint32_t page_tokens, uint32_t n_pages, void *ko,
+                                                       void *vo, size_t k_stride, size_t v_stride) {
+    constexpr int L = lanes_of(D), U = D / 8;
+    const uint32_t u = threadIdx.x % L;
+    const size_t r = (size_t)blockIdx.x * (kThreads / L) + threadIdx.x / L;
+    const Where w = where(r, (size_t)n * 2 * n_kv_heads, slots, n_kv_heads, page_tokens, n_pages);
+    if (!w.ok || u >= U) return;
+    float x[8];
+    load8<D, DT>(pool, w.row, u, DT == CT_KV_BF16 ? 1.0f : __ldg(scales + w.row), x);
+    const size_t at = (size_t)w.token * (w.kv ? v_stride : k_stride) + (size_t)w.head * D + u * 8;
+    if (F32) {
+        float4 *p = reinterpret_cast<float4 *>(static_cast<float *>(w.kv ? vo : ko) + at);
+        p[0] = make_float4(x[0], x[1], x[2], x[3]);
+        p[1] = make_float4(x[4], x[5], x[6], x[7]);
+    } else {
+        *reinterpret_cast<uint4 *>(static_cast<uint16_t *>(w.kv ? vo : ko) + at) =
+            make_uint4(pack2_bf16(x[0], x[1]), pack2_bf16(x[2], x[3]), pack2_bf16(x[4], x[5]), pack2_bf16(x[6], x[7]));
+    }
+}
+
+/* Bounds of a page's keys, one CTA per (listed page, head):
+ *   hi_d = max_t k_td, lo_d = min_t k_td over the page's first `count` tokens,
+ *   s = max_d max(|hi_d|, |lo_d|) / 127, codes ceil(hi / s) and floor(lo / s).
+ * Maxima and minima have no order, so a page's bounds are the same whichever
+ * way its tokens came.  A NaN or an infinity among the keys: scale NaN. */
+template <int D, int DT>
+__global__ void __launch_bounds__(128) k_gqa_bounds(const void *pool, const float *scales, uint32_t n_kv_heads, uint32_t page_tokens,
+                                                    uint32_t n_pages, const int32_t *pages, const int32_t *counts, int8_t *bounds,
+                                                    float *bound_scales) {
+    constexpr int U = D / 8, R = 128 / U;                    /* threads along the row, tokens at a time */
+    __shared__ float s_hi[R][D], s_lo[R][D];
+    __shared__ uint32_t s_top[4], s_bad;
+    const uint32_t i = blockIdx.x / n_kv_heads, head = blockIdx.x % n_kv_heads;
+    const int32_t page = pages[i];
+    if (page < 0 || (uint32_t)page >= n_pages) return;
+    const int32_t ct = counts[i];
+    const uint32_t count = ct < 0 ? 0u : ((uint32_t)ct > page_tokens ? page_tokens : (uint32_t)ct);
+    const uint32_t u = threadIdx.x % U, r = threadIdx.x / U;
+    const size_t row0 = ((size_t)page * 2 * n_kv_heads + head) * page_tokens;
+    if (threadIdx.x == 0) s_bad = 0;
+    __syncthreads();
+    float hi[8], lo[8];
+    uint32_t top = 0;
+    #pragma unroll
+    for (int e = 0; e < 8; e++) { hi[e] = -INFINITY; lo[e] = INFINITY; }
+    if (r < R) {
+        for (uint32_t t = r; t < count; t += R) {
+            float x[8];
+            load8<D, DT>(pool, row0 + t, u, DT == CT_KV_BF16 ? 1.0f : __ldg(scales + row0 + t), x);
+            #pragma unroll
+            for (int e = 0; e < 8; e++) {
+                top = max(top, __float_as_uint(x[e]) & 0x7FFFFFFFu);
+                hi[e] = fmaxf(hi[e], x[e]);
+                lo[e] = fminf(lo[e], x[e]);
+            }
+        }
+        #pragma unroll
+        for (int e = 0; e < 8; e++) { s_hi[r][u * 8 + e] = hi[e]; s_lo[r][u * 8 + e] = lo[e]; }
+    }
+    if (top >= 0x7F800000u) s_bad = 1;
+    #pragma unroll
+    for (int o = 16; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
+    if ((threadIdx.x & 31) == 0) s_top[threadIdx.x >> 5] = top;
+    __syncthreads();
+    top = max(max(s_top[0], s_top[1]), max(s_top[2], s_top[3]));
+    const bool bad = s_bad != 0;
+    const float s = __fdiv_rn(__uint_as_float(top), 127.0f);
+    const size_t out = (size_t)page * n_kv_heads + head;
+    for (uint32_t d = threadIdx.x; d < (uint32_t)D; d += 128) {
+        float h = s_hi[0][d], l = s_lo[0][d];
+        #pragma unroll 4
+        for (int k = 1; k < R; k++) { h = fmaxf(h, s_hi[k][d]); l = fminf(l, s_lo[k][d]); }
+        int ch = 0, cl = 0;
+        if (!bad && s > 0.0f) {
+            ch = max(-127, min(127, __float2int_ru(__fdiv_rn(h, s))));
+            cl = max(-127, min(127, __float2int_rd(__fdiv_rn(l, s))));
+        }
+        bounds[out * 2 * D + d] = (int8_t)ch;
+        bounds[out * 2 * D + D + d] = (int8_t)cl;
+    }
+    if (threadIdx.x == 0) bound_scales[out] = bad ? __uint_as_float(0x7FC00000u) : s;
+}
+
+#define CT_BY_DIM(call)                            \
+    switch (dim) {                                 \
+        case 32: { constexpr int D = 32; call; }   \
+        case 64: { constexpr int D = 64; call; }   \
+        case 96: { constexpr int D = 96; call; }   \
+        case 128: { constexpr int D = 128; call; } \
+        case 192: { constexpr int D = 192; call; } \
+        case 256: { constexpr int D = 256; call; } \
+        default: return CT_ERR_UNSUPPORTED;        \
+    }
+
+struct WriteCall {
+    void *pool; float *scales; const void *k, *v; size_t ks, vs; const int32_t *slots;
+    uint32_t n, heads, pt, np; cudaStream_t st;
+    template <int D, int DT, bool F32> int go() const {
+        constexpr int rows = kThreads / lanes_of(D);
+        const size_t n_rows = (size_t)n * 2 * heads;
+        k_gqa_write<D, DT, F32><<<(unsigned)((n_rows + rows - 1) / rows), kThreads, 0, st>>>(pool, scales, k, v, ks, vs, slots, n,
+                                                                                             heads, pt, np);
+        ct__count_launches(1);
+        return ct__cuda_status(cudaGetLastError(), "gqa write");
+    }
+};
+
+struct ReadCall {
+    const void *pool; const float *scales; const int32_t *slots; uint32_t n, heads, pt, np; void *k, *v; size_t ks, vs;
+    cudaStream_t st;
+    template <int D, int DT, bool F32> int go() const {
+        constexpr int rows = kThreads / lanes_of(D);
+        const size_t n_rows = (size_t)n * 2 * heads;
+        k_gqa_read<D, DT, F32><<<(unsigned)((n_rows + rows - 1) / rows), kThreads, 0, st>>>(pool, scales, slots, n, heads, pt, np,
+                                                                                            k, v, ks, vs);
+        ct__count_launches(1);
+        return ct__cuda_status(cudaGetLastError(), "gqa read");
+    }
+};
+
+template <int D, class Call> int by_type(const Call &c, uint32_t dtype, int f32) {
+    switch (dtype) {
+        case CT_KV_BF16: return f32 ? c.template go<D, CT_KV_BF16, true>() : c.template go<D, CT_KV_BF16, false>();
+        case CT_KV_INT8: return f32 ? c.template go<D, CT_KV_INT8, true>() : c.template go<D, CT_KV_INT8, false>();
+        case CT_KV_E4M3: return f32 ? c.template go<D, CT_KV_E4M3, true>() : c.template go<D, CT_KV_E4M3, false>();
+        default: return CT_ERR_UNSUPPORTED;
+    }
+}
+
+template <int D>
+int bounds_of(const void *pool, const float *scales, uint32_t dtype, uint32_t heads, uint32_t pt, uint32_t np, const int32_t *pages,
+              const int32_t *counts, uint32_t n, int8_t *bounds, float *bs, cudaStream_t st) {
+    const unsigned grid = (unsigned)n * heads;
+    if (dtype == CT_KV_BF16) k_gqa_bounds<D, CT_KV_BF16><<<grid, 128, 0, st>>>(pool, scales, heads, pt, np, pages, counts, bounds, bs);
+    else if (dtype == CT_KV_INT8) k_gqa_bounds<D, CT_KV_INT8><<<grid, 128, 0, st>>>(pool, scales, heads, pt, np, pages, counts, bounds, bs);
+    else k_gqa_bounds<D, CT_KV_E4M3><<<grid, 128, 0, st>>>(pool, scales, heads, pt, np, pages, counts, bounds, bs);
+    ct__count_launches(1);
+    return ct__cuda_status(cudaGetLastError(), "gqa bounds");
+}
+
+}  // namespace
+
+extern "C" int ct__launch_gqa_write(void *pool, float *scales, uint32_t dtype, uint32_t n_kv_heads, uint32_t dim, uint32_t page_tokens,
+                                    uint32_t n_pages, const void *k, const void *v, size_t k_stride, size_t v_stride, int src_f32,
+                                    const int32_t *slots, uint32_t n, void *stream) {
+    const WriteCall c = {pool, scales, k, v, k_stride, v_stride, slots, n, n_kv_heads, page_tokens, n_pages, (cudaStream_t)stream};
+    CT_BY_DIM(return by_type<D>(c, dtype, src_f32));
+}
+
+extern "C" int ct__launch_gqa_read(const void *pool, const float *scales, uint32_t dtype, uint32_t n_kv_heads, uint32_t dim,
+                                   uint32_t page_tokens, uint32_t n_pages, const int32_t *slots, uint32_t n, void *k, void *v,
+                                   size_t k_stride, size_t v_stride, int out_f32, void *stream) {
+    const ReadCall c = {pool, scales, slots, n, n_kv_heads, page_tokens, n_pages, k, v, k_stride, v_stride, (cudaStream_t)stream};
+    CT_BY_DIM(return by_type<D>(c, dtype, out_f32));
+}
+
+extern "C" int ct__launch_gqa_bounds(const void *pool, const float *scales, uint32_t dtype, uint32_t n_kv_heads, uint32_t dim,
+                                     uint32_t page_tokens, uint32_t n_pages, const int32_t *pages, const int32_t *counts, uint32_t n,
+                                     int8_t *bounds, float *bound_scales, void *stream) {
+    CT_BY_DIM(return bounds_of<D>(pool, scales, dtype, n_kv_heads, page_tokens, n_pages, pages, counts, n, bounds, bound_scales,
+                                  (cudaStream_t)stream));
+}

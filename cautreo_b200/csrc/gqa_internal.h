@@ -1,0 +1,78 @@
+/*
+ * gqa_internal.h -- kernel arguments and launchers of the grouped-query cache
+ * and its attention, shared by host/gqa.c and csrc/gqa_*.cu.
+ */
+#ifndef CT_GQA_INTERNAL_H
+#define CT_GQA_INTERNAL_H
+
+#include <stddef.h>
+#include <stdint.h>
+
+#ifdef __cplusplus
+extern "C" {
+#endif
+
+/* One decode launch.  All pointers are device pointers. */
+typedef struct {
+    const uint16_t *q;           /* bf16 [n_seq][n_q_heads][D], rows q_stride values apart */
+    const void *pool;            /* [n_pages][2][n_kv_heads][page_tokens][D] */
+    const float *scales;         /* [n_pages][2][n_kv_heads][page_tokens], 8-bit pools */
+    const int32_t *block_table;  /* [n_seq][max_pages] */
+    const int32_t *seq_lens;     /* [n_seq] */
+    const int32_t *picked;       /* [n_seq][n_kv_heads][n_pick] logical pages, or NULL: all */
+    uint16_t *out;               /* bf16 [n_seq][n_q_heads][D] */
+    float *lse;                  /* [n_seq][n_q_heads] or NULL */
+    float *part_o, *part_ml;     /* [2 n_workers][16][D], [2 n_workers][16][2] */
+    uint32_t *counters;          /* [n_workers], zero between launches */
+    uint64_t q_stride;
+    uint32_t n_seq, n_q_heads, n_kv_heads, group, n_tiles;   /* group = query heads a kv head, tiles of 16 of them */
+    uint32_t page_tokens, max_pages, n_pages, n_pick, window, blocked;
+    uint32_t min_steps;          /* least steps a worker takes */
+    float scale_log2;            /* scale x log2(e) */
+} ct_gqa_args_t;
+
+/* One selection launch. */
+typedef struct {
+    const uint16_t *q;
+    const int8_t *bounds;        /* [n_pages][n_kv_heads][2][D]: upper, lower */
+    const float *bound_scales;   /* [n_pages][n_kv_heads] */
+    const int32_t *block_table, *seq_lens;
+    int32_t *picked;             /* [n_seq][n_kv_heads][n_pick] */
+    uint64_t q_stride;
+    uint32_t n_seq, n_q_heads, n_kv_heads, group, dim;
+    uint32_t page_tokens, max_pages, n_pages, n_pick, n_first, n_last, window, blocked;
+} ct_gqa_select_args_t;
+
+/* Whether a kernel exists for these, CTAs it runs on an SM of the current
+ * device (0: none; also sets the kernel's shared-memory limit there). */
+int ct__gqa_decode_ctas(uint32_t dim, uint32_t dtype);
+int ct__launch_gqa_decode(const ct_gqa_args_t *a, uint32_t dim, uint32_t dtype, uint32_t n_workers, void *stream);
+/* The same for one storage type (gqa_decode_<type>.cu). */
+int ct__gqa_ctas_bf16(uint32_t dim);
+int ct__gqa_ctas_int8(uint32_t dim);
+int ct__gqa_ctas_e4m3(uint32_t dim);
+int ct__gqa_run_bf16(const ct_gqa_args_t *a, uint32_t dim, uint32_t n_workers, void *stream);
+int ct__gqa_run_int8(const ct_gqa_args_t *a, uint32_t dim, uint32_t n_workers, void *stream);
+int ct__gqa_run_e4m3(const ct_gqa_args_t *a, uint32_t dim, uint32_t n_workers, void *stream);
+
+/* Most pages a sequence may have for a selection; prepares the kernel on the
+ * current device. */
+int ct__gqa_select_prepare(void);
+uint32_t ct__gqa_select_max_pages(void);
+int ct__launch_gqa_select(const ct_gqa_select_args_t *a, void *stream);
+
+int ct__launch_gqa_write(void *pool, float *scales, uint32_t dtype, uint32_t n_kv_heads, uint32_t dim, uint32_t page_tokens,
+                         uint32_t n_pages, const void *k, const void *v, size_t k_stride, size_t v_stride, int src_f32,
+                         const int32_t *slots, uint32_t n, void *stream);
+int ct__launch_gqa_read(const void *pool, const float *scales, uint32_t dtype, uint32_t n_kv_heads, uint32_t dim,
+                        uint32_t page_tokens, uint32_t n_pages, const int32_t *slots, uint32_t n, void *k, void *v,
+                        size_t k_stride, size_t v_stride, int out_f32, void *stream);
+int ct__launch_gqa_bounds(const void *pool, const float *scales, uint32_t dtype, uint32_t n_kv_heads, uint32_t dim,
+                          uint32_t page_tokens, uint32_t n_pages, const int32_t *pages, const int32_t *counts, uint32_t n,
+                          int8_t *bounds, float *bound_scales, void *stream);
+
+#ifdef __cplusplus
+}
+#endif
+
+#endif /* CT_GQA_INTERNAL_H */

@@ -1,0 +1,257 @@
+/*
+ * gqa_select.cu -- the pages that a query is likely to attend, chosen by a
+ * cheap score for each (sequence, kv head).
+ *
+ * Math: a query head of the group is rounded to whole numbers, e = max|q|/127,
+ * c = rint(q / e).  With a page's bounds (upper and lower codes hi, lo and
+ * their scale s), the largest dot product that any key inside the bounds has
+ * is sum_d max(c_d, 0) hi_d + min(c_d, 0) lo_d, a dot product of length 2 D
+ * in int8 with an int32 sum; score = max over heads of (sum * e), times s.
+ * Whole-number sums are exact in every order, and the two products are
+ * single fp32 roundings, so the chosen pages do not depend on how the sums
+ * are split (ties go to the lowest page).
+ *
+ * Bound: HBM, 2 D + 4 bytes a page and head.  A CTA per (sequence, kv head):
+ * its warps take 8 pages at a time as the columns of mma.sync m16n8k32 (int8),
+ * the heads of the group being the rows; the scores become ordered 32-bit
+ * keys in shared memory, a radix select of 8 bits a pass finds the key of the
+ * last page chosen, and a scan writes the pages in ascending order.
+ */
+#include <cuda_runtime.h>
+#include <math.h>
+
+#include "../../include/hal.h"
+#include "../../include/kv_cache.h"
+#include "ct_internal.h"
+#include "gqa_internal.h"
+
+namespace {
+
+constexpr int kThreads = 256, kWarps = kThreads / 32;
+constexpr uint32_t kMaxPages = 49152;                        /* keys in shared memory: 192 KB */
+constexpr uint32_t kKeyInf = 0xFF800000u, kKeyForced = 0xFFFFFFFFu;
+
+CT_DEV void mma_s8(int *c, const uint32_t *a, uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+/* Ordered key of a score: larger score, larger key; 0 is kept for "never". */
+CT_DEV uint32_t key_of(float x) {
+    if (x != x) return kKeyInf;
+    const uint32_t u = __float_as_uint(x + 0.0f);            /* -0 and +0 tie */
+    return (u >> 31) ? ~u : u | 0x80000000u;
+}
+
+template <int D>
+__global__ void __launch_bounds__(kThreads) k_gqa_select(const ct_gqa_select_args_t a) {
+    extern __shared__ __align__(16) uint32_t keys[];
+    constexpr int kPitch = 2 * D + 16;
+    __shared__ __align__(16) int8_t s_q[16][kPitch];         /* (positive, negative) parts of 16 heads' codes */
+    __shared__ float s_e[16];
+    __shared__ uint32_t s_bad, s_hist[256], s_scan[2][kWarps], s_thr, s_left, s_nz;
+    const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, j = lane & 3;
+    const uint32_t seq = blockIdx.x / a.n_kv_heads, head = blockIdx.x % a.n_kv_heads;
+    int32_t *out = a.picked + (size_t)blockIdx.x * a.n_pick;
+    const int32_t n = a.seq_lens[seq];
+    const uint32_t cap = a.max_pages * a.page_tokens;
+    const uint32_t len = n < 0 ? 0u : ((uint32_t)n > cap ? cap : (uint32_t)n);
+    const uint32_t start = a.window && len > a.window ? len - a.window : 0u;
+    const uint32_t first = start / a.page_tokens;
+    const uint32_t have = len ? (len - 1) / a.page_tokens - first + 1 : 0u;
+    const int32_t *table = a.block_table + (size_t)seq * a.max_pages + first;
+    const bool choose = have > a.n_pick;
+    if (tid == 0) { s_bad = 0; s_nz = 0; }
+    __syncthreads();
+
+    const uint32_t n_tiles = (a.group + 15) / 16;
+    for (uint32_t tile = 0; choose && tile < n_tiles; tile++) {
+        /* the tile's heads as whole numbers: two rows a warp */
+        for (uint32_t r = warp; r < 16; r += kWarps) {
+            const uint32_t in_group = tile * 16 + r;
+            const bool live = in_group < a.group;
+            const uint32_t qh = a.blocked ? head * a.group + in_group : in_group * a.n_kv_heads + head;
+            const uint16_t *qp = a.q + (size_t)seq * a.q_stride + (size_t)qh * D;
+            float x[D / 32];
+            uint32_t top = 0;
+            #pragma unroll
+            for (int i = 0; i < D / 32; i++) {
+                x[i] = live ? ct_bf16_to_f32(qp[lane + 32 * i]) : 0.0f;
+                top = max(top, __float_as_uint(x[i]) & 0x7FFFFFFFu);
+            }
+            #pragma unroll
+            for (int o = 16; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
+            const float e = __fdiv_rn(__uint_as_float(top), 127.0f);
+            #pragma unroll
+            for (int i = 0; i < D / 32; i++) {
+                int c = 0;
+                if (top < 0x7F800000u && e > 0.0f) c = __float2int_rn(__fdiv_rn(x[i], e));
+                c = max(-127, min(127, c));
+                s_q[r][lane + 32 * i] = (int8_t)max(c, 0);
+                s_q[r][D + lane + 32 * i] = (int8_t)min(c, 0);
+            }
+            if (lane == 0) {
+                s_e[r] = e;
+                if (top >= 0x7F800000u) s_bad = 1;
+            }
+        }
+        __syncthreads();
+        uint32_t qa[D / 16][4];
+        #pragma unroll
+        for (int b = 0; b < D / 32; b++) {                   /* 64 bytes of the row: lane j owns bytes 16 j .. 16 j + 15 */
+            #pragma unroll
+            for (int h = 0; h < 2; h++) {
+                const uint4 w = *reinterpret_cast<const uint4 *>(&s_q[g + 8 * h][b * 64 + 16 * j]);
+                qa[2 * b][h] = w.x; qa[2 * b][2 + h] = w.y;
+                qa[2 * b + 1][h] = w.z; qa[2 * b + 1][2 + h] = w.w;
+            }
+        }
+        const uint32_t rows = a.group - tile * 16 < 16 ? a.group - tile * 16 : 16;
+        const float e0 = s_e[g], e1 = s_e[g + 8];
+        const bool bad = s_bad != 0;
+        for (uint32_t p0 = warp * 8; p0 < have; p0 += kWarps * 8) {
+            const uint32_t p = p0 + g;
+            const int32_t ph = p < have ? table[p] : -1;
+            const bool ok = (uint32_t)ph < a.n_pages;
+            const size_t at = (size_t)(ok ? ph : 0) * a.n_kv_heads + head;
+            const uint4 *src = reinterpret_cast<const uint4 *>(a.bounds + at * 2 * D) + j;
+            uint4 w[D / 32];
+            #pragma unroll
+            for (int b = 0; b < D / 32; b++) w[b] = ok ? __ldg(src + b * 4) : make_uint4(0u, 0u, 0u, 0u);
+            const float ps = ok ? __ldg(a.bound_scales + at) : 0.0f;
+            int c[4] = {0, 0, 0, 0};
+            #pragma unroll
+            for (int b = 0; b < D / 32; b++) {
+                mma_s8(c, qa[2 * b], w[b].x, w[b].y);
+                mma_s8(c, qa[2 * b + 1], w[b].z, w[b].w);
+            }
+            float m[2];
+            #pragma unroll
+            for (int h = 0; h < 2; h++) {                    /* pages p0 + 2j + h */
+                m[h] = g < rows ? __fmul_rn((float)c[h], e0) : -INFINITY;
+                if (g + 8 < rows) m[h] = fmaxf(m[h], __fmul_rn((float)c[2 + h], e1));
+                #pragma unroll
+                for (int o = 4; o < 32; o <<= 1) m[h] = fmaxf(m[h], __shfl_xor_sync(0xFFFFFFFFu, m[h], o));
+                const float pscale = __shfl_sync(0xFFFFFFFFu, ps, (2 * j + h) * 4);
+                const bool pok = __shfl_sync(0xFFFFFFFFu, ok ? 1 : 0, (2 * j + h) * 4) != 0;
+                const uint32_t pp = p0 + 2 * j + h;
+                if (g == 0 && pp < have) {
+                    uint32_t key = bad ? kKeyInf : key_of(__fmul_rn(m[h], pscale));
+                    if (pp < a.n_first || pp + a.n_last >= have) key = kKeyForced;
+                    if (!pok) key = 0;
+                    keys[pp] = tile ? max(keys[pp], key) : key;
+                }
+            }
+        }
+        __syncthreads();
+    }
+    if (!choose)
+        for (uint32_t p = tid; p < have; p += kThreads) keys[p] = (uint32_t)table[p] < a.n_pages ? 1u : 0u;
+    __syncthreads();
+
+    /* ---- the key of the last page chosen ---- */
+    uint32_t thr = 0, left = 0;                              /* keys above thr, and the first `left` equal to it, are chosen */
+    if (choose) {
+        uint32_t nz = 0;
+        for (uint32_t p = tid; p < have; p += kThreads) nz += keys[p] != 0;
+        nz = __reduce_add_sync(0xFFFFFFFFu, nz);
+        if (lane == 0) atomicAdd(&s_nz, nz);
+        __syncthreads();
+        if (s_nz > a.n_pick) {
+            uint32_t want = a.n_pick, prefix = 0;
+            for (int shift = 24; shift >= 0; shift -= 8) {
+                s_hist[tid] = 0;
+                __syncthreads();
+                for (uint32_t p = tid; p < have; p += kThreads) {
+                    const uint32_t k = keys[p];
+                    if (shift == 24 || (k >> (shift + 8)) == (prefix >> (shift + 8))) atomicAdd(&s_hist[(k >> shift) & 255u], 1u);
+                }
+                __syncthreads();
+                /* suffix counts over 256 bins; thread t looks at bin 255 - t */
+                const uint32_t cnt = s_hist[255 - tid];
+                uint32_t inc = cnt;
+                #pragma unroll
+                for (int o = 1; o < 32; o <<= 1) {
+                    const uint32_t y = __shfl_up_sync(0xFFFFFFFFu, inc, o);
+                    if (lane >= (uint32_t)o) inc += y;
+                }
+                if (lane == 31) s_scan[0][warp] = inc;
+                __syncthreads();
+                for (uint32_t w = 0; w < warp; w++) inc += s_scan[0][w];
+                if (inc >= want && inc - cnt < want) { s_thr = 255 - tid; s_left = want - (inc - cnt); }
+                __syncthreads();
+                prefix |= s_thr << shift;
+                want = s_left;
+                __syncthreads();
+            }
+            thr = prefix;
+            left = want;
+        }
+    }
+    /* ---- ascending pages: thread t owns a run of them ---- */
+    const uint32_t per = (have + kThreads - 1) / kThreads;
+    const uint32_t b0 = min(tid * per, have), b1 = min(b0 + per, have);
+    uint32_t gt = 0, eq = 0;
+    for (uint32_t p = b0; p < b1; p++) { gt += keys[p] > thr; eq += keys[p] == thr; }
+    uint32_t ig = gt, ie = eq;
+    #pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t yg = __shfl_up_sync(0xFFFFFFFFu, ig, o), ye = __shfl_up_sync(0xFFFFFFFFu, ie, o);
+        if (lane >= (uint32_t)o) { ig += yg; ie += ye; }
+    }
+    if (lane == 31) { s_scan[0][warp] = ig; s_scan[1][warp] = ie; }
+    __syncthreads();
+    uint32_t all_gt = 0;
+    for (uint32_t w = 0; w < kWarps; w++) {
+        if (w < warp) { ig += s_scan[0][w]; ie += s_scan[1][w]; }
+        all_gt += s_scan[0][w];
+    }
+    uint32_t ng = ig - gt, ne = ie - eq;
+    for (uint32_t p = b0; p < b1; p++) {
+        const uint32_t k = keys[p];
+        const bool take = k > thr || (k == thr && thr != 0 && ne < left);
+        if (take) out[ng + min(ne, left)] = (int32_t)(first + p);
+        ng += k > thr;
+        ne += k == thr;
+    }
+    for (uint32_t i = all_gt + left + tid; i < a.n_pick; i += kThreads) out[i] = -1;
+}
+
+template <int D> int prepare() {
+    return ct__cuda_status(cudaFuncSetAttribute(k_gqa_select<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxPages * 4),
+                           "gqa select");
+}
+
+template <int D> int run(const ct_gqa_select_args_t *a, cudaStream_t st) {
+    k_gqa_select<D><<<a->n_seq * a->n_kv_heads, kThreads, (size_t)a->max_pages * 4, st>>>(*a);
+    ct__count_launches(1);
+    return ct__cuda_status(cudaGetLastError(), "gqa select");
+}
+
+}  // namespace
+
+extern "C" uint32_t ct__gqa_select_max_pages(void) { return kMaxPages; }
+
+extern "C" int ct__gqa_select_prepare(void) {
+    int rc = prepare<32>();
+    if (!rc) rc = prepare<64>();
+    if (!rc) rc = prepare<96>();
+    if (!rc) rc = prepare<128>();
+    if (!rc) rc = prepare<192>();
+    if (!rc) rc = prepare<256>();
+    return rc;
+}
+
+extern "C" int ct__launch_gqa_select(const ct_gqa_select_args_t *a, void *stream) {
+    cudaStream_t st = (cudaStream_t)stream;
+    switch (a->dim) {
+        case 32: return run<32>(a, st);
+        case 64: return run<64>(a, st);
+        case 96: return run<96>(a, st);
+        case 128: return run<128>(a, st);
+        case 192: return run<192>(a, st);
+        case 256: return run<256>(a, st);
+        default: return CT_ERR_UNSUPPORTED;
+    }
+}

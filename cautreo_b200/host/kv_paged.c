@@ -28,6 +28,7 @@
 #include "../../include/hal.h"
 #include "../../include/kv_cache.h"
 #include "../csrc/ct_internal.h"
+#include "../csrc/gqa_internal.h"
 
 #include <cuda_runtime_api.h>
 #include <stdio.h>
@@ -36,6 +37,8 @@
 
 /* Device helper in kv_kernels.cu: dst[idx[i]] = val[i]. */
 int ct__launch_scatter_i32(int32_t *dst, const int32_t *pairs, uint32_t n_pairs, void *stream);
+/* Checks a grouped-query layout and fills in its defaults (gqa.c). */
+int ct__gqa_layout(const ct_kv_gqa_layout_t *in, ct_kv_gqa_layout_t *out);
 
 struct ct_kv_paged {
     ct_kv_paged_config_t cfg;
@@ -46,7 +49,13 @@ struct ct_kv_paged {
     /* device */
     void *pool;
     float *scales;
-    int pool_async;             /* pool / scales came from cudaMallocAsync (a compaction) */
+    int pool_async;             /* pool / scales / bounds came from cudaMallocAsync (a compaction) */
+    /* grouped-query caches (ct_kv_paged_create_gqa): an entry is K and V of
+     * every head, a page [K, V][head][slot][dim], a scale per row */
+    uint32_t gqa_heads, gqa_dim;        /* 0: another kind of cache */
+    size_t scale_rows;                  /* scales of a token: 1, or 2 x heads */
+    int8_t *bounds;                     /* [n_pages][heads][2][dim], or NULL */
+    float *bound_scales;                /* [n_pages][heads] */
     int32_t *bt_dev;
     int32_t *len_dev;
     int32_t *stage_dev;         /* staged dest slots + (index, value) pairs */
@@ -186,7 +195,7 @@ void ct_kv_paged_destroy(ct_kv_paged_t *h) {
         if (h->stage_pending) cudaEventSynchronize(h->stage_ev);
         cudaStreamSynchronize(h->stream);         /* no access to the buffers may be in flight */
         if (h->stage_ev) cudaEventDestroy(h->stage_ev);
-        cudaFree(h->pool); cudaFree(h->scales); cudaFree(h->bt_dev); cudaFree(h->len_dev); cudaFree(h->stage_dev);
+        cudaFree(h->pool); cudaFree(h->scales); cudaFree(h->bounds); cudaFree(h->bound_scales); cudaFree(h->bt_dev); cudaFree(h->len_dev); cudaFree(h->stage_dev);
         if (h->stage_host) cudaFreeHost(h->stage_host);
     }
     free(h->bt); free(h->len); free(h->lo); free(h->hi); free(h->last_access); free(h->rank); free(h->refc);
@@ -196,7 +205,7 @@ void ct_kv_paged_destroy(ct_kv_paged_t *h) {
     free(h);
 }
 
-ct_kv_paged_t *ct_kv_paged_create(const ct_kv_paged_config_t *cfg) {
+static ct_kv_paged_t *create_impl(const ct_kv_paged_config_t *cfg, uint32_t gqa_heads, uint32_t gqa_dim, int keep_bounds) {
     if (!cfg || cfg->n_seqs == 0 || cfg->n_pages == 0 || cfg->max_pages_per_seq == 0 || cfg->dtype > CT_KV_Q1_0) {
         ct__set_error("ct_kv_paged_create: bad config");
         return NULL;
@@ -204,6 +213,9 @@ ct_kv_paged_t *ct_kv_paged_create(const ct_kv_paged_config_t *cfg) {
     ct_kv_paged_t *h = (ct_kv_paged_t *)calloc(1, sizeof *h);
     if (!h) return NULL;
     h->cfg = *cfg;
+    h->gqa_heads = gqa_heads;
+    h->gqa_dim = gqa_dim;
+    h->scale_rows = gqa_heads ? 2 * (size_t)gqa_heads : 1;
     if (h->cfg.page_tokens == 0) h->cfg.page_tokens = 64;
     if (h->cfg.entry_dim == 0) h->cfg.entry_dim = 576;
     if (h->cfg.entry_dim % 16 != 0) { ct__set_error("ct_kv_paged_create: entry_dim % 16 != 0"); free(h); return NULL; }
@@ -249,16 +261,51 @@ ct_kv_paged_t *ct_kv_paged_create(const ct_kv_paged_config_t *cfg) {
     if (h->host_only) return h;
     int rc = ct__cuda_status(cudaMalloc(&h->pool, (size_t)NP * h->page_bytes), "ct_kv_paged_create pool");
     if (!rc && (h->cfg.dtype == CT_KV_INT8 || h->cfg.dtype == CT_KV_E4M3))
-        rc = ct__cuda_status(cudaMalloc((void **)&h->scales, (size_t)NP * P * sizeof(float)), "ct_kv_paged_create scales");
+        rc = ct__cuda_status(cudaMalloc((void **)&h->scales, (size_t)NP * P * h->scale_rows * sizeof(float)), "ct_kv_paged_create scales");
+    if (!rc && keep_bounds) {
+        const size_t nb = (size_t)NP * gqa_heads * 2 * gqa_dim, ns = (size_t)NP * gqa_heads * sizeof(float);
+        rc = ct__cuda_status(cudaMalloc((void **)&h->bounds, nb), "ct_kv_paged_create bounds");
+        if (!rc) rc = ct__cuda_status(cudaMalloc((void **)&h->bound_scales, ns), "ct_kv_paged_create bounds");
+        if (!rc) rc = ct__cuda_status(cudaMemset(h->bounds, 0, nb), "ct_kv_paged_create");
+        if (!rc) rc = ct__cuda_status(cudaMemset(h->bound_scales, 0, ns), "ct_kv_paged_create");
+    }
     if (!rc) rc = ct__cuda_status(cudaMalloc((void **)&h->bt_dev, bt_n * sizeof(int32_t)), "ct_kv_paged_create bt");
     if (!rc) rc = ct__cuda_status(cudaMalloc((void **)&h->len_dev, (size_t)S * sizeof(int32_t)), "ct_kv_paged_create len");
     if (!rc) rc = ct__cuda_status(cudaMemset(h->bt_dev, 0xFF, bt_n * sizeof(int32_t)), "ct_kv_paged_create");
     if (!rc) rc = ct__cuda_status(cudaMemset(h->len_dev, 0, (size_t)S * sizeof(int32_t)), "ct_kv_paged_create");
-    if (!rc && h->scales) rc = ct__cuda_status(cudaMemset(h->scales, 0, (size_t)NP * P * sizeof(float)), "ct_kv_paged_create");
+    if (!rc && h->scales)
+        rc = ct__cuda_status(cudaMemset(h->scales, 0, (size_t)NP * P * h->scale_rows * sizeof(float)), "ct_kv_paged_create");
     if (!rc) rc = ct__cuda_status(cudaEventCreateWithFlags(&h->stage_ev, cudaEventDisableTiming), "ct_kv_paged_create");
     if (rc) { ct_kv_paged_destroy(h); return NULL; }
     return h;
 }
+
+ct_kv_paged_t *ct_kv_paged_create(const ct_kv_paged_config_t *cfg) { return create_impl(cfg, 0, 0, 0); }
+
+ct_kv_paged_t *ct_kv_paged_create_gqa(const ct_kv_paged_config_t *cfg, uint32_t n_kv_heads, uint32_t head_dim, int keep_bounds) {
+    if (!cfg) { ct__set_error("ct_kv_paged_create_gqa: no config"); return NULL; }
+    const ct_kv_gqa_layout_t in = {n_kv_heads, head_dim, cfg->page_tokens, cfg->dtype, cfg->n_pages, cfg->max_pages_per_seq};
+    ct_kv_gqa_layout_t l;
+    if (ct__gqa_layout(&in, &l)) return NULL;
+    ct_kv_paged_config_t c = *cfg;
+    if (c.entry_dim == 0) c.entry_dim = 2 * n_kv_heads * head_dim;
+    if (c.entry_dim != 2 * n_kv_heads * head_dim) {
+        ct__set_error("ct_kv_paged_create_gqa: entry_dim is 2 x n_kv_heads x head_dim");
+        return NULL;
+    }
+    return create_impl(&c, n_kv_heads, head_dim, keep_bounds);
+}
+
+int ct_kv_paged_gqa_layout(const ct_kv_paged_t *h, ct_kv_gqa_layout_t *out) {
+    if (!h || !out) return CT_ERR_ARG;
+    if (!h->gqa_heads) return CT_ERR_UNSUPPORTED;
+    *out = (ct_kv_gqa_layout_t){h->gqa_heads, h->gqa_dim, h->cfg.page_tokens, h->cfg.dtype, h->cfg.n_pages,
+                                h->cfg.max_pages_per_seq};
+    return CT_OK;
+}
+
+int8_t *ct_kv_paged_bounds(ct_kv_paged_t *h) { return h ? h->bounds : NULL; }
+float *ct_kv_paged_bound_scales(ct_kv_paged_t *h) { return h ? h->bound_scales : NULL; }
 
 int ct_kv_paged_set_stream(ct_kv_paged_t *h, void *stream) {
     if (!h) return CT_ERR_ARG;
@@ -314,16 +361,30 @@ typedef struct {
     uint32_t norm_dim, n_in;
 } proj_args_t;
 
+/* K and V of ct_kv_paged_append_kv. */
+typedef struct {
+    const void *k, *v;
+    uint64_t k_stride, v_stride;
+} kv_args_t;
+
+/* Pages of a grouped-query cache whose keys changed, with their tokens. */
+typedef struct {
+    const int32_t *pages, *counts;
+    uint32_t n;
+} touched_t;
+
 /* Uploads n_dest token slots plus the pending bt / len (index, value) pairs
  * in one pinned staging copy, then runs the scatters and the token writes
- * (entries copied, or projected when pj is set). */
-static int flush(ct_kv_paged_t *h, const int32_t *dest, uint32_t n_dest, const void *entries, uint32_t src_dtype,
-                 const proj_args_t *pj) {
+ * (entries copied, or projected when pj is set, or K and V of kv), and makes
+ * the bounds of the touched pages. */
+static int flush_all(ct_kv_paged_t *h, const int32_t *dest, uint32_t n_dest, const void *entries, uint32_t src_dtype,
+                     const proj_args_t *pj, const kv_args_t *kv, const touched_t *tp) {
     const size_t n_pairs = (size_t)h->n_bt_pairs + h->n_len_pairs;
-    const size_t total = n_dest + 2 * n_pairs;
+    const size_t n_tp = tp && h->bounds ? tp->n : 0;
+    const size_t total = n_dest + 2 * n_pairs + 2 * n_tp;
     if (h->host_only) {
         h->n_bt_pairs = h->n_len_pairs = 0;
-        return entries || pj ? CT_ERR_UNSUPPORTED : CT_OK;
+        return entries || pj || kv ? CT_ERR_UNSUPPORTED : CT_OK;
     }
     if (total == 0) return CT_OK;
     int rc = stage_reserve(h, total);
@@ -340,6 +401,11 @@ static int flush(ct_kv_paged_t *h, const int32_t *dest, uint32_t n_dest, const v
         pr[2 * i] = h->pairs[2 * i];
         pr[2 * i + 1] = (int32_t)h->len[h->pairs[2 * i]];
     }
+    const size_t tp_at = n_dest + 2 * n_pairs;
+    if (n_tp) {
+        memcpy(h->stage_host + tp_at, tp->pages, n_tp * sizeof(int32_t));
+        memcpy(h->stage_host + tp_at + n_tp, tp->counts, n_tp * sizeof(int32_t));
+    }
     rc = ct__cuda_status(cudaMemcpyAsync(h->stage_dev, h->stage_host, total * sizeof(int32_t),
                                          cudaMemcpyHostToDevice, h->stream), "stage upload");
     if (!rc) rc = ct__cuda_status(cudaEventRecord(h->stage_ev, h->stream), "stage event");
@@ -351,11 +417,24 @@ static int flush(ct_kv_paged_t *h, const int32_t *dest, uint32_t n_dest, const v
     if (!rc && pj && n_dest)
         rc = ct_kv_project_write_slots(pj->x, pj->w, pj->norm_w, pj->eps, pj->norm_dim, n_dest, pj->n_in,
                                        h->cfg.entry_dim, h->pool, h->scales, h->cfg.dtype, h->stage_dev, h->stream);
+    else if (!rc && kv && n_dest)
+        rc = ct__launch_gqa_write(h->pool, h->scales, h->cfg.dtype, h->gqa_heads, h->gqa_dim, h->cfg.page_tokens,
+                                  h->cfg.n_pages, kv->k, kv->v, kv->k_stride, kv->v_stride, src_dtype == CT_KV_F32,
+                                  h->stage_dev, n_dest, h->stream);
     else if (!rc && entries && n_dest)
         rc = ct_kv_paged_write_slots(h->pool, h->scales, h->cfg.dtype, entries, src_dtype, h->stage_dev, n_dest,
                                      h->cfg.entry_dim, h->stream);
+    if (!rc && n_tp)
+        rc = ct__launch_gqa_bounds(h->pool, h->scales, h->cfg.dtype, h->gqa_heads, h->gqa_dim, h->cfg.page_tokens,
+                                   h->cfg.n_pages, h->stage_dev + tp_at, h->stage_dev + tp_at + n_tp, (uint32_t)n_tp, h->bounds,
+                                   h->bound_scales, h->stream);
     h->n_bt_pairs = h->n_len_pairs = 0;
     return rc;
+}
+
+static int flush(ct_kv_paged_t *h, const int32_t *dest, uint32_t n_dest, const void *entries, uint32_t src_dtype,
+                 const proj_args_t *pj) {
+    return flush_all(h, dest, n_dest, entries, src_dtype, pj, NULL, NULL);
 }
 
 static int push_len(ct_kv_paged_t *h, uint32_t s) {
@@ -369,10 +448,44 @@ static int push_len(ct_kv_paged_t *h, uint32_t s) {
 
 /* ---- append --------------------------------------------------------------- */
 
+/* The mapped pages that hold positions [from[i], len) of sequence seq_ids[i],
+ * and their tokens; pages and counts are one malloc (freed by the caller). */
+static int touched_pages(const ct_kv_paged_t *h, const uint32_t *seq_ids, const uint32_t *from, uint32_t n, touched_t *tp,
+                         int32_t **mem) {
+    const uint32_t P = h->cfg.page_tokens, MP = h->cfg.max_pages_per_seq;
+    size_t cap = 0;
+    for (uint32_t i = 0; i < n; i++)
+        if (h->len[seq_ids[i]] > from[i]) cap += (h->len[seq_ids[i]] - 1) / P - from[i] / P + 1;
+    int32_t *m = (int32_t *)malloc((cap ? cap : 1) * 2 * sizeof(int32_t));
+    if (!m || cap > 0x7FFFFFFFu) { free(m); return CT_ERR_NOMEM; }
+    uint32_t at = 0;
+    for (uint32_t i = 0; i < n; i++) {
+        const uint32_t s = seq_ids[i], len = h->len[s];
+        if (len <= from[i]) continue;
+        for (uint32_t lp = from[i] / P; lp <= (len - 1) / P; lp++) {
+            const int32_t ph = h->bt[(size_t)s * MP + lp];
+            if (ph < 0) continue;
+            m[at] = ph;
+            m[cap + at++] = (int32_t)(len - lp * P < P ? len - lp * P : P);
+        }
+    }
+    *tp = (touched_t){m, m + cap, at};
+    *mem = m;
+    return CT_OK;
+}
+
 static int append_impl(ct_kv_paged_t *h, const uint32_t *seq_ids, const uint32_t *counts, uint32_t n,
-                       const void *entries, uint32_t src_dtype, const proj_args_t *pj) {
+                       const void *entries, uint32_t src_dtype, const proj_args_t *pj, const kv_args_t *kv) {
     if (!h || (n && (!seq_ids || !counts))) return CT_ERR_ARG;
-    if (pj && h->host_only) return CT_ERR_UNSUPPORTED;
+    if ((pj || kv) && h->host_only) return CT_ERR_UNSUPPORTED;
+    if (pj && h->gqa_heads) return CT_ERR_UNSUPPORTED;
+    const size_t src_elt = src_dtype == CT_KV_F32 ? 4 : 2;
+    const kv_args_t whole = {entries, (const uint8_t *)entries + (size_t)h->gqa_heads * h->gqa_dim * src_elt,
+                             h->cfg.entry_dim, h->cfg.entry_dim};
+    if (h->gqa_heads && entries && !kv) {             /* an entry is K of all heads, then V */
+        if (((uintptr_t)entries & 15) != 0) { ct__set_error("append: entries are not 16-byte aligned"); return CT_ERR_ARG; }
+        kv = &whole;
+    }
     if (entries && h->host_only) return CT_ERR_UNSUPPORTED;
     if (entries && src_dtype != CT_KV_BF16 && src_dtype != CT_KV_F32) return CT_ERR_ARG;
     const uint32_t P = h->cfg.page_tokens, MP = h->cfg.max_pages_per_seq, W = h->cfg.window_tokens;
@@ -387,8 +500,9 @@ static int append_impl(ct_kv_paged_t *h, const uint32_t *seq_ids, const uint32_t
     int rc = CT_OK;
     size_t *off = (size_t *)malloc((n ? n : 1) * sizeof(size_t));
     int32_t *dest = (int32_t *)malloc((total ? total : 1) * sizeof(int32_t));
-    if (!off || !dest) { free(off); free(dest); return CT_ERR_NOMEM; }
-    for (uint32_t i = 0, acc = 0; i < n; i++) { off[i] = acc; acc += counts[i]; }
+    uint32_t *from = (uint32_t *)malloc((n ? n : 1) * sizeof(uint32_t));
+    if (!off || !dest || !from) { free(off); free(dest); free(from); return CT_ERR_NOMEM; }
+    for (uint32_t i = 0, acc = 0; i < n; i++) { off[i] = acc; acc += counts[i]; from[i] = h->len[seq_ids[i]]; }
     h->n_bt_pairs = h->n_len_pairs = 0;
 
     for (uint32_t k = 0; k < maxc && rc == CT_OK; k++) {
@@ -455,17 +569,39 @@ static int append_impl(ct_kv_paged_t *h, const uint32_t *seq_ids, const uint32_t
          * mirrors stay consistent, but write no token data. */
         flush(h, NULL, 0, NULL, 0, NULL);
         free(dest);
+        free(from);
         return rc;
     }
+    touched_t tp = {NULL, NULL, 0};
+    int32_t *tp_mem = NULL;
+    if (kv && h->bounds) rc = touched_pages(h, seq_ids, from, n, &tp, &tp_mem);
     /* Without entries only the tables change: the slots need not travel. */
-    rc = flush(h, dest, entries || pj ? (uint32_t)total : 0u, entries, src_dtype, pj);
+    const int rc2 = flush_all(h, dest, !rc && (entries || pj || kv) ? (uint32_t)total : 0u, entries, src_dtype, pj, kv, &tp);
+    free(tp_mem);
     free(dest);
-    return rc;
+    free(from);
+    return rc ? rc : rc2;
 }
 
 int ct_kv_paged_append(ct_kv_paged_t *h, const uint32_t *seq_ids, const uint32_t *counts, uint32_t n,
                        const void *entries, uint32_t src_dtype) {
-    return append_impl(h, seq_ids, counts, n, entries, src_dtype, NULL);
+    return append_impl(h, seq_ids, counts, n, entries, src_dtype, NULL, NULL);
+}
+
+int ct_kv_paged_append_kv(ct_kv_paged_t *h, const uint32_t *seq_ids, const uint32_t *counts, uint32_t n, const void *k,
+                          const void *v, uint64_t k_stride, uint64_t v_stride, uint32_t src_dtype) {
+    if (!h || !k != !v) return CT_ERR_ARG;
+    if (!h->gqa_heads) return CT_ERR_UNSUPPORTED;
+    if (!k) return append_impl(h, seq_ids, counts, n, NULL, 0, NULL, NULL);
+    const uint64_t width = (uint64_t)h->gqa_heads * h->gqa_dim, unit = src_dtype == CT_KV_F32 ? 4 : 8;
+    kv_args_t kv = {k, v, k_stride ? k_stride : width, v_stride ? v_stride : width};
+    if (src_dtype != CT_KV_BF16 && src_dtype != CT_KV_F32) return CT_ERR_ARG;
+    if ((((uintptr_t)k | (uintptr_t)v) & 15) != 0 || kv.k_stride < width || kv.v_stride < width || kv.k_stride % unit ||
+        kv.v_stride % unit) {
+        ct__set_error("ct_kv_paged_append_kv: alignment or stride");
+        return CT_ERR_ARG;
+    }
+    return append_impl(h, seq_ids, counts, n, NULL, src_dtype, NULL, &kv);
 }
 
 int ct_kv_paged_append_projected(ct_kv_paged_t *h, const uint32_t *seq_ids, const uint32_t *counts, uint32_t n,
@@ -473,7 +609,7 @@ int ct_kv_paged_append_projected(ct_kv_paged_t *h, const uint32_t *seq_ids, cons
                                  uint32_t norm_dim) {
     if (!x || !w) return CT_ERR_ARG;
     const proj_args_t pj = {x, w, norm_w, eps, norm_dim, n_in};
-    return append_impl(h, seq_ids, counts, n, NULL, 0, &pj);
+    return append_impl(h, seq_ids, counts, n, NULL, 0, &pj, NULL);
 }
 
 int ct_kv_paged_free_seq(ct_kv_paged_t *h, uint32_t s) {
@@ -569,6 +705,20 @@ int ct_kv_paged_fork(ct_kv_paged_t *h, uint32_t src, uint32_t dst, uint32_t n_to
     h->last_access[dst] = h->st.clock++;
     if ((rc = push_len(h, dst))) return rc;
     h->st.n_pages_free = h->heap_n;
+    if (!h->host_only && copy_to >= 0 && h->gqa_heads) {   /* the same, of each K and V head's run of slots */
+        const size_t row = h->page_bytes / P / h->scale_rows, runs = h->scale_rows;
+        rc = ct__cuda_status(cudaMemcpy2DAsync((uint8_t *)h->pool + (size_t)copy_to * h->page_bytes, P * row,
+                                               (const uint8_t *)h->pool + (size_t)copy_from * h->page_bytes, P * row, rem * row,
+                                               runs, cudaMemcpyDeviceToDevice, h->stream), "fork copy");
+        if (!rc && h->scales)
+            rc = ct__cuda_status(cudaMemcpy2DAsync(h->scales + (size_t)copy_to * P * runs, P * sizeof(float),
+                                                   h->scales + (size_t)copy_from * P * runs, P * sizeof(float),
+                                                   rem * sizeof(float), runs, cudaMemcpyDeviceToDevice, h->stream), "fork copy");
+        if (rc) return rc;
+        const int32_t count = (int32_t)rem;
+        const touched_t tp = {&copy_to, &count, 1};
+        return flush_all(h, NULL, 0, NULL, 0, NULL, NULL, &tp);
+    }
     if (!h->host_only && copy_to >= 0) {             /* first rem slots of the page, and their scales */
         const size_t tok_bytes = h->page_bytes / P;
         rc = ct__cuda_status(cudaMemcpyAsync((uint8_t *)h->pool + (size_t)copy_to * h->page_bytes,
@@ -655,31 +805,52 @@ int ct_kv_paged_compact(ct_kv_paged_t *h) {
     free(refc2);
     if (h->host_only) goto renumbered;
     void *new_pool = NULL;
-    float *new_scales = NULL;
+    float *new_scales = NULL, *new_bscales = NULL;
+    int8_t *new_bounds = NULL;
+    const size_t sc_row = (size_t)P * h->scale_rows;  /* scales of a page */
+    const size_t b_page = (size_t)h->gqa_heads * 2 * h->gqa_dim;
     /* stream-ordered allocations: after the first compaction the pool's
      * memory comes back from the driver's cache without a device sync */
     rc = ct__cuda_status(cudaMallocAsync(&new_pool, (size_t)NP * h->page_bytes, h->stream), "compact pool");
     if (!rc && h->scales)
-        rc = ct__cuda_status(cudaMallocAsync((void **)&new_scales, (size_t)NP * P * sizeof(float), h->stream),
+        rc = ct__cuda_status(cudaMallocAsync((void **)&new_scales, (size_t)NP * sc_row * sizeof(float), h->stream),
                              "compact scales");
-    if (!rc && new_scales) rc = ct__cuda_status(cudaMemsetAsync(new_scales, 0, (size_t)NP * P * sizeof(float), h->stream), "compact");
+    if (!rc && new_scales) rc = ct__cuda_status(cudaMemsetAsync(new_scales, 0, (size_t)NP * sc_row * sizeof(float), h->stream), "compact");
+    if (!rc && h->bounds) {
+        rc = ct__cuda_status(cudaMallocAsync((void **)&new_bounds, (size_t)NP * b_page, h->stream), "compact bounds");
+        if (!rc)
+            rc = ct__cuda_status(cudaMallocAsync((void **)&new_bscales, (size_t)NP * h->gqa_heads * sizeof(float), h->stream),
+                                 "compact bounds");
+    }
     /* bt image follows the map in the staging buffer */
     memcpy(map + n_live, h->bt, (size_t)S * MP * sizeof(int32_t));
     if (!rc) rc = ct__cuda_status(cudaMemcpyAsync(h->stage_dev, map, ((size_t)n_live + (size_t)S * MP) * sizeof(int32_t),
                                                   cudaMemcpyHostToDevice, h->stream), "compact upload");
-    if (!rc) rc = ct_kv_paged_move_pages(h->pool, h->scales, new_pool, new_scales, h->stage_dev, n_live,
-                                         h->page_bytes, P, h->stream);
+    if (!rc && !h->gqa_heads)
+        rc = ct_kv_paged_move_pages(h->pool, h->scales, new_pool, new_scales, h->stage_dev, n_live, h->page_bytes, P, h->stream);
+    if (!rc && h->gqa_heads) {                        /* a page's scales and bounds are byte runs of their own */
+        rc = ct_kv_paged_move_pages(h->pool, NULL, new_pool, NULL, h->stage_dev, n_live, h->page_bytes, P, h->stream);
+        if (!rc && h->scales)
+            rc = ct_kv_paged_move_pages(h->scales, NULL, new_scales, NULL, h->stage_dev, n_live, sc_row * sizeof(float), P,
+                                        h->stream);
+        if (!rc && h->bounds)
+            rc = ct_kv_paged_move_pages(h->bounds, h->bound_scales, new_bounds, new_bscales, h->stage_dev, n_live, b_page,
+                                        h->gqa_heads, h->stream);
+    }
     if (!rc) rc = ct__cuda_status(cudaMemcpyAsync(h->bt_dev, h->stage_dev + n_live, (size_t)S * MP * sizeof(int32_t),
                                                   cudaMemcpyDeviceToDevice, h->stream), "compact bt");
     if (rc) {
         if (new_pool) cudaFreeAsync(new_pool, h->stream);
         if (new_scales) cudaFreeAsync(new_scales, h->stream);
+        if (new_bounds) cudaFreeAsync(new_bounds, h->stream);
+        if (new_bscales) cudaFreeAsync(new_bscales, h->stream);
         cudaStreamSynchronize(h->stream);
         return rc;
     }
     if (h->pool_async) {                          /* from an earlier compaction: back to the cache */
         cudaFreeAsync(h->pool, h->stream);
         if (h->scales) cudaFreeAsync(h->scales, h->stream);
+        if (h->bounds) { cudaFreeAsync(h->bounds, h->stream); cudaFreeAsync(h->bound_scales, h->stream); }
     }
     /* the staging buffer is reused by the next call on the host */
     rc = ct__cuda_status(cudaStreamSynchronize(h->stream), "compact sync");
@@ -687,10 +858,14 @@ int ct_kv_paged_compact(ct_kv_paged_t *h) {
     if (!h->pool_async) {                         /* the create-time buffers */
         cudaFree(h->pool);
         cudaFree(h->scales);
+        cudaFree(h->bounds);
+        cudaFree(h->bound_scales);
     }
     h->pool_async = 1;
     h->pool = new_pool;
     h->scales = new_scales;
+    h->bounds = new_bounds;
+    h->bound_scales = new_bscales;
 renumbered:
     /* Free pages are now n_live..NP-1, handed out in ascending order. */
     for (uint32_t p = 0; p < NP; p++) h->rank[p] = p;
@@ -704,12 +879,60 @@ renumbered:
 
 /* ---- reads ------------------------------------------------------------------ */
 
+/* Ranges of a grouped-query cache, K and V rows k_stride / v_stride values
+ * apart: the tokens' slots are looked up here and staged. */
+static int gather_kv(ct_kv_paged_t *h, const uint32_t *seqs, const uint32_t *starts, const uint32_t *counts, uint32_t n,
+                     void *k, void *v, uint64_t k_stride, uint64_t v_stride, uint32_t out_dtype) {
+    const uint32_t P = h->cfg.page_tokens, MP = h->cfg.max_pages_per_seq;
+    if ((((uintptr_t)k | (uintptr_t)v) & 15) != 0) { ct__set_error("gather: rows are not 16-byte aligned"); return CT_ERR_ARG; }
+    size_t total = 0;
+    for (uint32_t i = 0; i < n; i++) {
+        if (seqs[i] >= h->cfg.n_seqs || (uint64_t)starts[i] + counts[i] > h->len[seqs[i]]) return CT_ERR_ARG;
+        total += counts[i];
+        if (counts[i] == 0) continue;
+        for (uint32_t lp = starts[i] / P; lp <= (starts[i] + counts[i] - 1) / P; lp++)
+            if (h->bt[(size_t)seqs[i] * MP + lp] < 0) return CT_ERR_UNMAPPED;
+    }
+    if (total == 0) return CT_OK;
+    if (total > 0x7FFFFFFFu) return CT_ERR_ARG;
+    int rc = stage_reserve(h, total);
+    if (rc) return rc;
+    size_t at = 0;
+    for (uint32_t i = 0; i < n; i++)
+        for (uint32_t t = starts[i]; t < starts[i] + counts[i]; t++)
+            h->stage_host[at++] = h->bt[(size_t)seqs[i] * MP + t / P] * (int32_t)P + (int32_t)(t % P);
+    rc = ct__cuda_status(cudaMemcpyAsync(h->stage_dev, h->stage_host, total * sizeof(int32_t), cudaMemcpyHostToDevice,
+                                         h->stream), "gather upload");
+    if (!rc) rc = ct__cuda_status(cudaEventRecord(h->stage_ev, h->stream), "gather event");
+    if (rc) return rc;
+    h->stage_pending = 1;
+    return ct__launch_gqa_read(h->pool, h->scales, h->cfg.dtype, h->gqa_heads, h->gqa_dim, P, h->cfg.n_pages, h->stage_dev,
+                               (uint32_t)total, k, v, k_stride, v_stride, out_dtype == CT_KV_F32, h->stream);
+}
+
+/* The same into rows [K of all heads | V of all heads]. */
+static int gather_entries(ct_kv_paged_t *h, const uint32_t *seqs, const uint32_t *starts, const uint32_t *counts, uint32_t n,
+                          void *out, uint32_t out_dtype) {
+    const size_t half = (size_t)h->gqa_heads * h->gqa_dim * (out_dtype == CT_KV_F32 ? 4 : 2);
+    return gather_kv(h, seqs, starts, counts, n, out, (uint8_t *)out + half, h->cfg.entry_dim, h->cfg.entry_dim, out_dtype);
+}
+
+int ct_kv_paged_gather_kv(ct_kv_paged_t *h, const uint32_t *seqs, const uint32_t *starts, const uint32_t *counts, uint32_t n,
+                          void *k_out, void *v_out, uint32_t out_dtype) {
+    if (!h || (n && (!seqs || !starts || !counts || !k_out || !v_out))) return CT_ERR_ARG;
+    if (!h->gqa_heads || h->host_only) return CT_ERR_UNSUPPORTED;
+    if (out_dtype != CT_KV_BF16 && out_dtype != CT_KV_F32) return CT_ERR_ARG;
+    const uint64_t width = (uint64_t)h->gqa_heads * h->gqa_dim;
+    return gather_kv(h, seqs, starts, counts, n, k_out, v_out, width, width, out_dtype);
+}
+
 int ct_kv_paged_gather(ct_kv_paged_t *h, uint32_t seq, uint32_t start, uint32_t n, void *out, uint32_t out_dtype) {
     if (!h || !out || seq >= h->cfg.n_seqs) return CT_ERR_ARG;
     if (h->host_only) return CT_ERR_UNSUPPORTED;
     if (out_dtype != CT_KV_BF16 && out_dtype != CT_KV_F32) return CT_ERR_ARG;
     if ((uint64_t)start + n > h->len[seq]) return CT_ERR_ARG;
     if (n == 0) return CT_OK;
+    if (h->gqa_heads) return gather_entries(h, &seq, &start, &n, 1, out, out_dtype);
     const uint32_t P = h->cfg.page_tokens;
     for (uint32_t lp = start / P; lp <= (start + n - 1) / P; lp++)
         if (h->bt[(size_t)seq * h->cfg.max_pages_per_seq + lp] < 0) return CT_ERR_UNMAPPED;
@@ -722,6 +945,7 @@ int ct_kv_paged_gather_batch(ct_kv_paged_t *h, const uint32_t *seqs, const uint3
     if (!h || (n && (!seqs || !starts || !counts || !out))) return CT_ERR_ARG;
     if (h->host_only) return CT_ERR_UNSUPPORTED;
     if (out_dtype != CT_KV_BF16 && out_dtype != CT_KV_F32) return CT_ERR_ARG;
+    if (h->gqa_heads) return gather_entries(h, seqs, starts, counts, n, out, out_dtype);
     const uint32_t P = h->cfg.page_tokens, MP = h->cfg.max_pages_per_seq;
     for (uint32_t i = 0; i < n; i++) {
         if (seqs[i] >= h->cfg.n_seqs || (uint64_t)starts[i] + counts[i] > h->len[seqs[i]]) return CT_ERR_ARG;
@@ -809,10 +1033,14 @@ const int32_t *ct_kv_paged_seq_lens_dev(const ct_kv_paged_t *h) { return h ? h->
  * count, 5 x u32 each); the live pages (u32 count, then per page its id (i32),
  * page bytes, and page_tokens fp32 scales for int8 / e4m3 pools); version 2
  * then the token ids (per sequence a u32 count and that many i32); last an
- * FNV-1a 64 of everything before it.  Version 1 files (no token ids) load. */
+ * FNV-1a 64 of everything before it.  Version 1 files (no token ids) load.
+ * Grouped-query caches are version 3: after the config words n_kv_heads,
+ * head_dim and whether bounds are kept (3 x u32), and 2 x n_kv_heads scales
+ * a token; the bounds are made again from the pages. */
 
 #define CKPT_MAGIC "CTKVPAGE"
 #define CKPT_VERSION 2u
+#define CKPT_VERSION_GQA 3u
 
 typedef struct {
     FILE *f;
@@ -845,13 +1073,15 @@ int ct_kv_paged_save(ct_kv_paged_t *h, const char *path) {
     FILE *f = fopen(path, "wb");
     if (!f) { ct__set_error("ct_kv_paged_save: cannot open the file"); return CT_ERR_IO; }
     ckpt_io_t io = {f, 0xCBF29CE484222325ull, 0};
-    const uint32_t ver = CKPT_VERSION, flags = h->host_only ? 0u : 1u;
+    const uint32_t ver = h->gqa_heads ? CKPT_VERSION_GQA : CKPT_VERSION, flags = h->host_only ? 0u : 1u;
     ck_write(&io, CKPT_MAGIC, 8);
     ck_write(&io, &ver, 4);
     ck_write(&io, &flags, 4);
     const uint32_t cfgw[8] = {h->cfg.n_seqs, h->cfg.max_pages_per_seq, h->cfg.n_pages, h->cfg.page_tokens,
                               h->cfg.entry_dim, h->cfg.window_tokens, h->cfg.dtype, (uint32_t)h->cfg.device};
     ck_write(&io, cfgw, sizeof cfgw);
+    const uint32_t gqaw[3] = {h->gqa_heads, h->gqa_dim, h->bounds != NULL};
+    if (h->gqa_heads) ck_write(&io, gqaw, sizeof gqaw);
     const uint64_t st64[5] = {h->st.n_appends, h->st.n_evict_window, h->st.n_evict_lru, h->st.n_compactions,
                               h->st.bytes_compacted};
     const uint32_t st32[2] = {h->st.n_pages_live, h->st.n_pages_free};
@@ -881,7 +1111,7 @@ int ct_kv_paged_save(ct_kv_paged_t *h, const char *path) {
     ck_write(&io, &n_live, 4);
     int rc = CT_OK;
     if (!h->host_only && n_live) {
-        const size_t sc_bytes = h->scales ? (size_t)P * sizeof(float) : 0;
+        const size_t sc_bytes = h->scales ? (size_t)P * h->scale_rows * sizeof(float) : 0;
         uint8_t *buf = (uint8_t *)malloc(h->page_bytes + sc_bytes);
         if (!buf) { free(seen); fclose(f); return CT_ERR_NOMEM; }
         for (size_t i = 0; i < (size_t)S * MP && !rc && !io.err; i++) {
@@ -891,7 +1121,7 @@ int ct_kv_paged_save(ct_kv_paged_t *h, const char *path) {
             rc = ct__cuda_status(cudaMemcpy(buf, (const uint8_t *)h->pool + (size_t)pg * h->page_bytes,
                                             h->page_bytes, cudaMemcpyDeviceToHost), "ct_kv_paged_save page");
             if (!rc && sc_bytes)
-                rc = ct__cuda_status(cudaMemcpy(buf + h->page_bytes, h->scales + (size_t)pg * P, sc_bytes,
+                rc = ct__cuda_status(cudaMemcpy(buf + h->page_bytes, h->scales + (size_t)pg * P * h->scale_rows, sc_bytes,
                                                 cudaMemcpyDeviceToHost), "ct_kv_paged_save scales");
             ck_write(&io, &pg, 4);
             ck_write(&io, buf, h->page_bytes + sc_bytes);
@@ -922,18 +1152,21 @@ ct_kv_paged_t *ct_kv_paged_load(const char *path, int device) {
     ck_read(&io, &ver, 4);
     ck_read(&io, &flags, 4);
     ck_read(&io, cfgw, sizeof cfgw);
-    if (io.err || memcmp(magic, CKPT_MAGIC, 8) != 0 || ver < 1 || ver > CKPT_VERSION) {
+    if (io.err || memcmp(magic, CKPT_MAGIC, 8) != 0 || ver < 1 || ver > CKPT_VERSION_GQA) {
         fclose(f);
-        ct__set_error("ct_kv_paged_load: not a paged KV checkpoint of version 1 or 2");
+        ct__set_error("ct_kv_paged_load: not a paged KV checkpoint of version 1, 2 or 3");
         return NULL;
     }
+    uint32_t gqaw[3] = {0, 0, 0};
+    if (ver == CKPT_VERSION_GQA) ck_read(&io, gqaw, sizeof gqaw);
     ct_kv_paged_config_t cfg = {cfgw[0], cfgw[1], cfgw[2], cfgw[3], cfgw[4], cfgw[5], cfgw[6], device};
     if ((flags & 1u) == 0 && device >= 0) {
         fclose(f);
         ct__set_error("ct_kv_paged_load: the checkpoint holds tables only (load it with device -1)");
         return NULL;
     }
-    ct_kv_paged_t *h = ct_kv_paged_create(&cfg);
+    ct_kv_paged_t *h = io.err ? NULL : ver == CKPT_VERSION_GQA ? ct_kv_paged_create_gqa(&cfg, gqaw[0], gqaw[1], gqaw[2] != 0)
+                                                               : ct_kv_paged_create(&cfg);
     if (!h) { fclose(f); return NULL; }
     const uint32_t S = h->cfg.n_seqs, MP = h->cfg.max_pages_per_seq, NP = h->cfg.n_pages, P = h->cfg.page_tokens;
     uint64_t st64[5];
@@ -1005,7 +1238,7 @@ ct_kv_paged_t *ct_kv_paged_load(const char *path, int device) {
         bad = io.err || n_live > NP;
     }
     if (!bad && (flags & 1u) && n_live) {
-        const size_t sc_bytes = h->scales ? (size_t)P * sizeof(float) : 0;
+        const size_t sc_bytes = h->scales ? (size_t)P * h->scale_rows * sizeof(float) : 0;
         uint8_t *buf = (uint8_t *)malloc(h->page_bytes + sc_bytes);
         bad = !buf;
         for (uint32_t i = 0; i < n_live && !bad; i++) {
@@ -1017,7 +1250,7 @@ ct_kv_paged_t *ct_kv_paged_load(const char *path, int device) {
                 bad = ct__cuda_status(cudaMemcpy((uint8_t *)h->pool + (size_t)pg * h->page_bytes, buf, h->page_bytes,
                                                  cudaMemcpyHostToDevice), "ct_kv_paged_load page") != CT_OK;
                 if (!bad && sc_bytes)
-                    bad = ct__cuda_status(cudaMemcpy(h->scales + (size_t)pg * P, buf + h->page_bytes, sc_bytes,
+                    bad = ct__cuda_status(cudaMemcpy(h->scales + (size_t)pg * P * h->scale_rows, buf + h->page_bytes, sc_bytes,
                                                      cudaMemcpyHostToDevice), "ct_kv_paged_load scales") != CT_OK;
             }
         }
@@ -1051,6 +1284,15 @@ ct_kv_paged_t *ct_kv_paged_load(const char *path, int device) {
                   ct__cuda_status(cudaMemcpy(h->len_dev, len32, (size_t)S * 4, cudaMemcpyHostToDevice), "load len");
             free(len32);
         }
+    }
+    if (!bad && h->bounds) {                           /* the bounds of every mapped page */
+        uint32_t *all = (uint32_t *)malloc((size_t)S * 4), *from = (uint32_t *)calloc(S, 4);
+        touched_t tp;
+        int32_t *mem = NULL;
+        for (uint32_t i = 0; all && i < S; i++) all[i] = i;
+        bad = !all || !from || touched_pages(h, all, from, S, &tp, &mem) != CT_OK ||
+              flush_all(h, NULL, 0, NULL, 0, NULL, NULL, &tp) != CT_OK;
+        free(all); free(from); free(mem);
     }
     if (bad) { ct_kv_paged_destroy(h); return NULL; }
     return h;

@@ -18,6 +18,8 @@
 #include <stddef.h>
 #include <stdint.h>
 
+#include "kv_cache.h"
+
 #ifdef __cplusplus
 extern "C" {
 #endif
@@ -172,6 +174,71 @@ int ct_attn_mla_decode_paged_noalloc(const ct_mla_shape_t *shape, const int32_t 
                                      uint32_t n_seq, const void *q, const void *pool,
                                      const float *scales, const int32_t *block_table,
                                      const int32_t *seq_lens, void *out, float *lse, void *stream);
+
+/* ---- paged grouped-query decode ----------------------------------------- */
+
+/* Which kv head query head h reads. */
+typedef enum {
+    CT_GQA_MODULO = 0,           /* h % n_kv_heads, as the engine (transformer.c:187) and ct_attn_decode_contig */
+    CT_GQA_BLOCKED = 1,          /* h / (n_q_heads / n_kv_heads) */
+} ct_gqa_head_order_t;
+
+/* Shape of one decode problem over a grouped-query cache (kv_cache.h). */
+typedef struct {
+    ct_kv_gqa_layout_t kv;
+    uint32_t n_q_heads;          /* a multiple of kv.n_kv_heads */
+    uint32_t window_tokens;      /* a sequence of length n attends tokens [n - window, n); 0: all of them */
+    uint32_t head_order;         /* ct_gqa_head_order_t */
+    float    scale;              /* 0 selects 1 / sqrt(head_dim) */
+} ct_gqa_shape_t;
+
+/* A plan holds the scratch of a batch of n_seq sequences on one device (the
+ * partial results of sequences that several SMs share); the work is split on
+ * the device from the current lengths inside each call, so one plan serves
+ * any lengths and a captured call any later ones.  Calls on one plan must not
+ * overlap on the device; different plans may.  NULL on a shape that no kernel
+ * takes (ct_hal_cuda_last_error() says which part). */
+typedef struct ct_gqa_plan ct_gqa_plan_t;
+ct_gqa_plan_t *ct_gqa_plan_create(const ct_gqa_shape_t *shape, uint32_t n_seq, int device);
+void           ct_gqa_plan_destroy(ct_gqa_plan_t *p);
+uint32_t       ct_gqa_plan_workers(const ct_gqa_plan_t *p);
+size_t         ct_gqa_plan_scratch_bytes(const ct_gqa_plan_t *p);
+
+/* out[s][h] = sum_t softmax_t(scale * q[s][h] . k_t) v_t over the tokens t of
+ * sequence s that the window keeps and whose page is mapped (block-table
+ * entries outside the pool are skipped, lengths are clamped to the table's
+ * row).  q: device bf16, head h of sequence s at q[s * q_stride + h *
+ * head_dim] (q_stride 0 selects n_q_heads x head_dim; a multiple of 8; q
+ * 16-byte aligned).  block_table: device [n_seq][max_pages_per_seq],
+ * seq_lens: device [n_seq].  out: device bf16 [n_seq][n_q_heads][head_dim],
+ * 8-byte aligned; lse (optional, device fp32 [n_seq][n_q_heads]): the
+ * natural-log softmax normaliser.  A sequence without tokens gives 0 and
+ * -inf.  Slots behind a sequence's end may hold anything. */
+int ct_attn_gqa_decode_paged(ct_gqa_plan_t *plan, const void *q, uint64_t q_stride, const void *pool, const float *scales,
+                             const int32_t *block_table, const int32_t *seq_lens, void *out, float *lse, void *stream);
+
+/* The pages a decode should attend, for each kv head: pages_out (device int32
+ * [n_seq][n_kv_heads][n_select]) receives the logical pages in ascending
+ * order, then -1.  Candidates are the mapped pages of the window; its first
+ * n_first and last n_last pages are always taken, the others by score, the
+ * largest first and the lower page on a tie:
+ *   score = max over the group's heads (float(sum_d max(c_d,0) hi_d + min(c_d,0) lo_d) * e) * s,
+ *   e = max|q| / 127,  c = rint(q / e),  hi, lo, s: the page's bounds,
+ * whole-number sums and single fp32 roundings, so the choice is the same on
+ * every run.  A score that is not a number counts as infinity.  n_first +
+ * n_last <= n_select; max_pages_per_seq at most 49152 (else
+ * CT_ERR_UNSUPPORTED). */
+int ct_attn_gqa_select_pages(ct_gqa_plan_t *plan, const void *q, uint64_t q_stride, const int8_t *bounds,
+                             const float *bound_scales, const int32_t *block_table, const int32_t *seq_lens, uint32_t n_select,
+                             uint32_t n_first, uint32_t n_last, int32_t *pages_out, void *stream);
+
+/* ct_attn_gqa_decode_paged over the listed pages only: pages as
+ * ct_attn_gqa_select_pages writes them, valid entries first (at most as many
+ * as the window has pages are read), each page once; -1 and pages outside
+ * the sequence are skipped. */
+int ct_attn_gqa_decode_selected(ct_gqa_plan_t *plan, const void *q, uint64_t q_stride, const void *pool, const float *scales,
+                                const int32_t *block_table, const int32_t *seq_lens, const int32_t *pages, uint32_t n_select,
+                                void *out, float *lse, void *stream);
 
 /* ======================================================================== */
 /* Part 3 -- the MLA-lite cache of ds4_forward.c on the device               */

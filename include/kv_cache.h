@@ -278,6 +278,79 @@ int ct_kv_project_write_slots(const void *x, const void *w, const float *norm_w,
  * clear != 0 resets it.  Synchronises with the device. */
 int ct_kv_project_error(int clear);
 
+/* ---- grouped-query caches: K and V per head ----------------------------- */
+
+/* A cache of a model whose tokens have K and V rows for each of n_kv_heads
+ * heads (the engine's transformer loop, transformer.c:183-214), paged:
+ *   pool    [n_pages][K, V][n_kv_heads][page_tokens][head_dim]
+ *   scales  [n_pages][K, V][n_kv_heads][page_tokens] fp32 (8-bit pools)
+ * so that a page of a head is contiguous.  kv_dtype CT_KV_BF16, CT_KV_INT8 or
+ * CT_KV_E4M3; 8-bit pools hold one scale per token, K or V, and head, with
+ * the arithmetic of the per-token codecs (quant.h): d = max|x| / 127 or / 448,
+ * code = floor(x (1/d) + 1/2) clamped to +-127, or e4m3(x (1/d)).  A row that
+ * holds a NaN or an infinity is stored with scale NaN (it reads back as NaN).
+ * n_kv_heads at most 256; head_dim 32, 64, 96, 128, 192 or 256; page_tokens a
+ * multiple of 16;
+ * n_pages x page_tokens and max_pages_per_seq x page_tokens below 2^31; pool
+ * and scales 16-byte aligned. */
+typedef struct {
+    uint32_t n_kv_heads;
+    uint32_t head_dim;
+    uint32_t page_tokens;        /* 0 selects 64 */
+    uint32_t kv_dtype;           /* ct_kv_dtype_t */
+    uint32_t n_pages;
+    uint32_t max_pages_per_seq;
+} ct_kv_gqa_layout_t;
+
+/* Writes K and V of n tokens to dest_slot[i] = page * page_tokens + slot
+ * (device int32; outside the pool skips the token; a slot given twice gets
+ * either token), converting / quantising.  Token i's K is k[i * k_stride]
+ * onwards, n_kv_heads x head_dim values of src_dtype (CT_KV_BF16 or
+ * CT_KV_F32), its V at v[i * v_stride]; a stride (in values) of 0 selects
+ * n_kv_heads x head_dim, so K and V may be columns of a fused projection.
+ * k, v and the strides in bytes: multiples of 16.  Runs on the current
+ * device, as the other calls without a handle. */
+int ct_kv_gqa_write_slots(const ct_kv_gqa_layout_t *layout, void *pool, float *scales, const void *k, const void *v,
+                          uint64_t k_stride, uint64_t v_stride, uint32_t src_dtype, const int32_t *dest_slot, uint32_t n,
+                          void *stream);
+/* The way back: row i of k_out / v_out (out_dtype CT_KV_BF16 or CT_KV_F32)
+ * from src_slot[i]; rows whose slot lies outside the pool stay as they were. */
+int ct_kv_gqa_read_slots(const ct_kv_gqa_layout_t *layout, const void *pool, const float *scales, const int32_t *src_slot,
+                         uint32_t n, void *k_out, void *v_out, uint64_t k_stride, uint64_t v_stride, uint32_t out_dtype,
+                         void *stream);
+/* Bounds of the keys of pages[i] (device int32; outside the pool skips), over
+ * the page's first counts[i] tokens, for ct_attn_gqa_select_pages:
+ *   bounds       int8 [n_pages][n_kv_heads][upper, lower][head_dim], 16-byte aligned
+ *   bound_scales fp32 [n_pages][n_kv_heads]
+ * hi_d / lo_d = the largest / smallest k_d, s = max(|hi|, |lo|) / 127, codes
+ * ceil(hi / s) and floor(lo / s).  A NaN or an infinity among the keys gives
+ * scale NaN (such a page is always chosen), no token scale 0. */
+int ct_kv_gqa_page_bounds(const ct_kv_gqa_layout_t *layout, const void *pool, const float *scales, const int32_t *pages,
+                          const int32_t *counts, uint32_t n, int8_t *bounds, float *bound_scales, void *stream);
+
+/* A paged cache handle of this layout: allocator, window, LRU, prefix
+ * sharing, compaction and checkpoints as above.  cfg->entry_dim 0 or
+ * 2 x n_kv_heads x head_dim; cfg->dtype as kv_dtype.  keep_bounds != 0 keeps
+ * every page's key bounds up to date.  ct_kv_paged_append takes entries
+ * [K of all heads | V of all heads], ct_kv_paged_gather and gather_batch give
+ * them back; ct_kv_paged_append_projected is CT_ERR_UNSUPPORTED. */
+ct_kv_paged_t *ct_kv_paged_create_gqa(const ct_kv_paged_config_t *cfg, uint32_t n_kv_heads, uint32_t head_dim, int keep_bounds);
+/* ct_kv_paged_append with K and V apart (device, as in
+ * ct_kv_gqa_write_slots, tokens ordered like `entries`).  With k and v NULL
+ * the slots are reserved; whoever writes them then refreshes the bounds. */
+int ct_kv_paged_append_kv(ct_kv_paged_t *h, const uint32_t *seq_ids, const uint32_t *counts, uint32_t n, const void *k,
+                          const void *v, uint64_t k_stride, uint64_t v_stride, uint32_t src_dtype);
+/* Tokens [starts[i], starts[i] + counts[i]) of sequence seqs[i], back to back
+ * in range order, K and V apart (contiguous rows of n_kv_heads x head_dim).
+ * CT_ERR_UNMAPPED if a page in a range is not mapped. */
+int ct_kv_paged_gather_kv(ct_kv_paged_t *h, const uint32_t *seqs, const uint32_t *starts, const uint32_t *counts, uint32_t n,
+                          void *k_out, void *v_out, uint32_t out_dtype);
+/* The handle's layout (CT_ERR_UNSUPPORTED for a handle of another kind), and
+ * its bounds on the device (NULL without keep_bounds). */
+int          ct_kv_paged_gqa_layout(const ct_kv_paged_t *h, ct_kv_gqa_layout_t *out);
+int8_t      *ct_kv_paged_bounds(ct_kv_paged_t *h);
+float       *ct_kv_paged_bound_scales(ct_kv_paged_t *h);
+
 /* Page-level gather: dst page i <- src page map[i] (device int32), whole
  * pages of page_bytes (codes) and page_tokens scales (if scales != NULL). */
 int ct_kv_paged_move_pages(const void *src_pool, const float *src_scales, void *dst_pool,
