@@ -29,6 +29,14 @@ typedef struct {
     uint32_t page_tokens, max_pages, n_pages, n_pick, window, blocked;
     uint32_t min_steps;          /* least steps a worker takes */
     float scale_log2;            /* scale x log2(e) */
+    uint32_t page_magic;         /* floor(2^32 / (page_tokens / 16)) + 1; 0 for pages of 16 */
+#ifdef __CUDACC__
+    /* Page of token v (below 2^31, page_tokens a multiple of 16 up to 512): a
+     * product instead of a division; exact while v / 16 < 2^32 / (page_tokens / 16). */
+    __device__ __forceinline__ uint32_t page_of(uint32_t v) const {
+        return page_magic ? __umulhi(v >> 4, page_magic) : v >> 4;
+    }
+#endif
 } ct_gqa_args_t;
 
 /* One selection launch. */
@@ -45,12 +53,12 @@ typedef struct {
 
 /* Whether a kernel exists for these, CTAs it runs on an SM of the current
  * device (0: none; also sets the kernel's shared-memory limit there). */
-int ct__gqa_decode_ctas(uint32_t dim, uint32_t dtype);
+int ct__gqa_decode_ctas(uint32_t dim, uint32_t dtype, uint32_t group);
 int ct__launch_gqa_decode(const ct_gqa_args_t *a, uint32_t dim, uint32_t dtype, uint32_t n_workers, void *stream);
 /* The same for one storage type (gqa_decode_<type>.cu). */
-int ct__gqa_ctas_bf16(uint32_t dim);
-int ct__gqa_ctas_int8(uint32_t dim);
-int ct__gqa_ctas_e4m3(uint32_t dim);
+int ct__gqa_ctas_bf16(uint32_t dim, uint32_t group);
+int ct__gqa_ctas_int8(uint32_t dim, uint32_t group);
+int ct__gqa_ctas_e4m3(uint32_t dim, uint32_t group);
 int ct__gqa_run_bf16(const ct_gqa_args_t *a, uint32_t dim, uint32_t n_workers, void *stream);
 int ct__gqa_run_int8(const ct_gqa_args_t *a, uint32_t dim, uint32_t n_workers, void *stream);
 int ct__gqa_run_e4m3(const ct_gqa_args_t *a, uint32_t dim, uint32_t n_workers, void *stream);

@@ -8,44 +8,47 @@
 
 namespace ct_gqa {
 
-template <int D, int DT> static int ctas() {
+template <int D, int DT, int HT> static int ctas() {
     using C = Cfg<D, DT>;
     int n = 0;
-    int rc = ct__cuda_status(cudaFuncSetAttribute(k_gqa_decode<D, DT>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kRing),
+    int rc = ct__cuda_status(cudaFuncSetAttribute(k_gqa_decode<D, DT, HT>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kRing),
                              "gqa decode");
     if (!rc)
-        rc = ct__cuda_status(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, k_gqa_decode<D, DT>, kThreads, C::kRing),
+        rc = ct__cuda_status(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, k_gqa_decode<D, DT, HT>, kThreads, C::kRing),
                              "gqa decode");
     return rc ? 0 : n;
 }
 
-template <int D, int DT> static int run(const ct_gqa_args_t *a, uint32_t n_workers, cudaStream_t st) {
-    k_gqa_decode<D, DT><<<n_workers, kThreads, Cfg<D, DT>::kRing, st>>>(*a);
+template <int D, int DT, int HT> static int run(const ct_gqa_args_t *a, uint32_t n_workers, cudaStream_t st) {
+    k_gqa_decode<D, DT, HT><<<n_workers, kThreads, Cfg<D, DT>::kRing, st>>>(*a);
     ct__count_launches(1);
     return ct__cuda_status(cudaGetLastError(), "gqa decode");
 }
 
-template <int DT> static int ctas_of(uint32_t dim) {
+/* Groups of up to 8 query heads take one column tile, larger ones two. */
+template <int DT> static int ctas_of(uint32_t dim, uint32_t group) {
+    const bool one = group <= 8;
     switch (dim) {
-        case 32: return ctas<32, DT>();
-        case 64: return ctas<64, DT>();
-        case 96: return ctas<96, DT>();
-        case 128: return ctas<128, DT>();
-        case 192: return ctas<192, DT>();
-        case 256: return ctas<256, DT>();
+        case 32: return one ? ctas<32, DT, 1>() : ctas<32, DT, 2>();
+        case 64: return one ? ctas<64, DT, 1>() : ctas<64, DT, 2>();
+        case 96: return one ? ctas<96, DT, 1>() : ctas<96, DT, 2>();
+        case 128: return one ? ctas<128, DT, 1>() : ctas<128, DT, 2>();
+        case 192: return one ? ctas<192, DT, 1>() : ctas<192, DT, 2>();
+        case 256: return one ? ctas<256, DT, 1>() : ctas<256, DT, 2>();
         default: return 0;
     }
 }
 
 template <int DT> static int run_of(const ct_gqa_args_t *a, uint32_t dim, uint32_t n_workers, void *stream) {
     cudaStream_t st = (cudaStream_t)stream;
+    const bool one = a->group <= 8;
     switch (dim) {
-        case 32: return run<32, DT>(a, n_workers, st);
-        case 64: return run<64, DT>(a, n_workers, st);
-        case 96: return run<96, DT>(a, n_workers, st);
-        case 128: return run<128, DT>(a, n_workers, st);
-        case 192: return run<192, DT>(a, n_workers, st);
-        case 256: return run<256, DT>(a, n_workers, st);
+        case 32: return one ? run<32, DT, 1>(a, n_workers, st) : run<32, DT, 2>(a, n_workers, st);
+        case 64: return one ? run<64, DT, 1>(a, n_workers, st) : run<64, DT, 2>(a, n_workers, st);
+        case 96: return one ? run<96, DT, 1>(a, n_workers, st) : run<96, DT, 2>(a, n_workers, st);
+        case 128: return one ? run<128, DT, 1>(a, n_workers, st) : run<128, DT, 2>(a, n_workers, st);
+        case 192: return one ? run<192, DT, 1>(a, n_workers, st) : run<192, DT, 2>(a, n_workers, st);
+        case 256: return one ? run<256, DT, 1>(a, n_workers, st) : run<256, DT, 2>(a, n_workers, st);
         default: return CT_ERR_UNSUPPORTED;
     }
 }

@@ -39,7 +39,7 @@ int ct__gqa_layout(const ct_kv_gqa_layout_t *in, ct_kv_gqa_layout_t *l) {
     *l = *in;
     if (l->page_tokens == 0) l->page_tokens = 64;
     if (l->n_kv_heads == 0 || l->n_kv_heads > 256u) return bad("gqa: n_kv_heads (1 .. 256)");
-    if (l->page_tokens % 16 != 0) return bad("gqa: page_tokens % 16 != 0");
+    if (l->page_tokens % 16 != 0 || l->page_tokens > 512) return bad("gqa: page_tokens is a multiple of 16, at most 512");
     if (l->n_pages == 0 || (uint64_t)l->n_pages * l->page_tokens > 0x7FFFFFFFu) return bad("gqa: n_pages x page_tokens");
     if ((uint64_t)l->max_pages_per_seq * l->page_tokens > 0x7FFFFFFFu) return bad("gqa: max_pages_per_seq x page_tokens");
     if (l->kv_dtype != CT_KV_BF16 && l->kv_dtype != CT_KV_INT8 && l->kv_dtype != CT_KV_E4M3) {
@@ -112,11 +112,11 @@ int ct_kv_gqa_page_bounds(const ct_kv_gqa_layout_t *layout, const void *pool, co
 
 /* ---- plans ---------------------------------------------------------------- */
 
-int ct__gqa_decode_ctas(uint32_t dim, uint32_t dtype) {
+int ct__gqa_decode_ctas(uint32_t dim, uint32_t dtype, uint32_t group) {
     switch (dtype) {
-        case CT_KV_BF16: return ct__gqa_ctas_bf16(dim);
-        case CT_KV_INT8: return ct__gqa_ctas_int8(dim);
-        case CT_KV_E4M3: return ct__gqa_ctas_e4m3(dim);
+        case CT_KV_BF16: return ct__gqa_ctas_bf16(dim, group);
+        case CT_KV_INT8: return ct__gqa_ctas_int8(dim, group);
+        case CT_KV_E4M3: return ct__gqa_ctas_e4m3(dim, group);
         default: return 0;
     }
 }
@@ -158,8 +158,10 @@ ct_gqa_plan_t *ct_gqa_plan_create(const ct_gqa_shape_t *shape, uint32_t n_seq, i
         ct__set_error("ct_gqa_plan_create: bad shape");
         return NULL;
     }
-    /* the kernel counts the batch's steps of 16 tokens or more in 32 bits */
-    if ((uint64_t)n_seq * ((uint64_t)l.max_pages_per_seq * l.page_tokens / 16 + 1) > 0xFFFFFFFFu ||
+    /* the kernel counts the batch's steps of 16 tokens or more, and the steps
+     * of a sequence's items, in 32 bits (5: an item's overhead, rounding) */
+    const uint64_t most = (uint64_t)l.max_pages_per_seq * l.page_tokens / 16 + 5;
+    if ((uint64_t)n_seq * most > 0xFFFFFFFFu || most * shape->n_q_heads > 0xFFFFFFFFu ||
         (uint64_t)n_seq * l.n_kv_heads > 0x7FFFFFFFu) {
         ct__set_error("ct_gqa_plan_create: too many sequences for their longest length");
         return NULL;
@@ -174,7 +176,7 @@ ct_gqa_plan_t *ct_gqa_plan_create(const ct_gqa_shape_t *shape, uint32_t n_seq, i
     int prev = 0;
     if (enter(device, &prev)) { free(p); return NULL; }
     int n_sms = 0, rc = ct__cuda_status(cudaDeviceGetAttribute(&n_sms, cudaDevAttrMultiProcessorCount, device), "gqa plan");
-    const int ctas = rc ? 0 : ct__gqa_decode_ctas(l.head_dim, l.kv_dtype);
+    const int ctas = rc ? 0 : ct__gqa_decode_ctas(l.head_dim, l.kv_dtype, shape->n_q_heads / l.n_kv_heads);
     if (!rc && ctas == 0) { ct__set_error("ct_gqa_plan_create: the decode kernel does not fit this device"); rc = CT_ERR_UNSUPPORTED; }
     if (!rc) rc = ct__gqa_select_prepare();
     if (!rc) {
@@ -213,6 +215,7 @@ static int decode(ct_gqa_plan_t *p, const void *q, uint64_t q_stride, const void
     if (!block_table || !seq_lens || !out || misaligned(out, 8)) return bad("gqa: table, lengths or out");
     if (p->n_seq == 0) return CT_OK;
     const uint32_t group = p->shape.n_q_heads / l->n_kv_heads;
+    const uint32_t page_groups = l->page_tokens / 16;
     const ct_gqa_args_t a = {
         .q = (const uint16_t *)q, .pool = pool, .scales = scales, .block_table = block_table, .seq_lens = seq_lens,
         .picked = pages, .out = (uint16_t *)out, .lse = lse, .part_o = p->part_o, .part_ml = p->part_ml,
@@ -221,6 +224,7 @@ static int decode(ct_gqa_plan_t *p, const void *q, uint64_t q_stride, const void
         .max_pages = l->max_pages_per_seq, .n_pages = l->n_pages, .n_pick = n_select, .window = p->shape.window_tokens,
         .blocked = p->shape.head_order == CT_GQA_BLOCKED, .min_steps = 8,
         .scale_log2 = p->shape.scale * 1.4426950408889634f,
+        .page_magic = page_groups == 1 ? 0u : (uint32_t)(0x100000000ull / page_groups) + 1u,
     };
     int prev = 0;
     if ((rc = enter(p->device, &prev))) return rc;

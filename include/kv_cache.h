@@ -290,7 +290,7 @@ int ct_kv_project_error(int clear);
  * code = floor(x (1/d) + 1/2) clamped to +-127, or e4m3(x (1/d)).  A row that
  * holds a NaN or an infinity is stored with scale NaN (it reads back as NaN).
  * n_kv_heads at most 256; head_dim 32, 64, 96, 128, 192 or 256; page_tokens a
- * multiple of 16;
+ * multiple of 16, at most 512;
  * n_pages x page_tokens and max_pages_per_seq x page_tokens below 2^31; pool
  * and scales 16-byte aligned. */
 typedef struct {

@@ -82,15 +82,19 @@ def attend(q, pool, scales, table, lens, dtype, hq, order, window=0, pages=None,
     return out, lse, weight, slack
 
 
-def check_attention(got, got_lse, ref, dim, n_tokens):
+def check_attention(got, got_lse, ref, dim, n_tokens, dtype):
     """|out - want| <= one rounding to bf16 + e * sum p |v|, with e the error that 32-bit scores, the exponential and
-    two-digit probabilities leave: a score is off by at most (dim + 4) roundings of its largest partial sum, 2^-23 each
-    (the products of bf16 values are exact), so each p by twice that relative to the sum; p as two bf16 digits is off by
-    2^-16, the exponential and the sums of the parts by 2^-18; the sum over n tokens adds n / 16 accumulations of 2^-24 a
-    warp, of values that may cancel, hence relative to sum p |v|."""
+    rounded weights leave: a score is off by at most (dim + 4) roundings of its largest partial sum, 2^-23 each
+    (the products of bf16 values are exact), so each p by twice that relative to the sum; bf16 pools take p as two bf16
+    digits, off by 2^-16; 8-bit pools take p times the V scale as one fp16 value, off by half a step, 2^-11 relative, so
+    by 2^-11 sum p |v| in all (and by 2^-25 where it is below 2^-14, in a unit where the largest weight of a step is 2^7
+    or more: 2^-32 n of that); the exponential and the sums of the parts are off by 2^-18; the sum over n tokens adds
+    n / 16 accumulations of 2^-24 a warp, of values that may cancel, hence relative to sum p |v|."""
     out, lse, weight, slack = ref
     score = (dim + 4) * 2.0 ** -23 * slack
     e = 2 * score + 2.0 ** -15 + n_tokens / 16 * 2.0 ** -23
+    if dtype != ct.CT_KV_BF16:
+        e = e + 2.0 ** -11
     err = (got.double() - out).abs()
     bound = BF16_HALF * (out.abs() + e[..., None] * weight) + e[..., None] * weight + 1e-38
     assert (err <= bound).all(), float((err - bound).max())

@@ -43,7 +43,7 @@ def decode(lens, heads, group, dim, page, dtype, order=MOD, window=0, seed=1, ho
     if check:
         ref = G.attend(qv.reshape(len(lens), hq, dim), pool, scales, table, lens, dtype, hq, order, window,
                        scale=scale or None)
-        G.check_attention(out, lse, ref, dim, max(max(lens), 1))
+        G.check_attention(out, lse, ref, dim, max(max(lens), 1), dtype)
     return out, lse, plan
 
 
@@ -153,7 +153,7 @@ def test_decode_values_of_very_different_size(dtype):
     plan.decode(q, pool, scales, table, torch.tensor([n], dtype=torch.int32, device="cuda"), out, lse, stream=stream())
     torch.cuda.synchronize()
     ref = G.attend(q, pool, scales, table, [n], dtype, 4, MOD, scale=2.0 ** -6)
-    G.check_attention(out, lse, ref, dim, n)
+    G.check_attention(out, lse, ref, dim, n, dtype)
 
 
 @pytest.mark.parametrize("dtype", [BF16, INT8])
@@ -183,7 +183,7 @@ def test_pool_beyond_32_bit_offsets():
     lse = torch.empty(1, 16, device="cuda")
     plan.decode(q, pool, None, pages, torch.tensor([180], dtype=torch.int32, device="cuda"), out, lse, stream=stream())
     torch.cuda.synchronize()
-    G.check_attention(out, lse, G.attend(q, pool, None, pages, [180], BF16, 16, MOD), dim, 180)
+    G.check_attention(out, lse, G.attend(q, pool, None, pages, [180], BF16, 16, MOD), dim, 180, BF16)
     rows = torch.randn(1, 2, heads * dim, generator=g, device="cuda").bfloat16()
     slot = torch.tensor([n_pages * page - 1], dtype=torch.int32, device="cuda")
     ct.gqa_write_slots(layout, pool, None, rows[:, 0], rows[:, 1], slot, 1, stream=stream())
@@ -403,7 +403,7 @@ def test_decode_selected(heads, group, dim, page, pick, window, dtype):
                          torch.from_numpy(pages).cuda(), pick, out, lse, stream=stream())
     torch.cuda.synchronize()
     ref = G.attend(q, pool, scales, table, lens, dtype, hq, MOD, window, pages=pages)
-    G.check_attention(out, lse, ref, dim, max(lens))
+    G.check_attention(out, lse, ref, dim, max(lens), dtype)
 
 
 def test_decode_selected_ignores_pages_outside_the_sequence():
@@ -419,7 +419,7 @@ def test_decode_selected_ignores_pages_outside_the_sequence():
     plan.decode_selected(q, pool, None, table, torch.tensor(lens, dtype=torch.int32, device="cuda"),
                          torch.from_numpy(pages).cuda(), 4, out, lse, stream=stream())
     torch.cuda.synchronize()
-    G.check_attention(out, lse, G.attend(q, pool, None, table, lens, BF16, 3, MOD, pages=pages), 64, 300)
+    G.check_attention(out, lse, G.attend(q, pool, None, table, lens, BF16, 3, MOD, pages=pages), 64, 300, BF16)
 
 
 # ---- the handle, and the operators together -----------------------------------------------------------------------------------
@@ -589,8 +589,9 @@ def test_serving_steps_append_select_decode(dtype):
         bs = dev_copy(kv.bound_scales, (NP, heads), torch.float32).cpu().numpy()
         want = G.select(q.float().cpu().numpy(), bounds, bs, tb.cpu().numpy(), lens, NP, page, hq, MOD, pick, 1, 1)
         assert np.array_equal(picked.cpu().numpy(), want)
-        G.check_attention(out_sel, lse_sel, G.attend(q, pool, scales, tb, lens, dtype, hq, MOD, pages=want), dim, max(lens))
-        G.check_attention(out, lse, G.attend(q, pool, scales, tb, lens, dtype, hq, MOD), dim, max(lens))
+        G.check_attention(out_sel, lse_sel, G.attend(q, pool, scales, tb, lens, dtype, hq, MOD, pages=want), dim, max(lens),
+                          dtype)
+        G.check_attention(out, lse, G.attend(q, pool, scales, tb, lens, dtype, hq, MOD), dim, max(lens), dtype)
 
 
 def test_two_plans_on_two_streams():
@@ -610,7 +611,7 @@ def test_two_plans_on_two_streams():
             plans[i].decode(q[i], pool, None, table, ld, outs[i], stream=streams[i].cuda_stream)
     torch.cuda.synchronize()
     for i in range(2):
-        G.check_attention(outs[i], None, G.attend(q[i], pool, None, table, lens, BF16, 8, MOD), 128, 5000)
+        G.check_attention(outs[i], None, G.attend(q[i], pool, None, table, lens, BF16, 8, MOD), 128, 5000, BF16)
 
 
 def test_results_do_not_change_from_run_to_run():
