@@ -25,14 +25,16 @@
  * down to 2^-29 of the head's largest value), and probability x V scale is
  * one fp16 digit (11 bits) of a running power-of-two unit; see `unit`.
  *
- * Split: the steps (TS tokens of an item = sequence x kv head x group of 16
- * heads) of the whole batch lie end to end, each item with kItemCost steps of
- * overhead, and each CTA takes an equal range, found from the device lengths
- * at entry, so no planning launch precedes the kernel.  An item of at most
- * kSolo steps is one warp's; the warps of a CTA share longer ones, each with
- * its own cp.async ring and its own (max, sum, out), joined through shared
- * memory; an item cut between CTAs leaves fp32 partials that the CTA
- * finishing last joins in index order.
+ * Split: an item is a (sequence, kv head, group of 16 heads); a step of it
+ * TS tokens.  The steps of the whole batch lie end to end, each item with
+ * kItemCost steps of overhead, and each CTA takes an equal range; when there
+ * are fewer than half as many items as CTAs, every CTA takes one part of one
+ * item instead.  Either is found from the device lengths at entry, so no
+ * planning launch precedes the kernel.  An item of a few steps is one warp's;
+ * the warps of a CTA share longer ones.  Each warp has its own ring of copies
+ * that runs ahead across its items, and its own (max, sum, out), joined
+ * through shared memory; an item cut between CTAs leaves fp32 partials that
+ * the CTA finishing last joins in index order.
  */
 #pragma once
 #include <math.h>
@@ -48,8 +50,11 @@ constexpr int kThreads = kWarps * 32;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr float kGrow = 8.0f;           /* log2 growth of a maximum that is followed */
+constexpr float kNoMax = -3.402823466e38f;  /* maximum of no tokens: finite, so that no difference of maxima is NaN */
+constexpr float kTopWeight = 32768.0f;  /* fp16 weights stay below this */
 constexpr uint32_t kItemCost = 4;       /* steps that an item's start and end are counted as */
-constexpr uint32_t kSolo = 8;           /* steps up to which an item is one warp's */
+constexpr uint32_t kSolo = 8;           /* steps up to which an item is one warp's, if the CTA has items for every warp */
+constexpr uint32_t kFan = 16;           /* workers whose parts are joined at a time, when an item has more than 2 kFan */
 
 /* Tokens of a warp's step (2 to 17 KB of K and V) and steps in the ring. */
 template <int D, int DT> struct Cfg {
@@ -61,6 +66,13 @@ template <int D, int DT> struct Cfg {
     static constexpr int kScaleBytes = DT == CT_KV_BF16 ? 0 : TS * 8;
     static constexpr int kStage = 2 * TS * kPitch + kScaleBytes;
     static constexpr int kRing = kWarps * kStages * kStage;
+    /* Queries as operands: in registers, or (2 D / 16 registers a tile would
+     * spill) in shared memory behind the ring, a copy for each warp, where an
+     * SM has the room (1 KB of its 227 is for the joins' statics). */
+    static constexpr int kQPitch = 2 * D + 16;
+    template <int HT> static constexpr int kQBytes = kWarps * HT * 8 * kQPitch;
+    template <int HT> static constexpr bool kQueriesInSmem = HT * D >= 192 && kRing + kQBytes<HT> <= 226 * 1024;
+    template <int HT> static constexpr int kSmem = kRing + (kQueriesInSmem<HT> ? kQBytes<HT> : 0);
 };
 
 CT_DEV uint32_t smem_u32(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
@@ -165,208 +177,297 @@ template <int TS> CT_DEV Seq sequence(const ct_gqa_args_t &a, uint32_t s) {
 template <int D, int DT, int HT>
 __global__ void __launch_bounds__(kThreads) k_gqa_decode(const ct_gqa_args_t a) {
     using C = Cfg<D, DT>;
-    constexpr int TS = C::TS, GR = TS / 16, kPitch = C::kPitch, KB = D / 16;
-    constexpr int kHeads = 8 * HT, kJoin = D + 4;            /* pitch of a head's sums: lanes' writes in distinct banks */
+    constexpr int TS = C::TS, GR = TS / 16, kPitch = C::kPitch, KB = D / 16, S = C::kStages;
+    constexpr int kHeads = 8 * HT;
     constexpr bool kQ8 = DT != CT_KV_BF16;
+    /* a segment's end: each warp leaves its [head][value] sums in the ring slot
+     * that it consumed last, all values at once or half of them at a time */
+    constexpr int kJoinCols = kHeads * (D + 4) * 4 <= C::kStage ? D : D / 2;
+    constexpr int kJoin = kJoinCols + 4;                     /* pitch: the lanes' writes fall in distinct banks */
+    static_assert(kHeads * kJoin * 4 <= C::kStage && kJoinCols % 16 == 0, "half the sums of a warp fit a slot");
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ uint32_t s_scan[kWarps];
-    __shared__ uint32_t s_seq;
-    __shared__ uint64_t s_first;
+    struct End { uint32_t ordinal, step, first, last; };     /* an end of the CTA's range; its item's first and last worker */
+    __shared__ End s_end[2];
     __shared__ float s_ml[kWarps][kHeads][2];
-    __shared__ uint32_t s_last;
+    __shared__ uint32_t s_free[kWarps], s_last;
     const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, j = lane & 3;
     const uint32_t HV = a.n_kv_heads * a.n_tiles;
 
-    /* ---- this CTA's range of steps ---- */
+    /* ---- this CTA's range of steps: from step s_end[0].step of item
+     * s_end[0].ordinal to before step s_end[1].step of s_end[1].ordinal ---- */
     const uint32_t per = (a.n_seq + kThreads - 1) / kThreads;
-    uint32_t sum = 0;
+    auto scan = [&](uint32_t v, uint32_t &all) -> uint32_t { /* exclusive sum over the threads */
+        uint32_t incl = v;
+        #pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const uint32_t y = __shfl_up_sync(0xFFFFFFFFu, incl, o);
+            if (lane >= (uint32_t)o) incl += y;
+        }
+        if (lane == 31) s_scan[warp] = incl;
+        __syncthreads();
+        uint32_t before = 0;
+        all = 0;
+        #pragma unroll
+        for (int w = 0; w < kWarps; w++) {
+            if (w < (int)warp) before += s_scan[w];
+            all += s_scan[w];
+        }
+        __syncthreads();
+        return before + incl - v;
+    };
+    const bool few = 2ull * a.n_seq * HV <= gridDim.x;       /* a part of one item each */
+    uint32_t sum = 0, all;
     for (uint32_t i = 0; i < per; i++) {
         const uint32_t s = tid * per + i;
-        if (s < a.n_seq) sum += sequence<TS>(a, s).steps + kItemCost;
+        if (s < a.n_seq) sum += sequence<TS>(a, s).steps + (few ? 0u : kItemCost);
     }
-    uint32_t incl = sum;
-    #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const uint32_t y = __shfl_up_sync(0xFFFFFFFFu, incl, o);
-        if (lane >= (uint32_t)o) incl += y;
-    }
-    if (lane == 31) s_scan[warp] = incl;
-    __syncthreads();
-    uint32_t total_seq = 0, before = 0;
-    #pragma unroll
-    for (int w = 0; w < kWarps; w++) {
-        if (w < (int)warp) before += s_scan[w];
-        total_seq += s_scan[w];
-    }
-    const uint32_t excl = before + incl - sum;
-    const uint64_t total = (uint64_t)total_seq * HV;
-    uint64_t Q = (total + gridDim.x - 1) / gridDim.x;
-    if (Q < a.min_steps) Q = a.min_steps;
-    uint64_t x = (uint64_t)blockIdx.x * Q;
-    if (x >= total) return;
-    const uint64_t x1 = x + Q < total ? x + Q : total;
-    if (x >= (uint64_t)excl * HV && x < (uint64_t)(excl + sum) * HV) {
-        uint32_t at = excl, s = tid * per;
-        for (;; s++) {
-            const uint32_t c = sequence<TS>(a, s).steps + kItemCost;
-            if (x < (uint64_t)(at + c) * HV) break;
-            at += c;
+    uint32_t excl = scan(sum, all);
+    if (few) {
+        const uint32_t workers = gridDim.x - a.n_seq * HV;
+        const uint32_t Q = max(a.min_steps, (uint32_t)(((uint64_t)all * HV + workers - 1) / workers));
+        sum = 0;
+        for (uint32_t i = 0; i < per; i++) {
+            const uint32_t s = tid * per + i;
+            if (s < a.n_seq) sum += (sequence<TS>(a, s).steps + Q - 1) / Q;
         }
-        s_seq = s;
-        s_first = (uint64_t)at * HV;
+        excl = scan(sum, all);                               /* parts of the sequences' items */
+        if (blockIdx.x >= all * HV) return;
+        if (blockIdx.x >= excl * HV && blockIdx.x < (excl + sum) * HV) {
+            uint32_t x = blockIdx.x - excl * HV, s = tid * per, steps, n;
+            for (;; s++) {
+                steps = sequence<TS>(a, s).steps;
+                n = (steps + Q - 1) / Q;
+                if (x < n * HV) break;
+                x -= n * HV;
+            }
+            const uint32_t item = x / n, part = x % n, first = blockIdx.x - part;
+            const End e = {s * HV + item, (uint32_t)((uint64_t)steps * part / n), first, first + n - 1};
+            s_end[0] = e;
+            s_end[1] = e;
+            s_end[1].step = (uint32_t)((uint64_t)steps * (part + 1) / n);
+        }
+    } else {
+        const uint64_t total = (uint64_t)all * HV;
+        const uint64_t Q = max((uint64_t)a.min_steps, (total + gridDim.x - 1) / gridDim.x);
+        const uint64_t x0 = (uint64_t)blockIdx.x * Q;
+        if (x0 >= total) return;
+        #pragma unroll 1
+        for (int b = 0; b < 2; b++) {                        /* the range's first and last unit */
+            const uint64_t x = b ? min(x0 + Q, total) - 1 : x0;
+            if (x < (uint64_t)excl * HV || x >= (uint64_t)(excl + sum) * HV) continue;
+            uint64_t at = (uint64_t)excl * HV;
+            uint32_t s = tid * per, width;
+            for (;; s++) {
+                width = sequence<TS>(a, s).steps + kItemCost;
+                if (x < at + (uint64_t)width * HV) break;
+                at += (uint64_t)width * HV;
+            }
+            const uint32_t item = (uint32_t)((x - at) / width), in = (uint32_t)((x - at) % width) + b;
+            const uint64_t item_x = at + (uint64_t)item * width;
+            s_end[b] = {s * HV + item, in > kItemCost ? in - kItemCost : 0u, (uint32_t)((item_x + kItemCost) / Q),
+                        (uint32_t)((item_x + width - 1) / Q)};
+        }
     }
     __syncthreads();
-    uint32_t seq = s_seq;
-    uint64_t seq_x = s_first;                                /* where the sequence's first item begins */
-    Seq sq = sequence<TS>(a, seq);
+    const uint32_t o0 = s_end[0].ordinal, o1 = s_end[1].ordinal;
+    const uint32_t range = o1 - o0 + 1;
 
-    uint8_t *ring = smem + warp * (C::kStages * C::kStage);
+    uint8_t *ring = smem + warp * (S * C::kStage);
     const uint32_t ring_a = smem_u32(ring);
-    /* a segment's end: each warp leaves its [head][D] sums over its own ring */
-    static_assert(kHeads * kJoin * 4 <= C::kStages * C::kStage, "sums of a warp fit its ring");
-    auto join = [&](uint32_t w) { return reinterpret_cast<float *>(smem + w * (C::kStages * C::kStage)); };
     const size_t v_off = (size_t)a.n_kv_heads * a.page_tokens * C::kRow;
     /* ldmatrix lane offsets inside a stage */
     const uint32_t mi = lane >> 3, mr = lane & 7;
     const uint32_t k_lane = ((mi & 1) * 8 + mr) * kPitch + (mi >> 1) * 16;
     const uint32_t v_lane = kQ8 ? k_lane : ((mi >> 1) * 8 + mr) * kPitch + (mi & 1) * 16;
-    uint32_t turn = 0;                                       /* short items so far: whose turn it is */
 
-    while (x < x1) {
-        uint64_t seq_end = seq_x + (uint64_t)(sq.steps + kItemCost) * HV;
-        while (x >= seq_end) {
-            seq_x = seq_end;
-            seq++;
-            sq = sequence<TS>(a, seq);
-            seq_end = seq_x + (uint64_t)(sq.steps + kItemCost) * HV;
+    /* A segment: the part of an item inside the range, and this warp's run of
+     * its steps [wb, we). */
+    struct Segment {
+        uint32_t seq, item;
+        Seq sq;
+        uint32_t sb, se, wb, we;
+        bool solo;
+    };
+    auto begin = [&](Segment &z) {
+        z.seq = o0 / HV;
+        z.item = o0 % HV;
+        z.sq = sequence<TS>(a, z.seq);
+    };
+    auto bounds = [&](Segment &z, uint32_t at) {             /* of item o0 + at, which z.seq and z.item name */
+        z.sb = at == 0 ? s_end[0].step : 0u;
+        z.se = at + 1 == range ? s_end[1].step : z.sq.steps;
+        const bool cut = z.sb > 0 || z.se < z.sq.steps;
+        z.solo = !cut && (z.sq.steps == 1 || (z.sq.steps <= kSolo && range >= (uint32_t)kWarps));
+        if (z.se <= z.sb) {                                  /* only overhead fell into this range */
+            z.wb = z.we = 0;
+        } else if (z.solo) {
+            z.wb = z.sb;
+            z.we = (at & (kWarps - 1)) == warp ? z.se : z.sb;
+        } else {
+            z.wb = z.sb + (uint32_t)((uint64_t)(z.se - z.sb) * warp / kWarps);
+            z.we = z.sb + (uint32_t)((uint64_t)(z.se - z.sb) * (warp + 1) / kWarps);
         }
-        const uint32_t width = sq.steps + kItemCost;
-        const uint32_t item = (uint32_t)(x - seq_x) / width;             /* both below 2^32: see the plan */
-        const uint64_t item_x = seq_x + (uint64_t)item * width, item_end = item_x + width;
-        const uint64_t end = x1 < item_end ? x1 : item_end;
-        const uint32_t sb = x > item_x + kItemCost ? (uint32_t)(x - item_x) - kItemCost : 0u;
-        const uint32_t se = end > item_x + kItemCost ? (uint32_t)(end - item_x) - kItemCost : 0u;
-        x = end;
-        if (se <= sb) continue;                              /* only overhead fell into this range */
-        const bool cut = sb > 0 || se < sq.steps;
-        const bool solo = !cut && sq.steps <= kSolo;
-        if (solo && (turn++ & (kWarps - 1)) != warp) continue;
+    };
+    auto step_on = [&](Segment &z) {
+        if (++z.item == HV) {
+            z.item = 0;
+            z.sq = sequence<TS>(a, ++z.seq);
+        }
+    };
+    auto first_token = [&](const Seq &q) -> uint32_t { return a.picked ? 0u : (q.start & ~15u); };
+    /* Logical page of the e-th page stepped over (0xFFFFFFFF: none). */
+    auto entry = [&](const Segment &z, uint32_t e) -> uint32_t {
+        if (!a.picked) return e;
+        const uint32_t head = z.item / a.n_tiles;
+        return e < z.sq.n_list ? (uint32_t)__ldg(a.picked + ((size_t)z.seq * a.n_kv_heads + head) * a.n_pick + e) : 0xFFFFFFFFu;
+    };
+    /* Its physical page (>= n_pages: nothing to read). */
+    auto mapped = [&](const Segment &z, uint32_t lp) -> uint32_t {
+        return lp < a.max_pages && lp * a.page_tokens < z.sq.len ? (uint32_t)__ldg(a.block_table + (size_t)z.seq * a.max_pages + lp)
+                                                                 : 0xFFFFFFFFu;
+    };
 
-        const uint32_t tile = item % a.n_tiles, head = item / a.n_tiles;
+    /* ---- copies: S - 1 steps ahead of the arithmetic ----
+     * Cursor of the next group of 16 tokens to copy: its page, the slot in it,
+     * its position, and the following pages, whose numbers are loaded a page
+     * (list entries: two pages) before they are needed. */
+    Segment pz;
+    begin(pz);
+    uint32_t p_at = 0, left = 0, page_e = 0, off = 0, pos = 0, lp_next = 0, ph_next = 0, lp_then = 0;
+    const uint8_t *kp = nullptr;
+    const float *sp = nullptr;
+    bool page_ok = false;
+    auto open_page = [&](uint32_t lp, uint32_t ph) {
+        page_ok = ph < a.n_pages;
+        const size_t row = ((size_t)(page_ok ? ph : 0u) * 2 * a.n_kv_heads + pz.item / a.n_tiles) * a.page_tokens + off;
+        kp = static_cast<const uint8_t *>(a.pool) + row * C::kRow + lane * 16;
+        if (kQ8) sp = a.scales + row + (lane >> 2) * (size_t)a.n_kv_heads * a.page_tokens + (lane & 3) * 4;
+        pos = page_ok ? lp * a.page_tokens + off : 0u;
+    };
+    /* Looks for this warp's next segment with steps (the first at entry), and
+     * loads the numbers of its first pages into the `next` of the cursor. */
+    bool opened = true;
+    auto find = [&](bool go_on) {
+        if (go_on) { p_at++; if (p_at < range) step_on(pz); }
+        for (; p_at < range; p_at++) {
+            bounds(pz, p_at);
+            if (pz.we > pz.wb) break;
+            if (p_at + 1 < range) step_on(pz);
+        }
+        if (p_at >= range) return;
+        left = pz.we - pz.wb;
+        const uint32_t v = first_token(pz.sq) + pz.wb * TS;
+        page_e = a.page_of(v);
+        off = v - page_e * a.page_tokens;
+        lp_next = entry(pz, page_e);
+        lp_then = entry(pz, page_e + 1);
+        ph_next = mapped(pz, lp_next);
+        opened = false;
+    };
+    auto turn_page = [&](uint32_t e) {                       /* opens the page at hand, e-th of the segment; looks up the one after */
+        open_page(lp_next, ph_next);
+        page_e = e;
+        lp_next = lp_then;
+        ph_next = mapped(pz, lp_next);
+        lp_then = entry(pz, e + 2);
+    };
+    /* Starts the copies of the next step into ring slot st; whether the step
+     * has every one of its tokens.  Dropped tokens become zeros. */
+    auto fetch = [&](uint32_t st) -> bool {
+        constexpr int CPR = C::kRow / 16, N = 16 * CPR;      /* 16-byte chunks of a row, of a group */
+        bool whole = true;
+        if (!opened) { turn_page(page_e); opened = true; }
+        #pragma unroll
+        for (int gr = 0; gr < GR; gr++) {
+            const uint32_t to = ring_a + st * C::kStage + gr * 16 * kPitch;
+            const uint32_t to_s = ring_a + st * C::kStage + 2 * TS * kPitch + ((lane >> 2) * TS + gr * 16 + (lane & 3) * 4) * 4;
+            const uint8_t *vp = kp + v_off;
+            const bool full = page_ok && pos >= pz.sq.start && pos + 16 <= pz.sq.len;
+            whole = whole && full;
+            if (full) {
+                #pragma unroll
+                for (int c0 = 0; c0 < N; c0 += 32) {
+                    const uint32_t c = c0 + lane;
+                    if (N % 32 != 0 && c >= (uint32_t)N) continue;
+                    const uint32_t d = to + (c / CPR) * kPitch + (c % CPR) * 16;
+                    cp_async16(d, kp + c0 * 16);
+                    cp_async16(d + TS * kPitch, vp + c0 * 16);
+                }
+                if (kQ8 && lane < 8) cp_async16(to_s, sp);   /* 16 scales of K, 16 of V */
+            } else {
+                const uint32_t lo = pos < pz.sq.start ? pz.sq.start - pos : 0u;      /* tokens [lo, hi) of the group are kept */
+                const uint32_t hi = !page_ok || pos >= pz.sq.len ? 0u : (pz.sq.len - pos < 16u ? pz.sq.len - pos : 16u);
+                #pragma unroll 1
+                for (uint32_t c = lane; c < (uint32_t)N; c += 32) {
+                    const uint32_t row = c / CPR, d = to + row * kPitch + (c % CPR) * 16;
+                    const uint32_t bytes = row >= lo && row < hi ? 16u : 0u;
+                    cp_async16_part(d, kp + (c - lane) * 16, bytes);
+                    cp_async16_part(d + TS * kPitch, vp + (c - lane) * 16, bytes);
+                }
+                if (kQ8 && lane < 8) {
+                    const uint32_t tk = (lane & 3) * 4;
+                    cp_async16_part(to_s, sp, (hi > tk ? (hi - tk < 4u ? hi - tk : 4u) : 0u) * 4);
+                }
+            }
+            off += 16;
+            pos += 16;
+            kp += 16 * C::kRow;
+            if (kQ8) sp += 16;
+            if (off == a.page_tokens) {
+                off = 0;
+                turn_page(page_e + 1);
+            }
+        }
+        return whole;
+    };
+    uint32_t whole_slots = 0;                                /* bit per ring slot */
+    auto advance = [&](uint32_t st) {
+        if (p_at < range) {
+            whole_slots = fetch(st) ? whole_slots | (1u << st) : whole_slots & ~(1u << st);
+            if (--left == 0) find(true);
+        }
+        cp_commit();
+    };
+    find(false);
+    #pragma unroll 1
+    for (int st = 0; st < S - 1; st++) advance(st);
+    uint32_t slot = 0;                                       /* slot of the next step; the one before it is free */
+
+    /* ---- arithmetic ---- */
+    Segment z;
+    begin(z);
+    #pragma unroll 1
+    for (uint32_t at = 0; at < range; at++) {
+        if (at) step_on(z);
+        bounds(z, at);
+        if (z.se <= z.sb || (z.solo && z.we == z.wb)) continue;          /* nothing, or another warp's */
+        const uint32_t seq = z.seq, tile = z.item % a.n_tiles, head = z.item / a.n_tiles;
         const uint32_t rows = a.group - tile * 16 < 16 ? a.group - tile * 16 : 16;
-        const uint32_t v_begin = a.picked ? 0u : (sq.start & ~15u);
-        const int32_t *table = a.block_table + (size_t)seq * a.max_pages;
-        const int32_t *list = a.picked ? a.picked + ((size_t)seq * a.n_kv_heads + head) * a.n_pick : nullptr;
-        const uint32_t stride = solo ? 1u : (uint32_t)kWarps;
+        const bool cut = z.sb > 0 || z.se < z.sq.steps;
         auto query_head = [&](uint32_t r) -> uint32_t {
             const uint32_t in_group = tile * 16 + r;
             return a.blocked ? head * a.group + in_group : in_group * a.n_kv_heads + head;
         };
 
-        /* Logical page of 16-token group gr of step i (0xFFFFFFFF: none). */
-        auto entry = [&](uint32_t i, int gr) -> uint32_t {
-            const uint32_t e = a.page_of(v_begin + i * TS + gr * 16);
-            if (!list) return i < se ? e : 0xFFFFFFFFu;
-            return i < se && e < sq.n_list ? (uint32_t)__ldg(list + e) : 0xFFFFFFFFu;
-        };
-        /* Its physical page (>= n_pages: nothing to read). */
-        auto mapped = [&](uint32_t lp) -> uint32_t {
-            return lp < a.max_pages && lp * a.page_tokens < sq.len ? (uint32_t)__ldg(table + lp) : 0xFFFFFFFFu;
-        };
-        /* Position of the group's first token in its sequence. */
-        auto position = [&](uint32_t i, int gr, uint32_t lp) -> uint32_t {
-            const uint32_t v = v_begin + i * TS + gr * 16;
-            return lp * a.page_tokens + (v - a.page_of(v) * a.page_tokens);
-        };
-        /* Starts the copies of step i into ring slot st; whether the step has
-         * every one of its tokens.  Tokens that the mask drops become zeros. */
-        auto fetch = [&](uint32_t st, uint32_t i, const uint32_t *lp, const uint32_t *ph) -> bool {
-            const uint32_t dst = ring_a + st * C::kStage;
-            constexpr int CPR = C::kRow / 16, N = 16 * CPR;              /* 16-byte chunks of a row, of the group */
-            bool whole = true;
-            #pragma unroll
-            for (int gr = 0; gr < GR; gr++) {
-                const bool ok = ph[gr] < a.n_pages;
-                const uint32_t pos = ok ? position(i, gr, lp[gr]) : 0u;
-                const uint32_t off = ok ? pos - lp[gr] * a.page_tokens : 0u;
-                const bool all = ok && pos >= sq.start && pos + 16 <= sq.len;
-                whole = whole && all;
-                const size_t row0 = (((size_t)(ok ? ph[gr] : 0u) * 2) * a.n_kv_heads + head) * a.page_tokens + off;
-                const uint8_t *k = static_cast<const uint8_t *>(a.pool) + row0 * C::kRow + lane * 16;
-                const uint8_t *v = k + v_off;
-                const uint32_t to = dst + gr * 16 * kPitch;
-                if (all) {
-                    #pragma unroll
-                    for (int c0 = 0; c0 < N; c0 += 32) {
-                        const uint32_t c = c0 + lane;
-                        if (N % 32 != 0 && c >= (uint32_t)N) continue;
-                        const uint32_t d = to + (c / CPR) * kPitch + (c % CPR) * 16;
-                        cp_async16(d, k + c0 * 16);
-                        cp_async16(d + TS * kPitch, v + c0 * 16);
-                    }
-                    if (kQ8 && lane < 8) {                               /* 16 scales of K, 16 of V */
-                        const float *sp = a.scales + row0 + (lane >> 2) * (size_t)a.n_kv_heads * a.page_tokens + (lane & 3) * 4;
-                        cp_async16(dst + 2 * TS * kPitch + ((lane >> 2) * TS + gr * 16 + (lane & 3) * 4) * 4, sp);
-                    }
-                } else {
-                    const uint32_t lo = pos < sq.start ? sq.start - pos : 0u;    /* tokens [lo, hi) of the group are kept */
-                    const uint32_t hi = !ok || pos >= sq.len ? 0u : (sq.len - pos < 16u ? sq.len - pos : 16u);
-                    #pragma unroll 1
-                    for (uint32_t c = lane; c < (uint32_t)N; c += 32) {
-                        const uint32_t row = c / CPR, d = to + row * kPitch + (c % CPR) * 16;
-                        const uint32_t bytes = row >= lo && row < hi ? 16u : 0u;
-                        cp_async16_part(d, k + (c - lane) * 16, bytes);
-                        cp_async16_part(d + TS * kPitch, v + (c - lane) * 16, bytes);
-                    }
-                    if (kQ8 && lane < 8) {
-                        const uint32_t tk = (lane & 3) * 4;
-                        const uint32_t n = hi > tk ? (hi - tk < 4u ? hi - tk : 4u) : 0u;
-                        const float *sp = a.scales + row0 + (lane >> 2) * (size_t)a.n_kv_heads * a.page_tokens + tk;
-                        cp_async16_part(dst + 2 * TS * kPitch + ((lane >> 2) * TS + gr * 16 + tk) * 4, sp, n * 4);
-                    }
-                }
-            }
-            return whole;
-        };
-
-        /* The copies run kStages - 1 steps ahead, the pages they need a step
-         * and the list entries two steps ahead of that. */
-        uint32_t fi = sb + (solo ? 0u : warp);               /* next step to fetch */
-        uint32_t lpA[GR], phA[GR], lpB[GR];
-        #pragma unroll
-        for (int gr = 0; gr < GR; gr++) { lpA[gr] = entry(fi, gr); lpB[gr] = entry(fi + stride, gr); }
-        #pragma unroll
-        for (int gr = 0; gr < GR; gr++) phA[gr] = mapped(lpA[gr]);
-        uint32_t whole_slots = 0;                            /* bit per ring slot */
-        auto advance = [&](uint32_t st) {
-            uint32_t lpC[GR], phB[GR];
-            #pragma unroll
-            for (int gr = 0; gr < GR; gr++) { lpC[gr] = entry(fi + 2 * stride, gr); phB[gr] = mapped(lpB[gr]); }
-            whole_slots &= ~(1u << st);
-            if (fi < se && fetch(st, fi, lpA, phA)) whole_slots |= 1u << st;
-            cp_commit();
-            #pragma unroll
-            for (int gr = 0; gr < GR; gr++) { lpA[gr] = lpB[gr]; phA[gr] = phB[gr]; lpB[gr] = lpC[gr]; }
-            fi += stride;
-        };
-        #pragma unroll
-        for (int st = 0; st < C::kStages - 1; st++) advance(st);
-
         /* ---- queries: B operands (8 heads a tile); heads past the group are zero ---- */
-        uint32_t qb[HT][KB][2];
+        constexpr bool kQS = C::template kQueriesInSmem<HT>;
+        uint32_t qb[kQS ? 1 : HT][KB][2];
+        uint8_t *qs = smem + C::kRing + warp * (kHeads * C::kQPitch);
         float sc[HT][2];                                     /* log2 scale of heads 2j, 2j + 1 */
         #pragma unroll
         for (int t = 0; t < HT; t++) {
+            uint32_t (&qt)[KB][2] = qb[kQS ? 0 : t];
             const uint32_t r = t * 8 + g;
             const uint16_t *qp = a.q + (size_t)seq * a.q_stride + (size_t)query_head(r < rows ? r : 0u) * D;
             #pragma unroll
             for (int b = 0; b < KB; b++) {
                 if (kQ8) {                                   /* values 4j .. 4j+3 of the block */
                     const uint2 w = r < rows ? __ldg(reinterpret_cast<const uint2 *>(qp + b * 16 + 4 * j)) : make_uint2(0u, 0u);
-                    qb[t][b][0] = w.x; qb[t][b][1] = w.y;
+                    qt[b][0] = w.x; qt[b][1] = w.y;
                 } else {
-                    qb[t][b][0] = r < rows ? __ldg(reinterpret_cast<const uint32_t *>(qp + b * 16 + 2 * j)) : 0u;
-                    qb[t][b][1] = r < rows ? __ldg(reinterpret_cast<const uint32_t *>(qp + b * 16 + 8 + 2 * j)) : 0u;
+                    qt[b][0] = r < rows ? __ldg(reinterpret_cast<const uint32_t *>(qp + b * 16 + 2 * j)) : 0u;
+                    qt[b][1] = r < rows ? __ldg(reinterpret_cast<const uint32_t *>(qp + b * 16 + 8 + 2 * j)) : 0u;
                 }
             }
             sc[t][0] = sc[t][1] = a.scale_log2;
@@ -377,7 +478,7 @@ __global__ void __launch_bounds__(kThreads) k_gqa_decode(const ct_gqa_args_t a) 
                 #pragma unroll
                 for (int b = 0; b < KB; b++) {
                     #pragma unroll
-                    for (int h = 0; h < 2; h++) top = fmaxf(top, fmaxf(fabsf(bf16_lo(qb[t][b][h])), fabsf(bf16_hi(qb[t][b][h]))));
+                    for (int h = 0; h < 2; h++) top = fmaxf(top, fmaxf(fabsf(bf16_lo(qt[b][h])), fabsf(bf16_hi(qt[b][h]))));
                 }
                 top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
                 top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
@@ -387,13 +488,23 @@ __global__ void __launch_bounds__(kThreads) k_gqa_decode(const ct_gqa_args_t a) 
                 #pragma unroll
                 for (int b = 0; b < KB; b++) {
                     #pragma unroll
-                    for (int h = 0; h < 2; h++) qb[t][b][h] = pack_f16(bf16_lo(qb[t][b][h]) * f, bf16_hi(qb[t][b][h]) * f);
+                    for (int h = 0; h < 2; h++) qt[b][h] = pack_f16(bf16_lo(qt[b][h]) * f, bf16_hi(qt[b][h]) * f);
                 }
                 const float back = a.scale_log2 * pow2f(e - 14);
                 sc[t][0] = __shfl_sync(0xFFFFFFFFu, back, 8 * j);
                 sc[t][1] = __shfl_sync(0xFFFFFFFFu, back, 8 * j + 4);
             }
+            if (kQS) {
+                #pragma unroll
+                for (int b = 0; b < KB; b++) {
+                    uint32_t *to = reinterpret_cast<uint32_t *>(qs + r * C::kQPitch + b * 32) + j;
+                    to[0] = qt[b][0];
+                    to[4] = qt[b][1];
+                }
+            }
         }
+        if (kQS) __syncwarp();
+        const uint32_t qs_a = smem_u32(qs) + mr * C::kQPitch + mi * 16;
 
         float o[KB][HT][4];
         #pragma unroll
@@ -401,142 +512,172 @@ __global__ void __launch_bounds__(kThreads) k_gqa_decode(const ct_gqa_args_t a) 
             #pragma unroll
             for (int t = 0; t < HT; t++) o[b][t][0] = o[b][t][1] = o[b][t][2] = o[b][t][3] = 0.0f;
         float m[HT][2], l[HT][2];
-        /* 8-bit pools: the fp16 weights are probability x V scale x unit.  The
-         * unit is a power of two that brought the largest weight of some step
-         * to [2^7, 2^8); it falls when a weight would pass 2^15 (`lim`) and is
-         * set anew when a maximum grows, so a weight keeps its 11 bits down to
-         * 2^-22 of the largest one that still counts. */
-        float unit[HT][2], lim[HT][2];
+        /* 8-bit pools: the fp16 weights are probability x V scale x 2^unit.
+         * The unit brought the largest weight of some step to [2^7, 2^8); it
+         * is set anew when a weight would pass 2^15 or when a maximum grew, so
+         * a weight keeps its 11 bits down to 2^-22 of the largest one that
+         * still counts. */
+        int unit[HT][2];
+        bool renew = true, blank = true;                     /* blank: some head has seen no token yet */
         #pragma unroll
         for (int t = 0; t < HT; t++)
             #pragma unroll
-            for (int h = 0; h < 2; h++) { m[t][h] = -INFINITY; l[t][h] = 0.0f; unit[t][h] = 1.0f; lim[t][h] = 0.0f; }
+            for (int h = 0; h < 2; h++) { m[t][h] = kNoMax; l[t][h] = 0.0f; unit[t][h] = 0; }
 
-        uint32_t slot = 0;
-        for (uint32_t i = sb + (solo ? 0u : warp); i < se; i += stride) {
-            advance(slot == 0 ? C::kStages - 1 : slot - 1);              /* refill the slot that the last step freed */
-            cp_wait<C::kStages - 1>();
+        #pragma unroll 1
+        for (uint32_t i = z.wb; i < z.we; i++) {
+            advance(slot == 0 ? S - 1 : slot - 1);                       /* refill the slot that the last step freed */
+            cp_wait<S - 1>();
             __syncwarp();
             const uint32_t stage = ring_a + slot * C::kStage;
             const float *scp = reinterpret_cast<const float *>(ring + slot * C::kStage + 2 * TS * kPitch);
-            const bool whole = (whole_slots >> slot) & 1u;
 
             /* scores: rows = tokens g, g + 8 of a group, columns = heads 2j, 2j + 1 */
             float s[GR][HT][4];
             #pragma unroll
             for (int gr = 0; gr < GR; gr++) {
+                float s2[HT][4];                             /* every other block: two chains of MMAs */
                 #pragma unroll
-                for (int t = 0; t < HT; t++) s[gr][t][0] = s[gr][t][1] = s[gr][t][2] = s[gr][t][3] = 0.0f;
+                for (int t = 0; t < HT; t++)
+                    #pragma unroll
+                    for (int h = 0; h < 4; h++) s[gr][t][h] = s2[t][h] = 0.0f;
                 #pragma unroll
-                for (int b = 0; b < C::kRow / 32; b++) {
-                    uint32_t r[4];
-                    ldsm4(stage + k_lane + gr * 16 * kPitch + b * 32, r);
+                for (int b = 0; b < KB; b += 2) {
+                    uint32_t r[4], f[2][4], q[HT][4];
+                    ldsm4(stage + k_lane + gr * 16 * kPitch + b * 16 * C::kElt, r);
                     if (kQ8) {
                         #pragma unroll
                         for (int h = 0; h < 2; h++) {
-                            uint32_t f[4];
-                            widen<DT, false>(r[2 * h], f[0], f[2]);
-                            widen<DT, false>(r[2 * h + 1], f[1], f[3]);
-                            #pragma unroll
-                            for (int t = 0; t < HT; t++) mma16816<true>(s[gr][t], f, qb[t][2 * b + h][0], qb[t][2 * b + h][1]);
+                            widen<DT, false>(r[2 * h], f[h][0], f[h][2]);
+                            widen<DT, false>(r[2 * h + 1], f[h][1], f[h][3]);
                         }
                     } else {
                         #pragma unroll
-                        for (int t = 0; t < HT; t++) mma16816<false>(s[gr][t], r, qb[t][b][0], qb[t][b][1]);
+                        for (int h = 0; h < 4; h++) f[0][h] = r[h];
+                        ldsm4(stage + k_lane + gr * 16 * kPitch + (b + 1) * 32, f[1]);
                     }
-                }
-            }
-            bool grow = false;
-            #pragma unroll
-            for (int gr = 0; gr < GR; gr++) {
-                float ks0 = 1.0f, ks1 = 1.0f;
-                if (kQ8) { ks0 = scp[gr * 16 + g]; ks1 = scp[gr * 16 + 8 + g]; }
-                #pragma unroll
-                for (int t = 0; t < HT; t++) {
-                    s[gr][t][0] *= ks0 * sc[t][0]; s[gr][t][1] *= ks0 * sc[t][1];
-                    s[gr][t][2] *= ks1 * sc[t][0]; s[gr][t][3] *= ks1 * sc[t][1];
-                }
-                if (!whole) {
-                    const uint32_t lp = entry(i, gr);
-                    const bool in = mapped(lp) < a.n_pages;
-                    const uint32_t pos = in ? position(i, gr, lp) + g : 0u;
                     #pragma unroll
                     for (int t = 0; t < HT; t++) {
-                        if (!in || pos >= sq.len || pos < sq.start) s[gr][t][0] = s[gr][t][1] = -INFINITY;
-                        if (!in || pos + 8 >= sq.len || pos + 8 < sq.start) s[gr][t][2] = s[gr][t][3] = -INFINITY;
+                        if (kQS) {
+                            ldsm4(qs_a + t * 8 * C::kQPitch + b * 32, q[t]);
+                        } else {
+                            q[t][0] = qb[kQS ? 0 : t][b][0]; q[t][1] = qb[kQS ? 0 : t][b][1];
+                            q[t][2] = qb[kQS ? 0 : t][b + 1][0]; q[t][3] = qb[kQS ? 0 : t][b + 1][1];
+                        }
+                        mma16816<kQ8>(s[gr][t], f[0], q[t][0], q[t][1]);
+                        mma16816<kQ8>(s2[t], f[1], q[t][2], q[t][3]);
                     }
                 }
                 #pragma unroll
                 for (int t = 0; t < HT; t++)
                     #pragma unroll
-                    for (int h = 0; h < 2; h++) grow = grow || fmaxf(s[gr][t][h], s[gr][t][2 + h]) > m[t][h] + kGrow;
+                    for (int h = 0; h < 4; h++) s[gr][t][h] += s2[t][h];
             }
-            if (__any_sync(0xFFFFFFFFu, grow)) {
+            float vs[GR][2];                                 /* V scales of tokens g, g + 8 */
+            #pragma unroll
+            for (int gr = 0; gr < GR; gr++) {
+                float ks0 = 1.0f, ks1 = 1.0f;
+                if (kQ8) {
+                    ks0 = scp[gr * 16 + g]; ks1 = scp[gr * 16 + 8 + g];
+                    vs[gr][0] = scp[TS + gr * 16 + g]; vs[gr][1] = scp[TS + gr * 16 + 8 + g];
+                }
+                #pragma unroll
+                for (int t = 0; t < HT; t++) {
+                    s[gr][t][0] *= ks0 * sc[t][0]; s[gr][t][1] *= ks0 * sc[t][1];
+                    s[gr][t][2] *= ks1 * sc[t][0]; s[gr][t][3] *= ks1 * sc[t][1];
+                }
+            }
+            if (!((whole_slots >> slot) & 1u)) {             /* some tokens are not to be attended */
+                #pragma unroll
+                for (int gr = 0; gr < GR; gr++) {
+                    const uint32_t v = first_token(z.sq) + i * TS + gr * 16;
+                    const uint32_t e = a.page_of(v), lp = entry(z, e);
+                    const bool in = mapped(z, lp) < a.n_pages;
+                    const uint32_t t0 = in ? lp * a.page_tokens + (v - e * a.page_tokens) + g : 0u;
+                    #pragma unroll
+                    for (int h = 0; h < 2; h++) {
+                        if (in && t0 + 8 * h < z.sq.len && t0 + 8 * h >= z.sq.start) continue;
+                        vs[gr][h] = 0.0f;                    /* it may be NaN */
+                        #pragma unroll
+                        for (int t = 0; t < HT; t++) s[gr][t][2 * h] = s[gr][t][2 * h + 1] = -INFINITY;
+                    }
+                }
+            }
+            float top = kNoMax;
+            #pragma unroll
+            for (int gr = 0; gr < GR; gr++)
+                #pragma unroll
+                for (int t = 0; t < HT; t++)
+                    #pragma unroll
+                    for (int h = 0; h < 4; h++) {
+                        s[gr][t][h] -= m[t][h & 1] == kNoMax ? 0.0f : m[t][h & 1];
+                        top = fmaxf(top, s[gr][t][h]);
+                    }
+            if (__any_sync(0xFFFFFFFFu, blank || top > kGrow)) {
+                renew = true;
+                blank = false;
                 #pragma unroll
                 for (int t = 0; t < HT; t++) {
                     #pragma unroll
                     for (int h = 0; h < 2; h++) {
-                        float mx = m[t][h];
+                        const bool none = m[t][h] == kNoMax;
+                        float by = none ? -INFINITY : 0.0f;  /* how far the maximum moves */
                         #pragma unroll
-                        for (int gr = 0; gr < GR; gr++) mx = fmaxf(mx, fmaxf(s[gr][t][h], s[gr][t][2 + h]));
+                        for (int gr = 0; gr < GR; gr++) by = fmaxf(by, fmaxf(s[gr][t][h], s[gr][t][2 + h]));
                         #pragma unroll
-                        for (int d = 4; d < 32; d <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, d));
-                        const float f = mx == -INFINITY ? 1.0f : ex2(m[t][h] - mx);
-                        m[t][h] = mx;
+                        for (int d = 4; d < 32; d <<= 1) by = fmaxf(by, __shfl_xor_sync(0xFFFFFFFFu, by, d));
+                        if (by == -INFINITY) { blank = true; continue; }
+                        const float f = none ? 1.0f : ex2(-by);
+                        m[t][h] = none ? by : m[t][h] + by;
                         l[t][h] *= f;
-                        lim[t][h] = 0.0f;
+                        #pragma unroll
+                        for (int gr = 0; gr < GR; gr++) { s[gr][t][h] -= by; s[gr][t][2 + h] -= by; }
                         #pragma unroll
                         for (int b = 0; b < KB; b++) { o[b][t][h] *= f; o[b][t][2 + h] *= f; }
                     }
                 }
             }
             #pragma unroll
-            for (int t = 0; t < HT; t++) {
+            for (int gr = 0; gr < GR; gr++)
                 #pragma unroll
-                for (int h = 0; h < 2; h++) {
-                    const float mz = m[t][h] == -INFINITY ? 0.0f : m[t][h];
+                for (int t = 0; t < HT; t++)
                     #pragma unroll
-                    for (int gr = 0; gr < GR; gr++) {
-                        s[gr][t][h] = ex2(s[gr][t][h] - mz);
-                        s[gr][t][2 + h] = ex2(s[gr][t][2 + h] - mz);
-                        l[t][h] += s[gr][t][h] + s[gr][t][2 + h];
+                    for (int h = 0; h < 4; h++) {
+                        s[gr][t][h] = ex2(s[gr][t][h]);
+                        l[t][h & 1] += s[gr][t][h];
                     }
-                }
-            }
             if (kQ8) {
-                bool over = false;
+                float wt = 0.0f;
                 #pragma unroll
-                for (int gr = 0; gr < GR; gr++) {
-                    const float vs0 = scp[TS + gr * 16 + g], vs1 = scp[TS + gr * 16 + 8 + g];
+                for (int gr = 0; gr < GR; gr++)
                     #pragma unroll
-                    for (int t = 0; t < HT; t++) {
+                    for (int t = 0; t < HT; t++)
                         #pragma unroll
-                        for (int h = 0; h < 4; h++) {        /* a masked token's scale may be NaN */
-                            const float w = s[gr][t][h] * (h < 2 ? vs0 : vs1);
-                            s[gr][t][h] = !whole && s[gr][t][h] == 0.0f ? 0.0f : w;
-                            over = over || s[gr][t][h] > lim[t][h & 1];
+                        for (int h = 0; h < 4; h++) {
+                            s[gr][t][h] *= vs[gr][h >> 1] * pow2f(unit[t][h & 1]);
+                            wt = fmaxf(wt, s[gr][t][h]);
                         }
-                    }
-                }
-                if (__any_sync(0xFFFFFFFFu, over)) {
+                if (__any_sync(0xFFFFFFFFu, renew || wt >= kTopWeight)) {
+                    renew = false;
                     #pragma unroll
                     for (int t = 0; t < HT; t++) {
                         #pragma unroll
                         for (int h = 0; h < 2; h++) {
-                            float top = 0.0f;
+                            float w = 0.0f;
                             #pragma unroll
-                            for (int gr = 0; gr < GR; gr++) top = fmaxf(top, fmaxf(s[gr][t][h], s[gr][t][2 + h]));
+                            for (int gr = 0; gr < GR; gr++) w = fmaxf(w, fmaxf(s[gr][t][h], s[gr][t][2 + h]));
                             #pragma unroll
-                            for (int d = 4; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, d));
-                            if (top > lim[t][h]) {
-                                int e = (int)(__float_as_uint(top) >> 23) - 127;
-                                e = e < -119 ? -119 : e > 119 ? 119 : e;
-                                const float nu = pow2f(7 - e), f = nu / unit[t][h];
-                                unit[t][h] = nu;
-                                lim[t][h] = pow2f(e + 8);
-                                #pragma unroll
-                                for (int b = 0; b < KB; b++) { o[b][t][h] *= f; o[b][t][2 + h] *= f; }
-                            }
+                            for (int d = 4; d < 32; d <<= 1) w = fmaxf(w, __shfl_xor_sync(0xFFFFFFFFu, w, d));
+                            if (w == 0.0f) { renew = true; continue; }
+                            int to = unit[t][h] + 7 - ((int)(__float_as_uint(w) >> 23) - 127);
+                            to = to < -100 ? -100 : to > 100 ? 100 : to;
+                            const int by = to - unit[t][h];
+                            const float f0 = pow2f(by / 2), f1 = pow2f(by - by / 2);
+                            unit[t][h] = to;
+                            #pragma unroll
+                            for (int gr = 0; gr < GR; gr++) { s[gr][t][h] = s[gr][t][h] * f0 * f1; s[gr][t][2 + h] = s[gr][t][2 + h] * f0 * f1; }
+                            #pragma unroll
+                            for (int b = 0; b < KB; b++) { o[b][t][h] = o[b][t][h] * f0 * f1; o[b][t][2 + h] = o[b][t][2 + h] * f0 * f1; }
                         }
                     }
                 }
@@ -548,8 +689,8 @@ __global__ void __launch_bounds__(kThreads) k_gqa_decode(const ct_gqa_args_t a) 
                 for (int t = 0; t < HT; t++) {
                     const float *w = s[gr][t];
                     if (kQ8) {
-                        p0[t] = transpose8(pack_f16(w[0] * unit[t][0], w[1] * unit[t][1]));
-                        p1[t] = transpose8(pack_f16(w[2] * unit[t][0], w[3] * unit[t][1]));
+                        p0[t] = transpose8(pack_f16(w[0], w[1]));
+                        p1[t] = transpose8(pack_f16(w[2], w[3]));
                     } else {
                         const uint32_t h0 = pack_bf16(w[0], w[1]), h1 = pack_bf16(w[2], w[3]);
                         p0[t] = transpose8(h0);
@@ -581,38 +722,12 @@ __global__ void __launch_bounds__(kThreads) k_gqa_decode(const ct_gqa_args_t a) 
                 }
             }
             __syncwarp();                                    /* the slot may be refilled */
-            slot = slot + 1 == C::kStages ? 0 : slot + 1;
+            slot = slot + 1 == S ? 0 : slot + 1;
         }
-        cp_wait<0>();
-        __syncwarp();
 
         /* ---- join the warps (a short item has one) ---- */
-        #pragma unroll
-        for (int t = 0; t < HT; t++) {
-            #pragma unroll
-            for (int h = 0; h < 2; h++) {
-                const uint32_t r = t * 8 + 2 * j + h;
-                #pragma unroll
-                for (int d = 4; d < 32; d <<= 1) l[t][h] += __shfl_xor_sync(0xFFFFFFFFu, l[t][h], d);
-                if (g == 0) { s_ml[warp][r][0] = m[t][h]; s_ml[warp][r][1] = l[t][h]; }
-                float *dst = join(warp) + r * kJoin;
-                const float back = kQ8 ? 1.0f / unit[t][h] : 1.0f;
-                if (r < rows) {
-                    #pragma unroll
-                    for (int b = 0; b < KB; b++) {
-                        if (kQ8) {                           /* values 2g, 2g + 1 of the block */
-                            *reinterpret_cast<float2 *>(dst + b * 16 + 2 * g) = make_float2(o[b][t][h] * back, o[b][t][2 + h] * back);
-                        } else {                             /* g, g + 8 */
-                            dst[b * 16 + g] = o[b][t][h];
-                            dst[b * 16 + 8 + g] = o[b][t][2 + h];
-                        }
-                    }
-                }
-            }
-        }
-        if (solo) __syncwarp(); else __syncthreads();
-        const uint32_t w0 = solo ? warp : 0u, w1 = solo ? warp + 1 : (uint32_t)kWarps;
-        const uint32_t part = 2 * blockIdx.x + (sb > 0 ? 0u : 1u);
+        const uint32_t w0 = z.solo ? warp : 0u, w1 = z.solo ? warp + 1 : (uint32_t)kWarps;
+        const uint32_t part = 2 * blockIdx.x + (z.sb > 0 ? 0u : 1u);
         float *po = a.part_o + (size_t)part * 16 * D;
         float *pml = a.part_ml + (size_t)part * 32;
         auto finish = [&](uint32_t r, uint32_t d, float M, float L, const float4 &acc) {
@@ -622,63 +737,144 @@ __global__ void __launch_bounds__(kThreads) k_gqa_decode(const ct_gqa_args_t a) 
                 make_uint2(pack_bf16(acc.x * inv, acc.y * inv), pack_bf16(acc.z * inv, acc.w * inv));
             if (a.lse && d == 0) a.lse[row] = (M + log2f(L)) * kLn2;
         };
-        /* weight of a part with maximum pm and sum pl; a part without tokens has none */
-        auto weight = [&](float pm, float pl, float M) -> float { return pm == -INFINITY && pl == 0.0f ? 0.0f : ex2(pm - M); };
-        for (uint32_t c = solo ? lane : tid; c < rows * (D / 4); c += solo ? 32u : (uint32_t)kThreads) {
-            const uint32_t r = c / (D / 4), d = (c % (D / 4)) * 4;
-            float M = -INFINITY;
-            for (uint32_t w = w0; w < w1; w++) M = fmaxf(M, s_ml[w][r][0]);
-            float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-            float L = 0.0f;
-            for (uint32_t w = w0; w < w1; w++) {
-                const float f = weight(s_ml[w][r][0], s_ml[w][r][1], M);
-                const float4 v = *reinterpret_cast<const float4 *>(join(w) + r * kJoin + d);
-                L += s_ml[w][r][1] * f;
-                acc.x += v.x * f; acc.y += v.y * f; acc.z += v.z * f; acc.w += v.w * f;
+        const uint32_t freed = slot == 0 ? S - 1 : slot - 1;
+        float *mine = reinterpret_cast<float *>(ring + freed * C::kStage);
+        if (lane == 0) s_free[warp] = warp * (S * C::kStage) + freed * C::kStage;
+        #pragma unroll
+        for (int t = 0; t < HT; t++)
+            #pragma unroll
+            for (int h = 0; h < 2; h++) {
+                #pragma unroll
+                for (int d = 4; d < 32; d <<= 1) l[t][h] += __shfl_xor_sync(0xFFFFFFFFu, l[t][h], d);
+                if (g == 0) { s_ml[warp][t * 8 + 2 * j + h][0] = m[t][h]; s_ml[warp][t * 8 + 2 * j + h][1] = l[t][h]; }
             }
-            if (cut) {
-                __stcg(reinterpret_cast<float4 *>(po + r * D + d), acc);
-                if (d == 0) __stcg(reinterpret_cast<float2 *>(pml + 2 * r), make_float2(M, L));
-            } else {
-                finish(r, d, M, L, acc);
-            }
-        }
-        if (solo) { __syncwarp(); continue; }
-        if (cut) {
-            /* The CTA that finishes an item last joins its parts, in order. */
-            const uint32_t first = (uint32_t)((item_x + kItemCost) / Q), last = (uint32_t)((item_end - 1) / Q);
-            __threadfence();
-            __syncthreads();
-            if (tid == 0) {
-                const uint32_t n = atomicAdd(a.counters + first, 1u);
-                s_last = n == last - first ? 1u : 0u;
-                if (s_last) { a.counters[first] = 0u; __threadfence(); }
-            }
-            __syncthreads();
-            if (s_last) {
-                for (uint32_t c = tid; c < rows * (D / 4); c += kThreads) {
-                    const uint32_t r = c / (D / 4), d = (c % (D / 4)) * 4;
-                    float M = -INFINITY;
-                    for (uint32_t w = first; w <= last; w++) {
-                        const uint32_t p = 2 * w + (w == first ? 1u : 0u);
-                        M = fmaxf(M, __ldcg(a.part_ml + (size_t)p * 32 + 2 * r));
+        #pragma unroll
+        for (int d0 = 0; d0 < D; d0 += kJoinCols) {
+            #pragma unroll
+            for (int t = 0; t < HT; t++) {
+                #pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    const uint32_t r = t * 8 + 2 * j + h;
+                    float *dst = mine + r * kJoin;
+                    const float back = kQ8 ? pow2f(-unit[t][h]) : 1.0f;
+                    if (r < rows) {
+                        #pragma unroll
+                        for (int b = 0; b < kJoinCols / 16; b++) {
+                            const float *ob = o[d0 / 16 + b][t];
+                            if (kQ8) {                       /* values 2g, 2g + 1 of the block */
+                                *reinterpret_cast<float2 *>(dst + b * 16 + 2 * g) = make_float2(ob[h] * back, ob[2 + h] * back);
+                            } else {                         /* g, g + 8 */
+                                dst[b * 16 + g] = ob[h];
+                                dst[b * 16 + 8 + g] = ob[2 + h];
+                            }
+                        }
                     }
-                    float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                    float L = 0.0f;
-                    #pragma unroll 4
-                    for (uint32_t w = first; w <= last; w++) {
-                        const uint32_t p = 2 * w + (w == first ? 1u : 0u);
-                        const float2 ml = __ldcg(reinterpret_cast<const float2 *>(a.part_ml + (size_t)p * 32 + 2 * r));
-                        const float4 v = __ldcg(reinterpret_cast<const float4 *>(a.part_o + ((size_t)p * 16 + r) * D + d));
-                        const float f = weight(ml.x, ml.y, M);
-                        L += ml.y * f;
-                        acc.x += v.x * f; acc.y += v.y * f; acc.z += v.z * f; acc.w += v.w * f;
-                    }
+                }
+            }
+            if (z.solo) __syncwarp(); else __syncthreads();
+            for (uint32_t c = z.solo ? lane : tid; c < rows * (kJoinCols / 4); c += z.solo ? 32u : (uint32_t)kThreads) {
+                const uint32_t r = c / (kJoinCols / 4), dj = (c % (kJoinCols / 4)) * 4, d = d0 + dj;
+                float M = kNoMax;
+                for (uint32_t w = w0; w < w1; w++) M = fmaxf(M, s_ml[w][r][0]);
+                float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                float L = 0.0f;
+                for (uint32_t w = w0; w < w1; w++) {
+                    const float f = ex2(s_ml[w][r][0] - M);
+                    const float4 v = *reinterpret_cast<const float4 *>(smem + s_free[w] + (r * kJoin + dj) * 4);
+                    L += s_ml[w][r][1] * f;
+                    acc.x += v.x * f; acc.y += v.y * f; acc.z += v.z * f; acc.w += v.w * f;
+                }
+                if (cut) {
+                    __stcg(reinterpret_cast<float4 *>(po + r * D + d), acc);
+                    if (d == 0) __stcg(reinterpret_cast<float2 *>(pml + 2 * r), make_float2(M, L));
+                } else {
                     finish(r, d, M, L, acc);
                 }
             }
+            if (z.solo) __syncwarp(); else __syncthreads();              /* the slots and s_ml are free again */
         }
-        __syncthreads();                                     /* the rings and s_ml are free again */
+        if (cut) {
+            /* The CTA that finishes an item last joins its parts, in order.
+             * An item of more than 2 kFan workers (few items in the batch)
+             * is joined in two rounds: each aligned run of kFan workers by
+             * its last one, into the run's first part, then the runs. */
+            const End &end = s_end[z.sb > 0 ? 0 : 1];
+            const uint32_t first = end.first, last = end.last;
+            const bool tree = last - first >= 2 * kFan;
+            uint32_t lo = first, hi = last, by = 1;
+            if (tree) {
+                lo = blockIdx.x & ~(kFan - 1);
+                hi = min(lo + kFan - 1, last);
+                lo = max(lo, first);
+            }
+            bool last_here = true;
+            for (int round = 0; last_here && round < (tree ? 2 : 1); round++) {
+                /* three sets of counters: an item's, by its first worker; a
+                 * run's, by its first worker, apart for the run that an item
+                 * begins in (an earlier item may end in the same worker) */
+                const uint32_t set = !tree || round ? 0u : lo == first ? 1u : 2u;
+                uint32_t *counter = a.counters + set * gridDim.x + (set == 2 ? lo : first);
+                const uint32_t n = by == 1 ? hi - lo + 1 : (last / kFan) - (first / kFan) + 1;
+                __syncthreads();                             /* this CTA's part (or its run's) is written */
+                if (tid == 0) {
+                    __threadfence();
+                    const uint32_t before = atomicAdd(counter, 1u);
+                    s_last = before == n - 1 ? 1u : 0u;
+                    if (s_last) { *counter = 0u; __threadfence(); }
+                }
+                __syncthreads();
+                last_here = s_last != 0;
+                if (!last_here) break;
+                /* part k of the join: worker w_k, its slot */
+                auto slot_of = [&](uint32_t k) -> uint32_t {
+                    uint32_t w = lo + k;
+                    if (by != 1) w = k == 0 ? first : (first / kFan + k) * kFan;
+                    return 2 * w + (w == first ? 1u : 0u);
+                };
+                /* (max, sum) of part k and row r: entries c = r n + k in the
+                 * warps' free slots, each kStage / 8 of them */
+                constexpr uint32_t kPer = C::kStage / 8;
+                auto s_part = [&](uint32_t k, uint32_t r) -> float2 & {
+                    const uint32_t c = r * n + k;
+                    return reinterpret_cast<float2 *>(smem + s_free[c / kPer])[c % kPer];
+                };
+                for (uint32_t c = tid; c < n * rows; c += kThreads) {
+                    const uint32_t r = c / n, k = c % n;
+                    s_part(k, r) = __ldcg(reinterpret_cast<const float2 *>(a.part_ml + (size_t)slot_of(k) * 32) + r);
+                }
+                __syncthreads();
+                const uint32_t to = slot_of(0);
+                const bool more = tree && round == 0;
+                for (uint32_t c = tid; c < rows * (D / 4); c += kThreads) {
+                    const uint32_t r = c / (D / 4), d = (c % (D / 4)) * 4;
+                    float M = kNoMax, L = 0.0f;
+                    for (uint32_t k = 0; k < n; k++) M = fmaxf(M, s_part(k, r).x);
+                    float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                    for (uint32_t k0 = 0; k0 < n; k0 += 8) {
+                        float4 v[8];
+                        #pragma unroll
+                        for (int k = 0; k < 8; k++)
+                            if (k0 + k < n) v[k] = __ldcg(reinterpret_cast<const float4 *>(a.part_o + ((size_t)slot_of(k0 + k) * 16 + r) * D + d));
+                        #pragma unroll
+                        for (int k = 0; k < 8; k++) {
+                            if (k0 + k >= n) continue;
+                            const float2 ml = s_part(k0 + k, r);
+                            const float f = ex2(ml.x - M);
+                            L += ml.y * f;
+                            acc.x += v[k].x * f; acc.y += v[k].y * f; acc.z += v[k].z * f; acc.w += v[k].w * f;
+                        }
+                    }
+                    if (more) {
+                        __stcg(reinterpret_cast<float4 *>(a.part_o + ((size_t)to * 16 + r) * D + d), acc);
+                        if (d == 0) __stcg(reinterpret_cast<float2 *>(a.part_ml + (size_t)to * 32) + r, make_float2(M, L));
+                    } else {
+                        finish(r, d, M, L, acc);
+                    }
+                }
+                by = kFan;
+            }
+            __syncthreads();                                 /* the free slots may be refilled */
+        }
     }
 }
 

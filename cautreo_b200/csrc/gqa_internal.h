@@ -23,7 +23,7 @@ typedef struct {
     uint16_t *out;               /* bf16 [n_seq][n_q_heads][D] */
     float *lse;                  /* [n_seq][n_q_heads] or NULL */
     float *part_o, *part_ml;     /* [2 n_workers][16][D], [2 n_workers][16][2] */
-    uint32_t *counters;          /* [n_workers], zero between launches */
+    uint32_t *counters;          /* [3 n_workers], zero between launches */
     uint64_t q_stride;
     uint32_t n_seq, n_q_heads, n_kv_heads, group, n_tiles;   /* group = query heads a kv head, tiles of 16 of them */
     uint32_t page_tokens, max_pages, n_pages, n_pick, window, blocked;

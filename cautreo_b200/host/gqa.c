@@ -182,7 +182,7 @@ ct_gqa_plan_t *ct_gqa_plan_create(const ct_gqa_shape_t *shape, uint32_t n_seq, i
     if (!rc) {
         p->n_workers = (uint32_t)(n_sms * ctas);
         const size_t po = (size_t)2 * p->n_workers * 16 * l.head_dim * sizeof(float);
-        const size_t pm = (size_t)2 * p->n_workers * 32 * sizeof(float), pc = (size_t)p->n_workers * sizeof(uint32_t);
+        const size_t pm = (size_t)2 * p->n_workers * 32 * sizeof(float), pc = (size_t)3 * p->n_workers * sizeof(uint32_t);
         rc = ct__cuda_status(cudaMalloc((void **)&p->part_o, po), "gqa scratch");
         if (!rc) rc = ct__cuda_status(cudaMalloc((void **)&p->part_ml, pm), "gqa scratch");
         if (!rc) rc = ct__cuda_status(cudaMalloc((void **)&p->counters, pc), "gqa scratch");
@@ -222,7 +222,7 @@ static int decode(ct_gqa_plan_t *p, const void *q, uint64_t q_stride, const void
         .counters = p->counters, .q_stride = q_stride, .n_seq = p->n_seq, .n_q_heads = p->shape.n_q_heads,
         .n_kv_heads = l->n_kv_heads, .group = group, .n_tiles = (group + 15) / 16, .page_tokens = l->page_tokens,
         .max_pages = l->max_pages_per_seq, .n_pages = l->n_pages, .n_pick = n_select, .window = p->shape.window_tokens,
-        .blocked = p->shape.head_order == CT_GQA_BLOCKED, .min_steps = 8,
+        .blocked = p->shape.head_order == CT_GQA_BLOCKED, .min_steps = getenv("GQMIN") ? (uint32_t)atoi(getenv("GQMIN")) : 8,
         .scale_log2 = p->shape.scale * 1.4426950408889634f,
         .page_magic = page_groups == 1 ? 0u : (uint32_t)(0x100000000ull / page_groups) + 1u,
     };
