@@ -32,141 +32,162 @@ CT_DEV uint32_t pack2_bf16(float lo, float hi) {
     return *reinterpret_cast<uint32_t *>(&h);
 }
 
-struct Where {
-    bool ok;
-    uint32_t token, kv, head;
-    size_t row;                  /* row of the pool */
-};
+/* Both directions: blockIdx.y is the row's place in a token (K heads, then V
+ * heads), blockIdx.x a run of tokens, so a block reads or writes a head's
+ * consecutive slots as one contiguous run.  A thread moves 8 values of T
+ * tokens; all its loads are in flight before the first is used. */
 
-/* Row r of the call, ordered (token, K / V, head). */
-CT_DEV Where where(size_t r, size_t n_rows, const int32_t *slots, uint32_t n_kv_heads, uint32_t page_tokens, uint32_t n_pages) {
-    Where w = {false, 0, 0, 0, 0};
-    if (r >= n_rows) return w;
-    w.token = (uint32_t)(r / (2 * n_kv_heads));
-    const uint32_t kh = (uint32_t)(r % (2 * n_kv_heads));
-    w.kv = kh / n_kv_heads;
-    w.head = kh % n_kv_heads;
-    const int32_t slot = slots[w.token];
-    if (slot < 0) return w;
+/* Row of the pool for a token's slot, or none. */
+CT_DEV bool pool_row(int32_t slot, uint32_t place, uint32_t n_kv_heads, uint32_t page_tokens, uint32_t n_pages, size_t &row) {
     const uint32_t page = (uint32_t)slot / page_tokens;
-    if (page >= n_pages) return w;
-    w.ok = true;
-    w.row = ((size_t)page * 2 * n_kv_heads + kh) * page_tokens + (uint32_t)slot % page_tokens;
-    return w;
+    if (slot < 0 || page >= n_pages) return false;
+    row = ((size_t)page * 2 * n_kv_heads + place) * page_tokens + ((uint32_t)slot - page * page_tokens);
+    return true;
 }
 
-template <int D, int DT, bool F32>
+template <int D, int DT, bool F32, int T>
 __global__ void __launch_bounds__(kThreads) k_gqa_write(void *pool, float *scales, const void *ks, const void *vs, size_t k_stride,
                                                         size_t v_stride, const int32_t *slots, uint32_t n, uint32_t n_kv_heads,
                                                         uint32_t page_tokens, uint32_t n_pages) {
-    constexpr int L = lanes_of(D), U = D / 8;
-    const uint32_t u = threadIdx.x % L;
-    const size_t n_rows = (size_t)n * 2 * n_kv_heads;
-    const size_t r = (size_t)blockIdx.x * (kThreads / L) + threadIdx.x / L;
-    const Where w = where(r, n_rows, slots, n_kv_heads, page_tokens, n_pages);
-    const bool mine = w.ok && u < U;
-    float x[8];
+    constexpr int L = lanes_of(D), U = D / 8, R = kThreads / L;
+    const uint32_t u = threadIdx.x % L, place = blockIdx.y;
+    const bool is_v = place >= n_kv_heads;
+    const uint32_t t0 = blockIdx.x * (R * T) + threadIdx.x / L;
+    const size_t col = (size_t)(is_v ? place - n_kv_heads : place) * D + u * 8, stride = is_v ? v_stride : k_stride;
+    const void *from = is_v ? vs : ks;
+    uint4 w[T][F32 ? 2 : 1];
+    int32_t slot[T];
     #pragma unroll
-    for (int i = 0; i < 8; i++) x[i] = 0.0f;
-    if (mine) {
-        const size_t at = (size_t)w.token * (w.kv ? v_stride : k_stride) + (size_t)w.head * D + u * 8;
-        if (F32) {
-            const float4 *p = reinterpret_cast<const float4 *>(static_cast<const float *>(w.kv ? vs : ks) + at);
-            const float4 a = __ldg(p), b = __ldg(p + 1);
-            x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w; x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
-        } else {
-            const uint4 a = __ldg(reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(w.kv ? vs : ks) + at));
-            if (DT == CT_KV_BF16) {
-                *reinterpret_cast<uint4 *>(static_cast<uint16_t *>(pool) + w.row * D + u * 8) = a;
-                return;
-            }
-            const uint32_t ws[4] = {a.x, a.y, a.z, a.w};
-            #pragma unroll
-            for (int i = 0; i < 4; i++) { x[2 * i] = __uint_as_float(ws[i] << 16); x[2 * i + 1] = __uint_as_float(ws[i] & 0xFFFF0000u); }
+    for (int i = 0; i < T; i++) {
+        const uint32_t t = t0 + i * R;
+        slot[i] = t < n ? __ldg(slots + t) : -1;
+        if (t >= n || u >= U) continue;
+        const size_t at = (size_t)t * stride + col;
+        const uint4 *p = F32 ? reinterpret_cast<const uint4 *>(static_cast<const float *>(from) + at)
+                             : reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(from) + at);
+        w[i][0] = __ldcs(p);
+        if (F32) w[i][F32 ? 1 : 0] = __ldcs(p + 1);
+    }
+    #pragma unroll
+    for (int i = 0; i < T; i++) {
+        size_t row = 0;
+        const bool mine = pool_row(slot[i], place, n_kv_heads, page_tokens, n_pages, row) && u < U;
+        if (DT == CT_KV_BF16 && !F32) {
+            if (mine) *reinterpret_cast<uint4 *>(static_cast<uint16_t *>(pool) + row * D + u * 8) = w[i][0];
+            continue;
         }
-    }
-    if (DT == CT_KV_BF16) {
-        if (mine)
-            *reinterpret_cast<uint4 *>(static_cast<uint16_t *>(pool) + w.row * D + u * 8) =
-                make_uint4(pack2_bf16(x[0], x[1]), pack2_bf16(x[2], x[3]), pack2_bf16(x[4], x[5]), pack2_bf16(x[6], x[7]));
-        return;
-    }
-    uint32_t top = 0;                                        /* bits of max|x|: NaN above Inf above every finite value */
-    #pragma unroll
-    for (int i = 0; i < 8; i++) top = max(top, __float_as_uint(x[i]) & 0x7FFFFFFFu);
-    #pragma unroll
-    for (int o = 1; o < L; o <<= 1) top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
-    if (!mine) return;
-    const bool fine = top < 0x7F800000u;
-    const float d = __fdiv_rn(__uint_as_float(top), DT == CT_KV_INT8 ? 127.0f : 448.0f);
-    const float id = fine && d > 0.0f ? fminf(__fdiv_rn(1.0f, d), FLT_MAX) : 0.0f;
-    uint32_t c[2] = {0u, 0u};
-    if (fine) {
+        float x[8];
+        const uint32_t ws[8] = {w[i][0].x, w[i][0].y, w[i][0].z, w[i][0].w, w[i][F32 ? 1 : 0].x, w[i][F32 ? 1 : 0].y,
+                                w[i][F32 ? 1 : 0].z, w[i][F32 ? 1 : 0].w};
         #pragma unroll
-        for (int k = 0; k < 2; k++) {
-            if (DT == CT_KV_INT8) {
-                uint32_t q[4];
-                #pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    const int v = __float2int_rd(__fadd_rn(__fmul_rn(x[4 * k + e], id), 0.5f));
-                    q[e] = (uint32_t)max(-127, min(127, v));
+        for (int e = 0; e < 8; e++)
+            x[e] = !mine ? 0.0f : F32 ? __uint_as_float(ws[e]) : __uint_as_float((e & 1) ? ws[e >> 1] & 0xFFFF0000u : ws[e >> 1] << 16);
+        if (DT == CT_KV_BF16) {
+            if (mine)
+                *reinterpret_cast<uint4 *>(static_cast<uint16_t *>(pool) + row * D + u * 8) =
+                    make_uint4(pack2_bf16(x[0], x[1]), pack2_bf16(x[2], x[3]), pack2_bf16(x[4], x[5]), pack2_bf16(x[6], x[7]));
+            continue;
+        }
+        uint32_t top = 0;                                    /* bits of max|x|: NaN above Inf above every finite value */
+        #pragma unroll
+        for (int e = 0; e < 8; e++) top = max(top, __float_as_uint(x[e]) & 0x7FFFFFFFu);
+        #pragma unroll
+        for (int o = 1; o < L; o <<= 1) top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
+        if (!mine) continue;
+        const bool fine = top < 0x7F800000u;
+        const float d = __fdiv_rn(__uint_as_float(top), DT == CT_KV_INT8 ? 127.0f : 448.0f);
+        const float id = fine && d > 0.0f ? fminf(__fdiv_rn(1.0f, d), FLT_MAX) : 0.0f;
+        uint32_t c[2] = {0u, 0u};
+        if (fine) {
+            #pragma unroll
+            for (int k = 0; k < 2; k++) {
+                if (DT == CT_KV_INT8) {
+                    /* floor by a round-down addition into the bits of 1.5 x 2^23;
+                     * |x id| <= 127 (1 + 2^-21), so no code passes +-127 */
+                    uint32_t q[4];
+                    #pragma unroll
+                    for (int e = 0; e < 4; e++)
+                        q[e] = __float_as_uint(__fadd_rd(__fadd_rn(__fmul_rn(x[4 * k + e], id), 0.5f), 12582912.0f));
+                    c[k] = __byte_perm(__byte_perm(q[0], q[1], 0x0040), __byte_perm(q[2], q[3], 0x0040), 0x5410);
+                } else {
+                    c[k] = (uint32_t)ct_e4m3x2_code(x[4 * k], x[4 * k + 1], id) |
+                           ((uint32_t)ct_e4m3x2_code(x[4 * k + 2], x[4 * k + 3], id) << 16);
                 }
-                c[k] = __byte_perm(__byte_perm(q[0], q[1], 0x0040), __byte_perm(q[2], q[3], 0x0040), 0x5410);
-            } else {
-                c[k] = (uint32_t)ct_e4m3x2_code(x[4 * k], x[4 * k + 1], id) |
-                       ((uint32_t)ct_e4m3x2_code(x[4 * k + 2], x[4 * k + 3], id) << 16);
             }
         }
+        *reinterpret_cast<uint2 *>(static_cast<uint8_t *>(pool) + row * D + u * 8) = make_uint2(c[0], c[1]);
+        if (u == 0) scales[row] = fine ? d : __uint_as_float(0x7FC00000u);
     }
-    *reinterpret_cast<uint2 *>(static_cast<uint8_t *>(pool) + w.row * D + u * 8) = make_uint2(c[0], c[1]);
-    if (u == 0) scales[w.row] = fine ? d : __uint_as_float(0x7FC00000u);
 }
 
-/* Eight stored values of a row in fp32. */
-template <int D, int DT>
-CT_DEV void load8(const void *pool, size_t row, uint32_t u, float sc, float *x) {
-    if (DT == CT_KV_BF16) {
-        const uint4 a = __ldg(reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(pool) + row * D + u * 8));
-        const uint32_t ws[4] = {a.x, a.y, a.z, a.w};
-        #pragma unroll
-        for (int i = 0; i < 4; i++) { x[2 * i] = __uint_as_float(ws[i] << 16); x[2 * i + 1] = __uint_as_float(ws[i] & 0xFFFF0000u); }
-    } else {
-        const uint2 a = __ldg(reinterpret_cast<const uint2 *>(static_cast<const uint8_t *>(pool) + row * D + u * 8));
-        const uint32_t ws[2] = {a.x, a.y};
-        #pragma unroll
-        for (int i = 0; i < 8; i += 2) {
-            const uint32_t w = ws[i >> 2] >> (8 * (i & 3));
+/* Eight stored values (w: 16 bytes of bf16, or 8 codes in x and y) in fp32. */
+template <int DT> CT_DEV void values8(const uint4 &w, float sc, float *x) {
+    const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
+    #pragma unroll
+    for (int i = 0; i < 8; i += 2) {
+        if (DT == CT_KV_BF16) {
+            x[i] = __uint_as_float(ws[i >> 1] << 16);
+            x[i + 1] = __uint_as_float(ws[i >> 1] & 0xFFFF0000u);
+        } else {
+            const uint32_t c = ws[i >> 2] >> (8 * (i & 3));
             if (DT == CT_KV_INT8) {
-                x[i] = __fmul_rn((float)(int8_t)(uint8_t)w, sc);
-                x[i + 1] = __fmul_rn((float)(int8_t)(uint8_t)(w >> 8), sc);
+                x[i] = __fmul_rn((float)(int8_t)(uint8_t)c, sc);
+                x[i + 1] = __fmul_rn((float)(int8_t)(uint8_t)(c >> 8), sc);
             } else {
-                const float2 f = ct_e4m3x2_to_f32x2((uint16_t)w);
+                const float2 f = ct_e4m3x2_to_f32x2((uint16_t)c);
                 x[i] = __fmul_rn(f.x, sc);
                 x[i + 1] = __fmul_rn(f.y, sc);
             }
         }
     }
 }
+template <int D, int DT> CT_DEV uint4 load8(const void *pool, size_t row, uint32_t u) {
+    if (DT == CT_KV_BF16) return __ldg(reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(pool) + row * D + u * 8));
+    const uint2 a = __ldg(reinterpret_cast<const uint2 *>(static_cast<const uint8_t *>(pool) + row * D + u * 8));
+    return make_uint4(a.x, a.y, 0u, 0u);
+}
 
-template <int D, int DT, bool F32>
+template <int D, int DT, bool F32, int T>
 __global__ void __launch_bounds__(kThreads) k_gqa_read(const void *pool, const float *scales, const int32_t *slots, uint32_t n,
                                                        uint32_t n_kv_heads, uint32_t page_tokens, uint32_t n_pages, void *ko,
                                                        void *vo, size_t k_stride, size_t v_stride) {
-    constexpr int L = lanes_of(D), U = D / 8;
-    const uint32_t u = threadIdx.x % L;
-    const size_t r = (size_t)blockIdx.x * (kThreads / L) + threadIdx.x / L;
-    const Where w = where(r, (size_t)n * 2 * n_kv_heads, slots, n_kv_heads, page_tokens, n_pages);
-    if (!w.ok || u >= U) return;
-    float x[8];
-    load8<D, DT>(pool, w.row, u, DT == CT_KV_BF16 ? 1.0f : __ldg(scales + w.row), x);
-    const size_t at = (size_t)w.token * (w.kv ? v_stride : k_stride) + (size_t)w.head * D + u * 8;
-    if (F32) {
-        float4 *p = reinterpret_cast<float4 *>(static_cast<float *>(w.kv ? vo : ko) + at);
-        p[0] = make_float4(x[0], x[1], x[2], x[3]);
-        p[1] = make_float4(x[4], x[5], x[6], x[7]);
-    } else {
-        *reinterpret_cast<uint4 *>(static_cast<uint16_t *>(w.kv ? vo : ko) + at) =
-            make_uint4(pack2_bf16(x[0], x[1]), pack2_bf16(x[2], x[3]), pack2_bf16(x[4], x[5]), pack2_bf16(x[6], x[7]));
+    constexpr int L = lanes_of(D), U = D / 8, R = kThreads / L;
+    const uint32_t u = threadIdx.x % L, place = blockIdx.y;
+    if (u >= U) return;
+    const bool is_v = place >= n_kv_heads;
+    const uint32_t t0 = blockIdx.x * (R * T) + threadIdx.x / L;
+    const size_t col = (size_t)(is_v ? place - n_kv_heads : place) * D + u * 8, stride = is_v ? v_stride : k_stride;
+    void *to = is_v ? vo : ko;
+    int32_t slot[T];
+    uint4 w[T];
+    float sc[T];
+    bool ok[T];
+    #pragma unroll
+    for (int i = 0; i < T; i++) slot[i] = t0 + i * R < n ? __ldg(slots + t0 + i * R) : -1;
+    #pragma unroll
+    for (int i = 0; i < T; i++) {
+        size_t row = 0;
+        ok[i] = pool_row(slot[i], place, n_kv_heads, page_tokens, n_pages, row);
+        sc[i] = 1.0f;
+        if (!ok[i]) continue;
+        w[i] = load8<D, DT>(pool, row, u);
+        if (DT != CT_KV_BF16) sc[i] = __ldg(scales + row);
+    }
+    #pragma unroll
+    for (int i = 0; i < T; i++) {
+        if (!ok[i]) continue;
+        float x[8];
+        values8<DT>(w[i], sc[i], x);
+        const size_t at = (size_t)(t0 + i * R) * stride + col;
+        if (F32) {
+            float4 *p = reinterpret_cast<float4 *>(static_cast<float *>(to) + at);
+            __stcs(p, make_float4(x[0], x[1], x[2], x[3]));
+            __stcs(p + 1, make_float4(x[4], x[5], x[6], x[7]));
+        } else {
+            const uint4 y = DT == CT_KV_BF16 ? w[i] : make_uint4(pack2_bf16(x[0], x[1]), pack2_bf16(x[2], x[3]),
+                                                                 pack2_bf16(x[4], x[5]), pack2_bf16(x[6], x[7]));
+            __stcs(reinterpret_cast<uint4 *>(static_cast<uint16_t *>(to) + at), y);
+        }
     }
 }
 
@@ -196,14 +217,25 @@ __global__ void __launch_bounds__(128) k_gqa_bounds(const void *pool, const floa
     #pragma unroll
     for (int e = 0; e < 8; e++) { hi[e] = -INFINITY; lo[e] = INFINITY; }
     if (r < R) {
-        for (uint32_t t = r; t < count; t += R) {
-            float x[8];
-            load8<D, DT>(pool, row0 + t, u, DT == CT_KV_BF16 ? 1.0f : __ldg(scales + row0 + t), x);
+        for (uint32_t t = r; t < count; t += 4 * R) {        /* four rows' loads in flight */
+            uint4 w[4];
+            float sc[4];
             #pragma unroll
-            for (int e = 0; e < 8; e++) {
-                top = max(top, __float_as_uint(x[e]) & 0x7FFFFFFFu);
-                hi[e] = fmaxf(hi[e], x[e]);
-                lo[e] = fminf(lo[e], x[e]);
+            for (int i = 0; i < 4; i++) {
+                const size_t row = row0 + min(t + i * R, count - 1);     /* past the end: the last token once more */
+                w[i] = load8<D, DT>(pool, row, u);
+                sc[i] = DT == CT_KV_BF16 ? 1.0f : __ldg(scales + row);
+            }
+            #pragma unroll
+            for (int i = 0; i < 4; i++) {
+                float x[8];
+                values8<DT>(w[i], sc[i], x);
+                #pragma unroll
+                for (int e = 0; e < 8; e++) {
+                    top = max(top, __float_as_uint(x[e]) & 0x7FFFFFFFu);
+                    hi[e] = fmaxf(hi[e], x[e]);
+                    lo[e] = fminf(lo[e], x[e]);
+                }
             }
         }
         #pragma unroll
@@ -244,14 +276,20 @@ __global__ void __launch_bounds__(128) k_gqa_bounds(const void *pool, const floa
         default: return CT_ERR_UNSUPPORTED;        \
     }
 
+/* Tokens a thread moves: 4 when the call fills the GPU with them, else 1. */
+inline bool many(uint32_t n, uint32_t heads) { return (uint64_t)n * heads >= 16384; }
+
 struct WriteCall {
     void *pool; float *scales; const void *k, *v; size_t ks, vs; const int32_t *slots;
     uint32_t n, heads, pt, np; cudaStream_t st;
     template <int D, int DT, bool F32> int go() const {
-        constexpr int rows = kThreads / lanes_of(D);
-        const size_t n_rows = (size_t)n * 2 * heads;
-        k_gqa_write<D, DT, F32><<<(unsigned)((n_rows + rows - 1) / rows), kThreads, 0, st>>>(pool, scales, k, v, ks, vs, slots, n,
-                                                                                             heads, pt, np);
+        constexpr uint32_t R = kThreads / lanes_of(D);
+        if (many(n, heads))
+            k_gqa_write<D, DT, F32, 4><<<dim3((n + 4 * R - 1) / (4 * R), 2 * heads), kThreads, 0, st>>>(pool, scales, k, v, ks, vs,
+                                                                                                        slots, n, heads, pt, np);
+        else
+            k_gqa_write<D, DT, F32, 1><<<dim3((n + R - 1) / R, 2 * heads), kThreads, 0, st>>>(pool, scales, k, v, ks, vs, slots, n,
+                                                                                              heads, pt, np);
         ct__count_launches(1);
         return ct__cuda_status(cudaGetLastError(), "gqa write");
     }
@@ -261,10 +299,13 @@ struct ReadCall {
     const void *pool; const float *scales; const int32_t *slots; uint32_t n, heads, pt, np; void *k, *v; size_t ks, vs;
     cudaStream_t st;
     template <int D, int DT, bool F32> int go() const {
-        constexpr int rows = kThreads / lanes_of(D);
-        const size_t n_rows = (size_t)n * 2 * heads;
-        k_gqa_read<D, DT, F32><<<(unsigned)((n_rows + rows - 1) / rows), kThreads, 0, st>>>(pool, scales, slots, n, heads, pt, np,
-                                                                                            k, v, ks, vs);
+        constexpr uint32_t R = kThreads / lanes_of(D);
+        if (many(n, heads))
+            k_gqa_read<D, DT, F32, 4><<<dim3((n + 4 * R - 1) / (4 * R), 2 * heads), kThreads, 0, st>>>(pool, scales, slots, n, heads,
+                                                                                                       pt, np, k, v, ks, vs);
+        else
+            k_gqa_read<D, DT, F32, 1><<<dim3((n + R - 1) / R, 2 * heads), kThreads, 0, st>>>(pool, scales, slots, n, heads, pt, np, k,
+                                                                                             v, ks, vs);
         ct__count_launches(1);
         return ct__cuda_status(cudaGetLastError(), "gqa read");
     }

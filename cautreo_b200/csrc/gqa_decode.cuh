@@ -56,12 +56,22 @@ constexpr uint32_t kItemCost = 4;       /* steps that an item's start and end ar
 constexpr uint32_t kSolo = 8;           /* steps up to which an item is one warp's, if the CTA has items for every warp */
 constexpr uint32_t kFan = 16;           /* workers whose parts are joined at a time, when an item has more than 2 kFan */
 
-/* Tokens of a warp's step (2 to 17 KB of K and V) and steps in the ring. */
-template <int D, int DT> struct Cfg {
+/* Tokens of a warp's step, steps in its ring, CTAs that an SM holds. */
+#ifndef GQ_TS
+#define GQ_TS (kRow <= 64 ? 32 : 16)
+#endif
+#ifndef GQ_S
+#define GQ_S 3
+#endif
+#ifndef GQ_MINB
+#define GQ_MINB 1
+#endif
+template <int D, int DT, int HT> struct Cfg {
     static constexpr int kElt = DT == CT_KV_BF16 ? 2 : 1;
     static constexpr int kRow = D * kElt;
-    static constexpr int TS = kRow <= 64 ? 32 : 16;
-    static constexpr int kStages = 3;
+    static constexpr int TS = GQ_TS;
+    static constexpr int kStages = GQ_S;
+    static constexpr int kMinB = GQ_MINB;
     static constexpr int kPitch = kRow + 16;                  /* odd number of 16-B units: conflict-free ldmatrix */
     static constexpr int kScaleBytes = DT == CT_KV_BF16 ? 0 : TS * 8;
     static constexpr int kStage = 2 * TS * kPitch + kScaleBytes;
@@ -70,9 +80,9 @@ template <int D, int DT> struct Cfg {
      * spill) in shared memory behind the ring, a copy for each warp, where an
      * SM has the room (1 KB of its 227 is for the joins' statics). */
     static constexpr int kQPitch = 2 * D + 16;
-    template <int HT> static constexpr int kQBytes = kWarps * HT * 8 * kQPitch;
-    template <int HT> static constexpr bool kQueriesInSmem = HT * D >= 192 && kRing + kQBytes<HT> <= 226 * 1024;
-    template <int HT> static constexpr int kSmem = kRing + (kQueriesInSmem<HT> ? kQBytes<HT> : 0);
+    static constexpr int kQBytes = kWarps * HT * 8 * kQPitch;
+    static constexpr bool kQueriesInSmem = HT * D >= 192 && kRing + kQBytes <= 226 * 1024;
+    static constexpr int kSmem = kRing + (kQueriesInSmem ? kQBytes : 0);
 };
 
 CT_DEV uint32_t smem_u32(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
@@ -175,8 +185,8 @@ template <int TS> CT_DEV Seq sequence(const ct_gqa_args_t &a, uint32_t s) {
 
 /* HT: column tiles of 8 query heads. */
 template <int D, int DT, int HT>
-__global__ void __launch_bounds__(kThreads) k_gqa_decode(const ct_gqa_args_t a) {
-    using C = Cfg<D, DT>;
+__global__ void __launch_bounds__(kThreads, Cfg<D, DT, HT>::kMinB) k_gqa_decode(const ct_gqa_args_t a) {
+    using C = Cfg<D, DT, HT>;
     constexpr int TS = C::TS, GR = TS / 16, kPitch = C::kPitch, KB = D / 16, S = C::kStages;
     constexpr int kHeads = 8 * HT;
     constexpr bool kQ8 = DT != CT_KV_BF16;
@@ -451,7 +461,7 @@ __global__ void __launch_bounds__(kThreads) k_gqa_decode(const ct_gqa_args_t a) 
         };
 
         /* ---- queries: B operands (8 heads a tile); heads past the group are zero ---- */
-        constexpr bool kQS = C::template kQueriesInSmem<HT>;
+        constexpr bool kQS = C::kQueriesInSmem;
         uint32_t qb[kQS ? 1 : HT][KB][2];
         uint8_t *qs = smem + C::kRing + warp * (kHeads * C::kQPitch);
         float sc[HT][2];                                     /* log2 scale of heads 2j, 2j + 1 */

@@ -49,6 +49,7 @@ typedef struct {
     uint64_t q_stride;
     uint32_t n_seq, n_q_heads, n_kv_heads, group, dim;
     uint32_t page_tokens, max_pages, n_pages, n_pick, n_first, n_last, window, blocked;
+    uint32_t n_sms;
 } ct_gqa_select_args_t;
 
 /* Whether a kernel exists for these, CTAs it runs on an SM of the current

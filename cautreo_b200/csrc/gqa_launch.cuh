@@ -9,18 +9,18 @@
 namespace ct_gqa {
 
 template <int D, int DT, int HT> static int ctas() {
-    using C = Cfg<D, DT>;
+    using C = Cfg<D, DT, HT>;
     int n = 0;
-    int rc = ct__cuda_status(cudaFuncSetAttribute(k_gqa_decode<D, DT, HT>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::template kSmem<HT>),
+    int rc = ct__cuda_status(cudaFuncSetAttribute(k_gqa_decode<D, DT, HT>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem),
                              "gqa decode");
     if (!rc)
-        rc = ct__cuda_status(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, k_gqa_decode<D, DT, HT>, kThreads, C::template kSmem<HT>),
+        rc = ct__cuda_status(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, k_gqa_decode<D, DT, HT>, kThreads, C::kSmem),
                              "gqa decode");
     return rc ? 0 : n;
 }
 
 template <int D, int DT, int HT> static int run(const ct_gqa_args_t *a, uint32_t n_workers, cudaStream_t st) {
-    k_gqa_decode<D, DT, HT><<<n_workers, kThreads, Cfg<D, DT>::template kSmem<HT>, st>>>(*a);
+    k_gqa_decode<D, DT, HT><<<n_workers, kThreads, Cfg<D, DT, HT>::kSmem, st>>>(*a);
     ct__count_launches(1);
     return ct__cuda_status(cudaGetLastError(), "gqa decode");
 }

@@ -11,12 +11,15 @@
  * single fp32 roundings, so the chosen pages do not depend on how the sums
  * are split (ties go to the lowest page).
  *
- * Bound: HBM, 2 D + 4 bytes a page and head.  A CTA per (sequence, kv head):
- * its warps take 8 pages at a time as the columns of mma.sync m16n8k32 (int8),
- * the heads of the group being the rows; the scores become ordered 32-bit
- * keys in shared memory, a radix select of 8 bits a pass finds the key of the
- * last page chosen, and a scan writes the pages in ascending order.
+ * Bound: HBM, 2 D + 4 bytes a page and head.  A CTA per (sequence, kv head),
+ * or a cluster of up to 8 when that leaves SMs idle: its warps take 16 pages
+ * at a time, 8 as the columns of a mma.sync m16n8k32 (int8), the heads of the
+ * group being the rows, with the next pages' numbers loaded ahead.  The scores
+ * become ordered 32-bit keys in the first CTA's shared memory; a radix select
+ * over the bits that differ finds the key of the last page chosen, and a scan
+ * writes the pages in ascending order.
  */
+#include <cooperative_groups.h>
 #include <cuda_runtime.h>
 #include <math.h>
 
@@ -27,8 +30,11 @@
 
 namespace {
 
+namespace cg = cooperative_groups;
+
 constexpr int kThreads = 256, kWarps = kThreads / 32;
 constexpr uint32_t kMaxPages = 49152;                        /* keys in shared memory: 192 KB */
+constexpr int kTiles = 2;                                    /* 8-page tiles a warp takes at a time */
 constexpr uint32_t kKeyInf = 0xFF800000u, kKeyForced = 0xFFFFFFFFu;
 
 CT_DEV void mma_s8(int *c, const uint32_t *a, uint32_t b0, uint32_t b1) {
@@ -50,10 +56,14 @@ __global__ void __launch_bounds__(kThreads) k_gqa_select(const ct_gqa_select_arg
     constexpr int kPitch = 2 * D + 16;
     __shared__ __align__(16) int8_t s_q[16][kPitch];         /* (positive, negative) parts of 16 heads' codes */
     __shared__ float s_e[16];
-    __shared__ uint32_t s_bad, s_hist[256], s_scan[2][kWarps], s_thr, s_left, s_nz;
+    __shared__ uint32_t s_bad, s_hist[256], s_scan[2][kWarps], s_thr, s_left, s_nz, s_all, s_any;
     const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, j = lane & 3;
-    const uint32_t seq = blockIdx.x / a.n_kv_heads, head = blockIdx.x % a.n_kv_heads;
-    int32_t *out = a.picked + (size_t)blockIdx.x * a.n_pick;
+    const cg::cluster_group cluster = cg::this_cluster();
+    const uint32_t ranks = cluster.num_blocks(), rank = cluster.block_rank();
+    const uint32_t pair = blockIdx.x / ranks;                /* (sequence, kv head) */
+    const uint32_t seq = pair / a.n_kv_heads, head = pair % a.n_kv_heads;
+    int32_t *out = a.picked + (size_t)pair * a.n_pick;
+    uint32_t *lead = ranks > 1 ? cluster.map_shared_rank(keys, 0) : keys;
     const int32_t n = a.seq_lens[seq];
     const uint32_t cap = a.max_pages * a.page_tokens;
     const uint32_t len = n < 0 ? 0u : ((uint32_t)n > cap ? cap : (uint32_t)n);
@@ -62,7 +72,9 @@ __global__ void __launch_bounds__(kThreads) k_gqa_select(const ct_gqa_select_arg
     const uint32_t have = len ? (len - 1) / a.page_tokens - first + 1 : 0u;
     const int32_t *table = a.block_table + (size_t)seq * a.max_pages + first;
     const bool choose = have > a.n_pick;
-    if (tid == 0) { s_bad = 0; s_nz = 0; }
+    if (!choose && rank) return;                             /* the whole cluster decides alike: no barrier is missed */
+    if (choose && ranks > 1) cluster.sync();                 /* the first CTA runs: its shared memory may be written */
+    if (tid == 0) { s_bad = 0; s_nz = 0; s_all = 0xFFFFFFFFu; s_any = 0; }
     __syncthreads();
 
     const uint32_t n_tiles = (a.group + 15) / 16;
@@ -110,41 +122,63 @@ __global__ void __launch_bounds__(kThreads) k_gqa_select(const ct_gqa_select_arg
         const uint32_t rows = a.group - tile * 16 < 16 ? a.group - tile * 16 : 16;
         const float e0 = s_e[g], e1 = s_e[g + 8];
         const bool bad = s_bad != 0;
-        for (uint32_t p0 = warp * 8; p0 < have; p0 += kWarps * 8) {
-            const uint32_t p = p0 + g;
-            const int32_t ph = p < have ? table[p] : -1;
-            const bool ok = (uint32_t)ph < a.n_pages;
-            const size_t at = (size_t)(ok ? ph : 0) * a.n_kv_heads + head;
-            const uint4 *src = reinterpret_cast<const uint4 *>(a.bounds + at * 2 * D) + j;
-            uint4 w[D / 32];
+        constexpr uint32_t kStep = kTiles * 8;
+        const uint32_t pb = (uint32_t)((uint64_t)have * rank / ranks), pe = (uint32_t)((uint64_t)have * (rank + 1) / ranks);
+        int32_t ph[kTiles];
+        #pragma unroll
+        for (int t = 0; t < kTiles; t++) {
+            const uint32_t p = pb + warp * kStep + t * 8 + g;
+            ph[t] = p < pe ? __ldg(table + p) : -1;
+        }
+        for (uint32_t p0 = pb + warp * kStep; p0 < pe; p0 += kWarps * kStep) {
+            uint4 w[kTiles][D / 32];
+            float ps[kTiles];
+            bool ok[kTiles];
             #pragma unroll
-            for (int b = 0; b < D / 32; b++) w[b] = ok ? __ldg(src + b * 4) : make_uint4(0u, 0u, 0u, 0u);
-            const float ps = ok ? __ldg(a.bound_scales + at) : 0.0f;
-            int c[4] = {0, 0, 0, 0};
-            #pragma unroll
-            for (int b = 0; b < D / 32; b++) {
-                mma_s8(c, qa[2 * b], w[b].x, w[b].y);
-                mma_s8(c, qa[2 * b + 1], w[b].z, w[b].w);
-            }
-            float m[2];
-            #pragma unroll
-            for (int h = 0; h < 2; h++) {                    /* pages p0 + 2j + h */
-                m[h] = g < rows ? __fmul_rn((float)c[h], e0) : -INFINITY;
-                if (g + 8 < rows) m[h] = fmaxf(m[h], __fmul_rn((float)c[2 + h], e1));
+            for (int t = 0; t < kTiles; t++) {
+                ok[t] = (uint32_t)ph[t] < a.n_pages;
+                const size_t at = (size_t)(ok[t] ? ph[t] : 0) * a.n_kv_heads + head;
+                const uint4 *src = reinterpret_cast<const uint4 *>(a.bounds + at * 2 * D) + j;
                 #pragma unroll
-                for (int o = 4; o < 32; o <<= 1) m[h] = fmaxf(m[h], __shfl_xor_sync(0xFFFFFFFFu, m[h], o));
-                const float pscale = __shfl_sync(0xFFFFFFFFu, ps, (2 * j + h) * 4);
-                const bool pok = __shfl_sync(0xFFFFFFFFu, ok ? 1 : 0, (2 * j + h) * 4) != 0;
-                const uint32_t pp = p0 + 2 * j + h;
-                if (g == 0 && pp < have) {
-                    uint32_t key = bad ? kKeyInf : key_of(__fmul_rn(m[h], pscale));
-                    if (pp < a.n_first || pp + a.n_last >= have) key = kKeyForced;
-                    if (!pok) key = 0;
-                    keys[pp] = tile ? max(keys[pp], key) : key;
+                for (int b = 0; b < D / 32; b++) w[t][b] = ok[t] ? __ldg(src + b * 4) : make_uint4(0u, 0u, 0u, 0u);
+                ps[t] = ok[t] ? __ldg(a.bound_scales + at) : 0.0f;
+            }
+            #pragma unroll
+            for (int t = 0; t < kTiles; t++) {
+                const uint32_t p = p0 + kWarps * kStep + t * 8 + g;
+                ph[t] = p < pe ? __ldg(table + p) : -1;
+            }
+            #pragma unroll
+            for (int t = 0; t < kTiles; t++) {
+                int c[4] = {0, 0, 0, 0};
+                #pragma unroll
+                for (int b = 0; b < D / 32; b++) {
+                    mma_s8(c, qa[2 * b], w[t][b].x, w[t][b].y);
+                    mma_s8(c, qa[2 * b + 1], w[t][b].z, w[t][b].w);
+                }
+                #pragma unroll
+                for (int h = 0; h < 2; h++) {                /* pages p0 + 8t + 2j + h */
+                    float m = g < rows ? __fmul_rn((float)c[h], e0) : -INFINITY;
+                    if (g + 8 < rows) m = fmaxf(m, __fmul_rn((float)c[2 + h], e1));
+                    #pragma unroll
+                    for (int o = 4; o < 32; o <<= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
+                    const float pscale = __shfl_sync(0xFFFFFFFFu, ps[t], (2 * j + h) * 4);
+                    const bool pok = __shfl_sync(0xFFFFFFFFu, ok[t] ? 1 : 0, (2 * j + h) * 4) != 0;
+                    const uint32_t pp = p0 + t * 8 + 2 * j + h;
+                    if (g == 0 && pp < pe) {
+                        uint32_t key = bad ? kKeyInf : key_of(__fmul_rn(m, pscale));
+                        if (pp < a.n_first || pp + a.n_last >= have) key = kKeyForced;
+                        if (!pok) key = 0;
+                        lead[pp] = tile ? max(lead[pp], key) : key;
+                    }
                 }
             }
         }
         __syncthreads();
+    }
+    if (choose && ranks > 1) {
+        cluster.sync();                                      /* every rank's keys have reached the first CTA */
+        if (rank) return;
     }
     if (!choose)
         for (uint32_t p = tid; p < have; p += kThreads) keys[p] = (uint32_t)table[p] < a.n_pages ? 1u : 0u;
@@ -153,40 +187,59 @@ __global__ void __launch_bounds__(kThreads) k_gqa_select(const ct_gqa_select_arg
     /* ---- the key of the last page chosen ---- */
     uint32_t thr = 0, left = 0;                              /* keys above thr, and the first `left` equal to it, are chosen */
     if (choose) {
-        uint32_t nz = 0;
-        for (uint32_t p = tid; p < have; p += kThreads) nz += keys[p] != 0;
+        /* mapped pages, forced ones apart, and the bits in which the other keys differ */
+        uint32_t nz = 0, all = 0xFFFFFFFFu, any = 0;
+        for (uint32_t p = tid; p < have; p += kThreads) {
+            const uint32_t k = keys[p];
+            nz += (k != 0) + ((k == kKeyForced) << 16);
+            if (k != 0 && k != kKeyForced) { all &= k; any |= k; }
+        }
+        /* at most 49152 pages: both counts fit 16 bits of the sum */
         nz = __reduce_add_sync(0xFFFFFFFFu, nz);
-        if (lane == 0) atomicAdd(&s_nz, nz);
+        all = __reduce_and_sync(0xFFFFFFFFu, all);
+        any = __reduce_or_sync(0xFFFFFFFFu, any);
+        if (lane == 0) { atomicAdd(&s_nz, nz); atomicAnd(&s_all, all); atomicOr(&s_any, any); }
+        s_hist[tid] = 0;
         __syncthreads();
-        if (s_nz > a.n_pick) {
-            uint32_t want = a.n_pick, prefix = 0;
-            for (int shift = 24; shift >= 0; shift -= 8) {
-                s_hist[tid] = 0;
-                __syncthreads();
-                for (uint32_t p = tid; p < have; p += kThreads) {
-                    const uint32_t k = keys[p];
-                    if (shift == 24 || (k >> (shift + 8)) == (prefix >> (shift + 8))) atomicAdd(&s_hist[(k >> shift) & 255u], 1u);
+        if ((s_nz & 0xFFFFu) > a.n_pick) {
+            uint32_t want = a.n_pick - (s_nz >> 16);         /* forced pages come first */
+            if (want == 0) {
+                thr = kKeyForced - 1;
+            } else {
+                const uint32_t differ = s_all ^ s_any;
+                int shift = differ ? 24 - __clz(differ) : 0; /* lowest bit of the first pass's digit */
+                uint32_t prefix = s_all;                     /* the bits above the digits are the same in all */
+                uint32_t known = shift >= 24 ? 0u : 0xFFFFFFFFu << (shift < 0 ? 8 : shift + 8);
+                for (;;) {
+                    const int lo = shift < 0 ? 0 : shift;
+                    for (uint32_t p = tid; p < have; p += kThreads) {
+                        const uint32_t k = keys[p];
+                        if (k != 0 && k != kKeyForced && ((k ^ prefix) & known) == 0) atomicAdd(&s_hist[(k >> lo) & 255u], 1u);
+                    }
+                    __syncthreads();
+                    /* suffix counts over 256 bins; thread t looks at bin 255 - t */
+                    const uint32_t cnt = s_hist[255 - tid];
+                    uint32_t inc = cnt;
+                    #pragma unroll
+                    for (int o = 1; o < 32; o <<= 1) {
+                        const uint32_t y = __shfl_up_sync(0xFFFFFFFFu, inc, o);
+                        if (lane >= (uint32_t)o) inc += y;
+                    }
+                    if (lane == 31) s_scan[0][warp] = inc;
+                    __syncthreads();
+                    s_hist[tid] = 0;
+                    for (uint32_t w = 0; w < warp; w++) inc += s_scan[0][w];
+                    if (inc >= want && inc - cnt < want) { s_thr = 255 - tid; s_left = want - (inc - cnt); }
+                    __syncthreads();
+                    known = 0xFFFFFFFFu << lo;
+                    prefix = (prefix & ~(255u << lo)) | (s_thr << lo);
+                    want = s_left;
+                    if (lo == 0) break;
+                    shift -= 8;
                 }
-                __syncthreads();
-                /* suffix counts over 256 bins; thread t looks at bin 255 - t */
-                const uint32_t cnt = s_hist[255 - tid];
-                uint32_t inc = cnt;
-                #pragma unroll
-                for (int o = 1; o < 32; o <<= 1) {
-                    const uint32_t y = __shfl_up_sync(0xFFFFFFFFu, inc, o);
-                    if (lane >= (uint32_t)o) inc += y;
-                }
-                if (lane == 31) s_scan[0][warp] = inc;
-                __syncthreads();
-                for (uint32_t w = 0; w < warp; w++) inc += s_scan[0][w];
-                if (inc >= want && inc - cnt < want) { s_thr = 255 - tid; s_left = want - (inc - cnt); }
-                __syncthreads();
-                prefix |= s_thr << shift;
-                want = s_left;
-                __syncthreads();
+                thr = prefix;
+                left = want;
             }
-            thr = prefix;
-            left = want;
         }
     }
     /* ---- ascending pages: thread t owns a run of them ---- */
@@ -224,9 +277,23 @@ template <int D> int prepare() {
 }
 
 template <int D> int run(const ct_gqa_select_args_t *a, cudaStream_t st) {
-    k_gqa_select<D><<<a->n_seq * a->n_kv_heads, kThreads, (size_t)a->max_pages * 4, st>>>(*a);
+    /* CTAs for each (sequence, kv head): more than one when the batch leaves
+     * SMs idle and its rows are long enough to share. */
+    uint32_t ranks = 1;
+    while (ranks < 8 && 2 * ranks * a->n_seq * a->n_kv_heads <= a->n_sms && a->max_pages >= 256 * ranks) ranks *= 2;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(a->n_seq * a->n_kv_heads * ranks);
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = (size_t)a->max_pages * 4;
+    cfg.stream = st;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = ranks;
+    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
     ct__count_launches(1);
-    return ct__cuda_status(cudaGetLastError(), "gqa select");
+    return ct__cuda_status(cudaLaunchKernelEx(&cfg, k_gqa_select<D>, *a), "gqa select");
 }
 
 }  // namespace

@@ -19,7 +19,7 @@
 
 struct ct_gqa_plan {
     ct_gqa_shape_t shape;
-    uint32_t n_seq, n_workers;
+    uint32_t n_seq, n_workers, n_sms;
     int device;
     float *part_o, *part_ml;
     uint32_t *counters;
@@ -80,7 +80,7 @@ int ct_kv_gqa_write_slots(const ct_kv_gqa_layout_t *layout, void *pool, float *s
     if (rc || n == 0) return rc;
     if ((rc = check_pool(&l, pool, scales)) || (rc = check_rows(&l, k, v, &k_stride, &v_stride, src_dtype))) return rc;
     if (!dest_slot) return bad("gqa: no slots");
-    if ((uint64_t)n * 2 * l.n_kv_heads / 8 >= 0x7FFFFFFFu) return bad("gqa: too many rows in one call");
+    if (n > 0x7FFFFFFFu) return bad("gqa: too many tokens in one call");
     return ct__launch_gqa_write(pool, scales, l.kv_dtype, l.n_kv_heads, l.head_dim, l.page_tokens, l.n_pages, k, v, k_stride,
                                 v_stride, src_dtype == CT_KV_F32, dest_slot, n, stream);
 }
@@ -93,7 +93,7 @@ int ct_kv_gqa_read_slots(const ct_kv_gqa_layout_t *layout, const void *pool, con
     if (rc || n == 0) return rc;
     if ((rc = check_pool(&l, pool, scales)) || (rc = check_rows(&l, k_out, v_out, &k_stride, &v_stride, out_dtype))) return rc;
     if (!src_slot) return bad("gqa: no slots");
-    if ((uint64_t)n * 2 * l.n_kv_heads / 8 >= 0x7FFFFFFFu) return bad("gqa: too many rows in one call");
+    if (n > 0x7FFFFFFFu) return bad("gqa: too many tokens in one call");
     return ct__launch_gqa_read(pool, scales, l.kv_dtype, l.n_kv_heads, l.head_dim, l.page_tokens, l.n_pages, src_slot, n, k_out,
                                v_out, k_stride, v_stride, out_dtype == CT_KV_F32, stream);
 }
@@ -180,6 +180,7 @@ ct_gqa_plan_t *ct_gqa_plan_create(const ct_gqa_shape_t *shape, uint32_t n_seq, i
     if (!rc && ctas == 0) { ct__set_error("ct_gqa_plan_create: the decode kernel does not fit this device"); rc = CT_ERR_UNSUPPORTED; }
     if (!rc) rc = ct__gqa_select_prepare();
     if (!rc) {
+        p->n_sms = (uint32_t)n_sms;
         p->n_workers = (uint32_t)(n_sms * ctas);
         const size_t po = (size_t)2 * p->n_workers * 16 * l.head_dim * sizeof(float);
         const size_t pm = (size_t)2 * p->n_workers * 32 * sizeof(float), pc = (size_t)3 * p->n_workers * sizeof(uint32_t);
@@ -268,7 +269,7 @@ int ct_attn_gqa_select_pages(ct_gqa_plan_t *plan, const void *q, uint64_t q_stri
         .n_q_heads = plan->shape.n_q_heads, .n_kv_heads = l->n_kv_heads, .group = plan->shape.n_q_heads / l->n_kv_heads,
         .dim = l->head_dim, .page_tokens = l->page_tokens, .max_pages = l->max_pages_per_seq, .n_pages = l->n_pages,
         .n_pick = n_select, .n_first = n_first, .n_last = n_last, .window = plan->shape.window_tokens,
-        .blocked = plan->shape.head_order == CT_GQA_BLOCKED,
+        .blocked = plan->shape.head_order == CT_GQA_BLOCKED, .n_sms = plan->n_sms,
     };
     int prev = 0;
     if ((rc = enter(plan->device, &prev))) return rc;
