@@ -52,6 +52,7 @@ __global__ void __launch_bounds__(kThreads) k_gqa_write(void *pool, float *scale
     constexpr int L = lanes_of(D), U = D / 8, R = kThreads / L;
     const uint32_t u = threadIdx.x % L, place = blockIdx.y;
     const bool is_v = place >= n_kv_heads;
+    ct_gqa_enter();
     const uint32_t t0 = blockIdx.x * (R * T) + threadIdx.x / L;
     const size_t col = (size_t)(is_v ? place - n_kv_heads : place) * D + u * 8, stride = is_v ? v_stride : k_stride;
     const void *from = is_v ? vs : ks;
@@ -153,6 +154,7 @@ __global__ void __launch_bounds__(kThreads) k_gqa_read(const void *pool, const f
                                                        void *vo, size_t k_stride, size_t v_stride) {
     constexpr int L = lanes_of(D), U = D / 8, R = kThreads / L;
     const uint32_t u = threadIdx.x % L, place = blockIdx.y;
+    ct_gqa_enter();
     if (u >= U) return;
     const bool is_v = place >= n_kv_heads;
     const uint32_t t0 = blockIdx.x * (R * T) + threadIdx.x / L;
@@ -203,6 +205,7 @@ __global__ void __launch_bounds__(128) k_gqa_bounds(const void *pool, const floa
     constexpr int U = D / 8, R = 128 / U;                    /* threads along the row, tokens at a time */
     __shared__ float s_hi[R][D], s_lo[R][D];
     __shared__ uint32_t s_top[4], s_bad;
+    ct_gqa_enter();
     const uint32_t i = blockIdx.x / n_kv_heads, head = blockIdx.x % n_kv_heads;
     const int32_t page = pages[i];
     if (page < 0 || (uint32_t)page >= n_pages) return;
@@ -284,14 +287,13 @@ struct WriteCall {
     uint32_t n, heads, pt, np; cudaStream_t st;
     template <int D, int DT, bool F32> int go() const {
         constexpr uint32_t R = kThreads / lanes_of(D);
-        if (many(n, heads))
-            k_gqa_write<D, DT, F32, 4><<<dim3((n + 4 * R - 1) / (4 * R), 2 * heads), kThreads, 0, st>>>(pool, scales, k, v, ks, vs,
-                                                                                                        slots, n, heads, pt, np);
-        else
-            k_gqa_write<D, DT, F32, 1><<<dim3((n + R - 1) / R, 2 * heads), kThreads, 0, st>>>(pool, scales, k, v, ks, vs, slots, n,
-                                                                                              heads, pt, np);
         ct__count_launches(1);
-        return ct__cuda_status(cudaGetLastError(), "gqa write");
+        return ct__cuda_status(many(n, heads) ? launch(k_gqa_write<D, DT, F32, 4>, 4 * R) : launch(k_gqa_write<D, DT, F32, 1>, R),
+                               "gqa write");
+    }
+    template <class K> cudaError_t launch(K k_, uint32_t tokens) const {
+        return ct_gqa_launch(k_, dim3((n + tokens - 1) / tokens, 2 * heads), dim3(kThreads), 0, st, 1, pool, scales, k, v, ks, vs,
+                             slots, n, heads, pt, np);
     }
 };
 
@@ -300,14 +302,13 @@ struct ReadCall {
     cudaStream_t st;
     template <int D, int DT, bool F32> int go() const {
         constexpr uint32_t R = kThreads / lanes_of(D);
-        if (many(n, heads))
-            k_gqa_read<D, DT, F32, 4><<<dim3((n + 4 * R - 1) / (4 * R), 2 * heads), kThreads, 0, st>>>(pool, scales, slots, n, heads,
-                                                                                                       pt, np, k, v, ks, vs);
-        else
-            k_gqa_read<D, DT, F32, 1><<<dim3((n + R - 1) / R, 2 * heads), kThreads, 0, st>>>(pool, scales, slots, n, heads, pt, np, k,
-                                                                                             v, ks, vs);
         ct__count_launches(1);
-        return ct__cuda_status(cudaGetLastError(), "gqa read");
+        return ct__cuda_status(many(n, heads) ? launch(k_gqa_read<D, DT, F32, 4>, 4 * R) : launch(k_gqa_read<D, DT, F32, 1>, R),
+                               "gqa read");
+    }
+    template <class K> cudaError_t launch(K k_, uint32_t tokens) const {
+        return ct_gqa_launch(k_, dim3((n + tokens - 1) / tokens, 2 * heads), dim3(kThreads), 0, st, 1, pool, scales, slots, n, heads,
+                             pt, np, k, v, ks, vs);
     }
 };
 
@@ -323,12 +324,11 @@ template <int D, class Call> int by_type(const Call &c, uint32_t dtype, int f32)
 template <int D>
 int bounds_of(const void *pool, const float *scales, uint32_t dtype, uint32_t heads, uint32_t pt, uint32_t np, const int32_t *pages,
               const int32_t *counts, uint32_t n, int8_t *bounds, float *bs, cudaStream_t st) {
-    const unsigned grid = (unsigned)n * heads;
-    if (dtype == CT_KV_BF16) k_gqa_bounds<D, CT_KV_BF16><<<grid, 128, 0, st>>>(pool, scales, heads, pt, np, pages, counts, bounds, bs);
-    else if (dtype == CT_KV_INT8) k_gqa_bounds<D, CT_KV_INT8><<<grid, 128, 0, st>>>(pool, scales, heads, pt, np, pages, counts, bounds, bs);
-    else k_gqa_bounds<D, CT_KV_E4M3><<<grid, 128, 0, st>>>(pool, scales, heads, pt, np, pages, counts, bounds, bs);
+    auto kernel = dtype == CT_KV_BF16 ? k_gqa_bounds<D, CT_KV_BF16> : dtype == CT_KV_INT8 ? k_gqa_bounds<D, CT_KV_INT8>
+                                                                                     : k_gqa_bounds<D, CT_KV_E4M3>;
     ct__count_launches(1);
-    return ct__cuda_status(cudaGetLastError(), "gqa bounds");
+    return ct__cuda_status(ct_gqa_launch(kernel, dim3(n * heads), dim3(128), 0, st, 1, pool, scales, heads, pt, np, pages, counts,
+                                         bounds, bs), "gqa bounds");
 }
 
 }  // namespace

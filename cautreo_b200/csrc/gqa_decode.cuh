@@ -203,6 +203,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, DT, HT>::kMinB) k_gqa_decode(
     __shared__ uint32_t s_free[kWarps], s_last;
     const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, j = lane & 3;
     const uint32_t HV = a.n_kv_heads * a.n_tiles;
+    ct_gqa_enter();
 
     /* ---- this CTA's range of steps: from step s_end[0].step of item
      * s_end[0].ordinal to before step s_end[1].step of s_end[1].ordinal ---- */

@@ -20,9 +20,9 @@ template <int D, int DT, int HT> static int ctas() {
 }
 
 template <int D, int DT, int HT> static int run(const ct_gqa_args_t *a, uint32_t n_workers, cudaStream_t st) {
-    k_gqa_decode<D, DT, HT><<<n_workers, kThreads, Cfg<D, DT, HT>::kSmem, st>>>(*a);
     ct__count_launches(1);
-    return ct__cuda_status(cudaGetLastError(), "gqa decode");
+    return ct__cuda_status(ct_gqa_launch(k_gqa_decode<D, DT, HT>, dim3(n_workers), dim3(kThreads), Cfg<D, DT, HT>::kSmem, st, 1, *a),
+                           "gqa decode");
 }
 
 /* Groups of up to 8 query heads take one column tile, larger ones two. */

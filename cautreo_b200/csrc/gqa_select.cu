@@ -51,9 +51,9 @@ CT_DEV uint32_t key_of(float x) {
 }
 
 template <int D>
-__global__ void __launch_bounds__(kThreads) k_gqa_select(const ct_gqa_select_args_t a) {
+__global__ void __launch_bounds__(kThreads, D <= 128 ? 4 : 2) k_gqa_select(const ct_gqa_select_args_t a) {
     extern __shared__ __align__(16) uint32_t keys[];
-    constexpr int kPitch = 2 * D + 16;
+    constexpr int kPitch = 2 * D + 64;                       /* rows g, g + 1 in different halves of the banks */
     __shared__ __align__(16) int8_t s_q[16][kPitch];         /* (positive, negative) parts of 16 heads' codes */
     __shared__ float s_e[16];
     __shared__ uint32_t s_bad, s_hist[256], s_scan[2][kWarps], s_thr, s_left, s_nz, s_all, s_any;
@@ -64,6 +64,7 @@ __global__ void __launch_bounds__(kThreads) k_gqa_select(const ct_gqa_select_arg
     const uint32_t seq = pair / a.n_kv_heads, head = pair % a.n_kv_heads;
     int32_t *out = a.picked + (size_t)pair * a.n_pick;
     uint32_t *lead = ranks > 1 ? cluster.map_shared_rank(keys, 0) : keys;
+    ct_gqa_enter();
     const int32_t n = a.seq_lens[seq];
     const uint32_t cap = a.max_pages * a.page_tokens;
     const uint32_t len = n < 0 ? 0u : ((uint32_t)n > cap ? cap : (uint32_t)n);
@@ -109,16 +110,6 @@ __global__ void __launch_bounds__(kThreads) k_gqa_select(const ct_gqa_select_arg
             }
         }
         __syncthreads();
-        uint32_t qa[D / 16][4];
-        #pragma unroll
-        for (int b = 0; b < D / 32; b++) {                   /* 64 bytes of the row: lane j owns bytes 16 j .. 16 j + 15 */
-            #pragma unroll
-            for (int h = 0; h < 2; h++) {
-                const uint4 w = *reinterpret_cast<const uint4 *>(&s_q[g + 8 * h][b * 64 + 16 * j]);
-                qa[2 * b][h] = w.x; qa[2 * b][2 + h] = w.y;
-                qa[2 * b + 1][h] = w.z; qa[2 * b + 1][2 + h] = w.w;
-            }
-        }
         const uint32_t rows = a.group - tile * 16 < 16 ? a.group - tile * 16 : 16;
         const float e0 = s_e[g], e1 = s_e[g + 8];
         const bool bad = s_bad != 0;
@@ -148,18 +139,26 @@ __global__ void __launch_bounds__(kThreads) k_gqa_select(const ct_gqa_select_arg
                 const uint32_t p = p0 + kWarps * kStep + t * 8 + g;
                 ph[t] = p < pe ? __ldg(table + p) : -1;
             }
+            int c[kTiles][4];
+            #pragma unroll
+            for (int t = 0; t < kTiles; t++) c[t][0] = c[t][1] = c[t][2] = c[t][3] = 0;
+            #pragma unroll
+            for (int b = 0; b < D / 32; b++) {               /* 64 bytes of a row: lane j owns bytes 16 j .. 16 j + 15 */
+                const uint4 q0 = *reinterpret_cast<const uint4 *>(&s_q[g][b * 64 + 16 * j]);
+                const uint4 q1 = rows > 8 ? *reinterpret_cast<const uint4 *>(&s_q[g + 8][b * 64 + 16 * j]) : make_uint4(0u, 0u, 0u, 0u);
+                const uint32_t a0[4] = {q0.x, q1.x, q0.y, q1.y}, a1[4] = {q0.z, q1.z, q0.w, q1.w};
+                #pragma unroll
+                for (int t = 0; t < kTiles; t++) {
+                    mma_s8(c[t], a0, w[t][b].x, w[t][b].y);
+                    mma_s8(c[t], a1, w[t][b].z, w[t][b].w);
+                }
+            }
             #pragma unroll
             for (int t = 0; t < kTiles; t++) {
-                int c[4] = {0, 0, 0, 0};
-                #pragma unroll
-                for (int b = 0; b < D / 32; b++) {
-                    mma_s8(c, qa[2 * b], w[t][b].x, w[t][b].y);
-                    mma_s8(c, qa[2 * b + 1], w[t][b].z, w[t][b].w);
-                }
                 #pragma unroll
                 for (int h = 0; h < 2; h++) {                /* pages p0 + 8t + 2j + h */
-                    float m = g < rows ? __fmul_rn((float)c[h], e0) : -INFINITY;
-                    if (g + 8 < rows) m = fmaxf(m, __fmul_rn((float)c[2 + h], e1));
+                    float m = g < rows ? __fmul_rn((float)c[t][h], e0) : -INFINITY;
+                    if (g + 8 < rows) m = fmaxf(m, __fmul_rn((float)c[t][2 + h], e1));
                     #pragma unroll
                     for (int o = 4; o < 32; o <<= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
                     const float pscale = __shfl_sync(0xFFFFFFFFu, ps[t], (2 * j + h) * 4);
@@ -281,19 +280,10 @@ template <int D> int run(const ct_gqa_select_args_t *a, cudaStream_t st) {
      * SMs idle and its rows are long enough to share. */
     uint32_t ranks = 1;
     while (ranks < 8 && 2 * ranks * a->n_seq * a->n_kv_heads <= a->n_sms && a->max_pages >= 256 * ranks) ranks *= 2;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(a->n_seq * a->n_kv_heads * ranks);
-    cfg.blockDim = dim3(kThreads);
-    cfg.dynamicSmemBytes = (size_t)a->max_pages * 4;
-    cfg.stream = st;
-    cudaLaunchAttribute at[1];
-    at[0].id = cudaLaunchAttributeClusterDimension;
-    at[0].val.clusterDim.x = ranks;
-    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
-    cfg.attrs = at;
-    cfg.numAttrs = 1;
     ct__count_launches(1);
-    return ct__cuda_status(cudaLaunchKernelEx(&cfg, k_gqa_select<D>, *a), "gqa select");
+    return ct__cuda_status(ct_gqa_launch(k_gqa_select<D>, dim3(a->n_seq * a->n_kv_heads * ranks), dim3(kThreads),
+                                         (size_t)a->max_pages * 4, st, ranks, *a),
+                           "gqa select");
 }
 
 }  // namespace
