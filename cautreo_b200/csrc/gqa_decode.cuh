@@ -45,7 +45,10 @@
 
 namespace ct_gqa {
 
-constexpr int kWarps = 4;
+#ifndef GQ_WARPS
+#define GQ_WARPS 4
+#endif
+constexpr int kWarps = GQ_WARPS;
 constexpr int kThreads = kWarps * 32;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
@@ -53,7 +56,24 @@ constexpr float kGrow = 8.0f;           /* log2 growth of a maximum that is foll
 constexpr float kNoMax = -3.402823466e38f;  /* maximum of no tokens: finite, so that no difference of maxima is NaN */
 constexpr float kTopWeight = 32768.0f;  /* fp16 weights stay below this */
 constexpr uint32_t kItemCost = 4;       /* steps that an item's start and end are counted as */
-constexpr uint32_t kSolo = 8;           /* steps up to which an item is one warp's, if the CTA has items for every warp */
+#ifndef GQ_CMIN
+#define GQ_CMIN 12u
+#endif
+#ifndef GQ_CDIV
+#define GQ_CDIV 4
+#endif
+#ifndef GQ_CMAX
+#define GQ_CMAX 40u
+#endif
+#define GQ_CUT max(GQ_CMIN, min(Q / GQ_CDIV, GQ_CMAX))
+#ifndef GQ_SOLO
+#define GQ_SOLO 16
+#endif
+constexpr uint32_t kSoloMost = GQ_SOLO; /* longest item of one warp: longer ones would leave the others idle at the end */
+constexpr uint32_t kSoloCost = 3;       /* start and end of an item, in steps of one warp, */
+constexpr uint32_t kShareCost = 10;     /* and of one that the warps share */
+constexpr uint32_t kWhole = 8;          /* items of at most so many steps are not cut between CTAs */
+constexpr uint32_t kFewSteps = 32;      /* steps a CTA up to which a part of one item each is the better split */
 constexpr uint32_t kFan = 16;           /* workers whose parts are joined at a time, when an item has more than 2 kFan */
 
 /* Tokens of a warp's step, steps in its ring, CTAs that an SM holds. */
@@ -61,10 +81,10 @@ constexpr uint32_t kFan = 16;           /* workers whose parts are joined at a t
 #define GQ_TS (kRow <= 64 ? 32 : 16)
 #endif
 #ifndef GQ_S
-#define GQ_S 3
+#define GQ_S (kElt == 1 && HT * D == 512 ? 2 : 3)
 #endif
 #ifndef GQ_MINB
-#define GQ_MINB 1
+#define GQ_MINB (HT == 1 && D <= 128 && (kElt == 1 || D <= 64) ? 3 : 1)
 #endif
 template <int D, int DT, int HT> struct Cfg {
     static constexpr int kElt = DT == CT_KV_BF16 ? 2 : 1;
@@ -207,9 +227,46 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, DT, HT>::kMinB) k_gqa_decode(
 
     /* ---- this CTA's range of steps: from step s_end[0].step of item
      * s_end[0].ordinal to before step s_end[1].step of s_end[1].ordinal ---- */
-    const uint32_t per = (a.n_seq + kThreads - 1) / kThreads;
-    auto scan = [&](uint32_t v, uint32_t &all) -> uint32_t { /* exclusive sum over the threads */
-        uint32_t incl = v;
+    bool few = 2ull * a.n_seq * HV <= gridDim.x;
+    if (few) {                                               /* each warp for itself: no barrier */
+        uint32_t sum = 0;
+        #pragma unroll 1
+        for (uint32_t s = lane; s < a.n_seq; s += 32) sum += sequence<TS>(a, s).steps;
+        sum = __reduce_add_sync(0xFFFFFFFFu, sum);
+        few = (uint64_t)sum * HV <= (uint64_t)kFewSteps * gridDim.x;
+        if (few) {
+            const uint32_t Q = max(a.min_steps, (sum * HV - 1) / (gridDim.x - a.n_seq * HV) + 1);
+            uint32_t at = 0, all = 0;                        /* parts before the sequences at hand */
+            #pragma unroll 1
+            for (uint32_t s0 = 0; s0 < a.n_seq; s0 += 32) {
+                const uint32_t s = s0 + lane, steps = s < a.n_seq ? sequence<TS>(a, s).steps : 0u, n = (steps + Q - 1) / Q;
+                uint32_t incl = n * HV;
+                #pragma unroll
+                for (int o = 1; o < 32; o <<= 1) {
+                    const uint32_t y = __shfl_up_sync(0xFFFFFFFFu, incl, o);
+                    if (lane >= (uint32_t)o) incl += y;
+                }
+                const uint32_t x = blockIdx.x - (all + incl - n * HV);
+                if (n && blockIdx.x >= all + incl - n * HV && x < n * HV && warp == 0) {
+                    const uint32_t item = x / n, part = x - item * n, first = blockIdx.x - part;
+                    s_end[0] = {s * HV + item, steps * part / n, first, first + n - 1};
+                    s_end[1] = {s * HV + item, steps * (part + 1) / n, first, first + n - 1};
+                }
+                all += __shfl_sync(0xFFFFFFFFu, incl, 31);
+                at = all;
+            }
+            if (blockIdx.x >= at) return;
+        }
+    }
+    if (!few) {
+        const uint32_t per = (a.n_seq + kThreads - 1) / kThreads;
+        uint32_t sum = 0;
+        #pragma unroll 1
+        for (uint32_t i = 0; i < per; i++) {
+            const uint32_t s = tid * per + i;
+            if (s < a.n_seq) sum += sequence<TS>(a, s).steps + kItemCost;
+        }
+        uint32_t incl = sum;
         #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
             const uint32_t y = __shfl_up_sync(0xFFFFFFFFu, incl, o);
@@ -217,72 +274,43 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, DT, HT>::kMinB) k_gqa_decode(
         }
         if (lane == 31) s_scan[warp] = incl;
         __syncthreads();
-        uint32_t before = 0;
-        all = 0;
+        uint32_t before = 0, all = 0;
         #pragma unroll
         for (int w = 0; w < kWarps; w++) {
             if (w < (int)warp) before += s_scan[w];
             all += s_scan[w];
         }
-        __syncthreads();
-        return before + incl - v;
-    };
-    const bool few = 2ull * a.n_seq * HV <= gridDim.x;       /* a part of one item each */
-    uint32_t sum = 0, all;
-    for (uint32_t i = 0; i < per; i++) {
-        const uint32_t s = tid * per + i;
-        if (s < a.n_seq) sum += sequence<TS>(a, s).steps + (few ? 0u : kItemCost);
-    }
-    uint32_t excl = scan(sum, all);
-    if (few) {
-        const uint32_t workers = gridDim.x - a.n_seq * HV;
-        const uint32_t Q = max(a.min_steps, (uint32_t)(((uint64_t)all * HV + workers - 1) / workers));
-        sum = 0;
-        for (uint32_t i = 0; i < per; i++) {
-            const uint32_t s = tid * per + i;
-            if (s < a.n_seq) sum += (sequence<TS>(a, s).steps + Q - 1) / Q;
-        }
-        excl = scan(sum, all);                               /* parts of the sequences' items */
-        if (blockIdx.x >= all * HV) return;
-        if (blockIdx.x >= excl * HV && blockIdx.x < (excl + sum) * HV) {
-            uint32_t x = blockIdx.x - excl * HV, s = tid * per, steps, n;
-            for (;; s++) {
-                steps = sequence<TS>(a, s).steps;
-                n = (steps + Q - 1) / Q;
-                if (x < n * HV) break;
-                x -= n * HV;
-            }
-            const uint32_t item = x / n, part = x % n, first = blockIdx.x - part;
-            const End e = {s * HV + item, (uint32_t)((uint64_t)steps * part / n), first, first + n - 1};
-            s_end[0] = e;
-            s_end[1] = e;
-            s_end[1].step = (uint32_t)((uint64_t)steps * (part + 1) / n);
-        }
-    } else {
-        const uint64_t total = (uint64_t)all * HV;
-        const uint64_t Q = max((uint64_t)a.min_steps, (total + gridDim.x - 1) / gridDim.x);
+        const uint64_t total = (uint64_t)all * HV, excl = (uint64_t)(before + incl - sum) * HV, next = excl + (uint64_t)sum * HV;
+        const uint32_t Q = max(a.min_steps, (uint32_t)__umul64hi(total + gridDim.x - 1, a.worker_magic));
         const uint64_t x0 = (uint64_t)blockIdx.x * Q;
         if (x0 >= total) return;
+        if (tid == 0 && x0 + Q >= total) s_end[1] = {a.n_seq * HV, 0u, 0u, 0u};
         #pragma unroll 1
-        for (int b = 0; b < 2; b++) {                        /* the range's first and last unit */
-            const uint64_t x = b ? min(x0 + Q, total) - 1 : x0;
-            if (x < (uint64_t)excl * HV || x >= (uint64_t)(excl + sum) * HV) continue;
-            uint64_t at = (uint64_t)excl * HV;
+        for (uint32_t b = 0; b < 2; b++) {                   /* where the range begins, where the next one does */
+            const uint64_t x = x0 + b * Q;
+            if (x < excl || x >= next) continue;
+            uint64_t at = excl;
             uint32_t s = tid * per, width;
+            #pragma unroll 1
             for (;; s++) {
                 width = sequence<TS>(a, s).steps + kItemCost;
                 if (x < at + (uint64_t)width * HV) break;
                 at += (uint64_t)width * HV;
             }
-            const uint32_t item = (uint32_t)((x - at) / width), in = (uint32_t)((x - at) % width) + b;
-            const uint64_t item_x = at + (uint64_t)item * width;
-            s_end[b] = {s * HV + item, in > kItemCost ? in - kItemCost : 0u, (uint32_t)((item_x + kItemCost) / Q),
-                        (uint32_t)((item_x + width - 1) / Q)};
+            const uint32_t rel = (uint32_t)(x - at), item = rel / width;          /* below 2^32: see the plan */
+            uint32_t in = rel - item * width;
+            if (width <= GQ_CUT) in = 0;                     /* a short item goes to the later CTA as a whole */
+            const uint32_t step = in > kItemCost ? in - kItemCost : 0u;
+            /* workers that hold steps of the item: from the one of its first
+             * step (this one if the item begins here) to that of its last */
+            const uint32_t here = blockIdx.x + b;
+            s_end[b] = {s * HV + item, step, here - (step + Q - 1) / Q, here + (width - 1 - in) / Q};
         }
     }
     __syncthreads();
-    const uint32_t o0 = s_end[0].ordinal, o1 = s_end[1].ordinal;
-    const uint32_t range = o1 - o0 + 1;
+    const uint32_t o0 = s_end[0].ordinal;
+    const uint32_t range = s_end[1].ordinal - o0 + (s_end[1].step ? 1u : 0u);      /* items */
+    if (range == 0) return;
 
     uint8_t *ring = smem + warp * (S * C::kStage);
     const uint32_t ring_a = smem_u32(ring);
@@ -307,17 +335,20 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, DT, HT>::kMinB) k_gqa_decode(
     };
     auto bounds = [&](Segment &z, uint32_t at) {             /* of item o0 + at, which z.seq and z.item name */
         z.sb = at == 0 ? s_end[0].step : 0u;
-        z.se = at + 1 == range ? s_end[1].step : z.sq.steps;
-        const bool cut = z.sb > 0 || z.se < z.sq.steps;
-        z.solo = !cut && (z.sq.steps == 1 || (z.sq.steps <= kSolo && range >= (uint32_t)kWarps));
-        if (z.se <= z.sb) {                                  /* only overhead fell into this range */
-            z.wb = z.we = 0;
-        } else if (z.solo) {
+        z.se = at + 1 == range && s_end[1].step ? s_end[1].step : z.sq.steps;
+        const uint32_t n = z.se - z.sb;
+        /* A whole item is one warp's if there is nothing to share, or if the
+         * range's whole items, handed out one by one, take
+         * less of the warps' time so than shared. */
+        const uint32_t items = range - (s_end[0].step ? 1u : 0u) - (s_end[1].step ? 1u : 0u), rounds = (items + kWarps - 1) / kWarps;
+        z.solo = n == z.sq.steps && (n == 1 || (n <= kSoloMost && items > 1 &&
+                                                kWarps * rounds * (n + kSoloCost) <= items * (n + kShareCost)));
+        if (z.solo) {
             z.wb = z.sb;
             z.we = (at & (kWarps - 1)) == warp ? z.se : z.sb;
-        } else {
-            z.wb = z.sb + (uint32_t)((uint64_t)(z.se - z.sb) * warp / kWarps);
-            z.we = z.sb + (uint32_t)((uint64_t)(z.se - z.sb) * (warp + 1) / kWarps);
+        } else {                                             /* n below 2^28: four times it fits */
+            z.wb = z.sb + n * warp / kWarps;
+            z.we = z.sb + n * (warp + 1) / kWarps;
         }
     };
     auto step_on = [&](Segment &z) {
@@ -345,105 +376,93 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, DT, HT>::kMinB) k_gqa_decode(
      * (list entries: two pages) before they are needed. */
     Segment pz;
     begin(pz);
-    uint32_t p_at = 0, left = 0, page_e = 0, off = 0, pos = 0, lp_next = 0, ph_next = 0, lp_then = 0;
+    uint32_t p_at = 0xFFFFFFFFu, left = 0, page_e = 0, off = 0, pos = 0, lp_next = 0, ph_next = 0, lp_then = 0;
     const uint8_t *kp = nullptr;
     const float *sp = nullptr;
-    bool page_ok = false;
-    auto open_page = [&](uint32_t lp, uint32_t ph) {
-        page_ok = ph < a.n_pages;
-        const size_t row = ((size_t)(page_ok ? ph : 0u) * 2 * a.n_kv_heads + pz.item / a.n_tiles) * a.page_tokens + off;
-        kp = static_cast<const uint8_t *>(a.pool) + row * C::kRow + lane * 16;
-        if (kQ8) sp = a.scales + row + (lane >> 2) * (size_t)a.n_kv_heads * a.page_tokens + (lane & 3) * 4;
-        pos = page_ok ? lp * a.page_tokens + off : 0u;
-    };
-    /* Looks for this warp's next segment with steps (the first at entry), and
-     * loads the numbers of its first pages into the `next` of the cursor. */
-    bool opened = true;
-    auto find = [&](bool go_on) {
-        if (go_on) { p_at++; if (p_at < range) step_on(pz); }
-        for (; p_at < range; p_at++) {
-            bounds(pz, p_at);
-            if (pz.we > pz.wb) break;
-            if (p_at + 1 < range) step_on(pz);
-        }
-        if (p_at >= range) return;
-        left = pz.we - pz.wb;
-        const uint32_t v = first_token(pz.sq) + pz.wb * TS;
-        page_e = a.page_of(v);
-        off = v - page_e * a.page_tokens;
-        lp_next = entry(pz, page_e);
-        lp_then = entry(pz, page_e + 1);
-        ph_next = mapped(pz, lp_next);
-        opened = false;
-    };
-    auto turn_page = [&](uint32_t e) {                       /* opens the page at hand, e-th of the segment; looks up the one after */
-        open_page(lp_next, ph_next);
-        page_e = e;
-        lp_next = lp_then;
-        ph_next = mapped(pz, lp_next);
-        lp_then = entry(pz, e + 2);
-    };
-    /* Starts the copies of the next step into ring slot st; whether the step
-     * has every one of its tokens.  Dropped tokens become zeros. */
-    auto fetch = [&](uint32_t st) -> bool {
-        constexpr int CPR = C::kRow / 16, N = 16 * CPR;      /* 16-byte chunks of a row, of a group */
-        bool whole = true;
-        if (!opened) { turn_page(page_e); opened = true; }
-        #pragma unroll
-        for (int gr = 0; gr < GR; gr++) {
-            const uint32_t to = ring_a + st * C::kStage + gr * 16 * kPitch;
-            const uint32_t to_s = ring_a + st * C::kStage + 2 * TS * kPitch + ((lane >> 2) * TS + gr * 16 + (lane & 3) * 4) * 4;
-            const uint8_t *vp = kp + v_off;
-            const bool full = page_ok && pos >= pz.sq.start && pos + 16 <= pz.sq.len;
-            whole = whole && full;
-            if (full) {
-                #pragma unroll
-                for (int c0 = 0; c0 < N; c0 += 32) {
-                    const uint32_t c = c0 + lane;
-                    if (N % 32 != 0 && c >= (uint32_t)N) continue;
-                    const uint32_t d = to + (c / CPR) * kPitch + (c % CPR) * 16;
-                    cp_async16(d, kp + c0 * 16);
-                    cp_async16(d + TS * kPitch, vp + c0 * 16);
+    bool page_ok = false, turn = false, done = false;
+    uint32_t whole_slots = 0, fill = 0;                      /* bit per ring slot; slot of the next copies */
+    /* Starts the copies of this warp's next step (tokens that the mask drops
+     * become zeros), then, if that was the last of its segment, looks for the
+     * next segment and loads the numbers of its first pages. */
+    auto advance = [&]() {
+        if (left) {
+            constexpr int CPR = C::kRow / 16, N = 16 * CPR;  /* 16-byte chunks of a row, of a group */
+            bool whole = true;
+            #pragma unroll 1
+            for (uint32_t gr = 0; gr < (uint32_t)GR; gr++) {
+                if (turn) {                                  /* open the page at hand, look up the one after */
+                    page_ok = ph_next < a.n_pages;
+                    const size_t row = ((size_t)(page_ok ? ph_next : 0u) * 2 * a.n_kv_heads + pz.item / a.n_tiles) * a.page_tokens + off;
+                    kp = static_cast<const uint8_t *>(a.pool) + row * C::kRow + lane * 16;
+                    if (kQ8) sp = a.scales + row + (lane >> 2) * (size_t)a.n_kv_heads * a.page_tokens + (lane & 3) * 4;
+                    pos = page_ok ? lp_next * a.page_tokens + off : 0u;
+                    lp_next = lp_then;
+                    ph_next = mapped(pz, lp_next);
+                    lp_then = entry(pz, page_e + 2);
+                    page_e++;
+                    turn = false;
                 }
-                if (kQ8 && lane < 8) cp_async16(to_s, sp);   /* 16 scales of K, 16 of V */
-            } else {
-                const uint32_t lo = pos < pz.sq.start ? pz.sq.start - pos : 0u;      /* tokens [lo, hi) of the group are kept */
-                const uint32_t hi = !page_ok || pos >= pz.sq.len ? 0u : (pz.sq.len - pos < 16u ? pz.sq.len - pos : 16u);
-                #pragma unroll 1
-                for (uint32_t c = lane; c < (uint32_t)N; c += 32) {
-                    const uint32_t row = c / CPR, d = to + row * kPitch + (c % CPR) * 16;
-                    const uint32_t bytes = row >= lo && row < hi ? 16u : 0u;
-                    cp_async16_part(d, kp + (c - lane) * 16, bytes);
-                    cp_async16_part(d + TS * kPitch, vp + (c - lane) * 16, bytes);
+                const uint32_t to = ring_a + fill * C::kStage + gr * 16 * kPitch;
+                const uint32_t to_s = ring_a + fill * C::kStage + 2 * TS * kPitch + ((lane >> 2) * TS + gr * 16 + (lane & 3) * 4) * 4;
+                const uint8_t *vp = kp + v_off;
+                if (page_ok && pos >= pz.sq.start && pos + 16 <= pz.sq.len) {
+                    #pragma unroll
+                    for (int c0 = 0; c0 < N; c0 += 32) {
+                        const uint32_t c = c0 + lane;
+                        if (N % 32 != 0 && c >= (uint32_t)N) continue;
+                        const uint32_t d = to + (c / CPR) * kPitch + (c % CPR) * 16;
+                        cp_async16(d, kp + c0 * 16);
+                        cp_async16(d + TS * kPitch, vp + c0 * 16);
+                    }
+                    if (kQ8 && lane < 8) cp_async16(to_s, sp);           /* 16 scales of K, 16 of V */
+                } else {
+                    whole = false;
+                    const uint32_t lo = pos < pz.sq.start ? pz.sq.start - pos : 0u;      /* tokens [lo, hi) of the group are kept */
+                    const uint32_t hi = !page_ok || pos >= pz.sq.len ? 0u : (pz.sq.len - pos < 16u ? pz.sq.len - pos : 16u);
+                    #pragma unroll 1
+                    for (uint32_t c = lane; c < (uint32_t)N; c += 32) {
+                        const uint32_t row = c / CPR, d = to + row * kPitch + (c % CPR) * 16;
+                        const uint32_t bytes = row >= lo && row < hi ? 16u : 0u;
+                        cp_async16_part(d, kp + (c - lane) * 16, bytes);
+                        cp_async16_part(d + TS * kPitch, vp + (c - lane) * 16, bytes);
+                    }
+                    if (kQ8 && lane < 8) {
+                        const uint32_t tk = (lane & 3) * 4;
+                        cp_async16_part(to_s, sp, (hi > tk ? (hi - tk < 4u ? hi - tk : 4u) : 0u) * 4);
+                    }
                 }
-                if (kQ8 && lane < 8) {
-                    const uint32_t tk = (lane & 3) * 4;
-                    cp_async16_part(to_s, sp, (hi > tk ? (hi - tk < 4u ? hi - tk : 4u) : 0u) * 4);
-                }
+                pos += 16;
+                kp += 16 * C::kRow;
+                if (kQ8) sp += 16;
+                off += 16;
+                if (off == a.page_tokens) { off = 0; turn = true; }
             }
-            off += 16;
-            pos += 16;
-            kp += 16 * C::kRow;
-            if (kQ8) sp += 16;
-            if (off == a.page_tokens) {
-                off = 0;
-                turn_page(page_e + 1);
-            }
-        }
-        return whole;
-    };
-    uint32_t whole_slots = 0;                                /* bit per ring slot */
-    auto advance = [&](uint32_t st) {
-        if (p_at < range) {
-            whole_slots = fetch(st) ? whole_slots | (1u << st) : whole_slots & ~(1u << st);
-            if (--left == 0) find(true);
+            whole_slots = whole ? whole_slots | (1u << fill) : whole_slots & ~(1u << fill);
+            fill = fill + 1 == S ? 0 : fill + 1;
+            left--;
         }
         cp_commit();
+        if (left == 0 && !done) {
+            #pragma unroll 1
+            do {
+                if (++p_at == range) { done = true; break; }
+                if (p_at) step_on(pz);
+                bounds(pz, p_at);
+                left = pz.we - pz.wb;
+            } while (left == 0);
+            if (left) {
+                const uint32_t v = first_token(pz.sq) + pz.wb * TS;
+                page_e = a.page_of(v);
+                off = v - page_e * a.page_tokens;
+                lp_next = entry(pz, page_e);
+                lp_then = entry(pz, page_e + 1);
+                ph_next = mapped(pz, lp_next);
+                turn = true;
+            }
+        }
     };
-    find(false);
-    #pragma unroll 1
-    for (int st = 0; st < S - 1; st++) advance(st);
     uint32_t slot = 0;                                       /* slot of the next step; the one before it is free */
+    int prime = S;                                           /* the first call looks for a segment, S - 1 fill the ring */
 
     /* ---- arithmetic ---- */
     Segment z;
@@ -452,7 +471,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, DT, HT>::kMinB) k_gqa_decode(
     for (uint32_t at = 0; at < range; at++) {
         if (at) step_on(z);
         bounds(z, at);
-        if (z.se <= z.sb || (z.solo && z.we == z.wb)) continue;          /* nothing, or another warp's */
+        if (z.solo && z.we == z.wb) continue;                /* another warp's */
         const uint32_t seq = z.seq, tile = z.item % a.n_tiles, head = z.item / a.n_tiles;
         const uint32_t rows = a.group - tile * 16 < 16 ? a.group - tile * 16 : 16;
         const bool cut = z.sb > 0 || z.se < z.sq.steps;
@@ -536,8 +555,9 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, DT, HT>::kMinB) k_gqa_decode(
             for (int h = 0; h < 2; h++) { m[t][h] = kNoMax; l[t][h] = 0.0f; unit[t][h] = 0; }
 
         #pragma unroll 1
-        for (uint32_t i = z.wb; i < z.we; i++) {
-            advance(slot == 0 ? S - 1 : slot - 1);                       /* refill the slot that the last step freed */
+        for (uint32_t i = z.wb; i < z.we;) {
+            advance();                                       /* refill the slot that the last step freed */
+            if (prime) { prime--; continue; }
             cp_wait<S - 1>();
             __syncwarp();
             const uint32_t stage = ring_a + slot * C::kStage;
@@ -734,10 +754,10 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, DT, HT>::kMinB) k_gqa_decode(
             }
             __syncwarp();                                    /* the slot may be refilled */
             slot = slot + 1 == S ? 0 : slot + 1;
+            i++;
         }
 
         /* ---- join the warps (a short item has one) ---- */
-        const uint32_t w0 = z.solo ? warp : 0u, w1 = z.solo ? warp + 1 : (uint32_t)kWarps;
         const uint32_t part = 2 * blockIdx.x + (z.sb > 0 ? 0u : 1u);
         float *po = a.part_o + (size_t)part * 16 * D;
         float *pml = a.part_ml + (size_t)part * 32;
@@ -783,17 +803,24 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, DT, HT>::kMinB) k_gqa_decode(
                 }
             }
             if (z.solo) __syncwarp(); else __syncthreads();
+            #pragma unroll 1
             for (uint32_t c = z.solo ? lane : tid; c < rows * (kJoinCols / 4); c += z.solo ? 32u : (uint32_t)kThreads) {
                 const uint32_t r = c / (kJoinCols / 4), dj = (c % (kJoinCols / 4)) * 4, d = d0 + dj;
-                float M = kNoMax;
-                for (uint32_t w = w0; w < w1; w++) M = fmaxf(M, s_ml[w][r][0]);
-                float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                float L = 0.0f;
-                for (uint32_t w = w0; w < w1; w++) {
-                    const float f = ex2(s_ml[w][r][0] - M);
-                    const float4 v = *reinterpret_cast<const float4 *>(smem + s_free[w] + (r * kJoin + dj) * 4);
-                    L += s_ml[w][r][1] * f;
-                    acc.x += v.x * f; acc.y += v.y * f; acc.z += v.z * f; acc.w += v.w * f;
+                float M = s_ml[warp][r][0], L = s_ml[warp][r][1];
+                float4 acc = *reinterpret_cast<const float4 *>(smem + s_free[warp] + (r * kJoin + dj) * 4);
+                if (!z.solo) {
+                    M = kNoMax;
+                    #pragma unroll
+                    for (int w = 0; w < kWarps; w++) M = fmaxf(M, s_ml[w][r][0]);
+                    acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                    L = 0.0f;
+                    #pragma unroll
+                    for (int w = 0; w < kWarps; w++) {
+                        const float f = ex2(s_ml[w][r][0] - M);
+                        const float4 v = *reinterpret_cast<const float4 *>(smem + s_free[w] + (r * kJoin + dj) * 4);
+                        L += s_ml[w][r][1] * f;
+                        acc.x += v.x * f; acc.y += v.y * f; acc.z += v.z * f; acc.w += v.w * f;
+                    }
                 }
                 if (cut) {
                     __stcg(reinterpret_cast<float4 *>(po + r * D + d), acc);
@@ -819,6 +846,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, DT, HT>::kMinB) k_gqa_decode(
                 lo = max(lo, first);
             }
             bool last_here = true;
+            #pragma unroll 1
             for (int round = 0; last_here && round < (tree ? 2 : 1); round++) {
                 /* three sets of counters: an item's, by its first worker; a
                  * run's, by its first worker, apart for the run that an item
@@ -849,6 +877,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, DT, HT>::kMinB) k_gqa_decode(
                     const uint32_t c = r * n + k;
                     return reinterpret_cast<float2 *>(smem + s_free[c / kPer])[c % kPer];
                 };
+                #pragma unroll 1
                 for (uint32_t c = tid; c < n * rows; c += kThreads) {
                     const uint32_t r = c / n, k = c % n;
                     s_part(k, r) = __ldcg(reinterpret_cast<const float2 *>(a.part_ml + (size_t)slot_of(k) * 32) + r);
@@ -856,11 +885,14 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, DT, HT>::kMinB) k_gqa_decode(
                 __syncthreads();
                 const uint32_t to = slot_of(0);
                 const bool more = tree && round == 0;
+                #pragma unroll 1
                 for (uint32_t c = tid; c < rows * (D / 4); c += kThreads) {
                     const uint32_t r = c / (D / 4), d = (c % (D / 4)) * 4;
                     float M = kNoMax, L = 0.0f;
+                    #pragma unroll 1
                     for (uint32_t k = 0; k < n; k++) M = fmaxf(M, s_part(k, r).x);
                     float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                    #pragma unroll 1
                     for (uint32_t k0 = 0; k0 < n; k0 += 8) {
                         float4 v[8];
                         #pragma unroll

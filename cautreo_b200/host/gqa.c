@@ -225,6 +225,7 @@ static int decode(ct_gqa_plan_t *p, const void *q, uint64_t q_stride, const void
         .max_pages = l->max_pages_per_seq, .n_pages = l->n_pages, .n_pick = n_select, .window = p->shape.window_tokens,
         .blocked = p->shape.head_order == CT_GQA_BLOCKED, .min_steps = getenv("GQMIN") ? (uint32_t)atoi(getenv("GQMIN")) : 8,
         .scale_log2 = p->shape.scale * 1.4426950408889634f,
+        .worker_magic = UINT64_MAX / p->n_workers + 1,
         .page_magic = page_groups == 1 ? 0u : (uint32_t)(0x100000000ull / page_groups) + 1u,
     };
     int prev = 0;
