@@ -181,6 +181,7 @@ template <int DT, bool Even> CT_DEV void widen(uint32_t w, uint32_t &a, uint32_t
 struct Seq {
     uint32_t len, start;                                     /* tokens [start, len) are attended */
     uint32_t n_list;                                         /* listed pages stepped over */
+    uint32_t pages;                                          /* of the whole sequence, at most max_pages */
     uint32_t steps;
 };
 template <int TS> CT_DEV Seq sequence(const ct_gqa_args_t &a, uint32_t s) {
@@ -190,9 +191,10 @@ template <int TS> CT_DEV Seq sequence(const ct_gqa_args_t &a, uint32_t s) {
     r.len = n < 0 ? 0u : ((uint32_t)n > cap ? cap : (uint32_t)n);
     r.start = a.window && r.len > a.window ? r.len - a.window : 0u;
     r.n_list = 0;
+    r.pages = r.len ? a.page_of(r.len - 1) + 1 : 0u;
     uint32_t v;                                              /* tokens to step over */
     if (a.picked) {                                          /* listed pages: as many as the window has, at most */
-        const uint32_t have = r.len ? a.page_of(r.len - 1) - a.page_of(r.start) + 1 : 0u;
+        const uint32_t have = r.len ? r.pages - a.page_of(r.start) : 0u;
         r.n_list = have < a.n_pick ? have : a.n_pick;
         v = r.n_list * a.page_tokens;
     } else {
@@ -366,77 +368,90 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, DT, HT>::kMinB) k_gqa_decode(
     };
     /* Its physical page (>= n_pages: nothing to read). */
     auto mapped = [&](const Segment &z, uint32_t lp) -> uint32_t {
-        return lp < a.max_pages && lp * a.page_tokens < z.sq.len ? (uint32_t)__ldg(a.block_table + (size_t)z.seq * a.max_pages + lp)
+        return lp < z.sq.pages ? (uint32_t)__ldg(a.block_table + (size_t)z.seq * a.max_pages + lp)
                                                                  : 0xFFFFFFFFu;
     };
 
     /* ---- copies: S - 1 steps ahead of the arithmetic ----
-     * Cursor of the next group of 16 tokens to copy: its page, the slot in it,
-     * its position, and the following pages, whose numbers are loaded a page
-     * (list entries: two pages) before they are needed. */
+     * Cursor of the next tokens to copy: their address, the slot in their page
+     * and the page's slots [page_lo, page_hi) that the mask keeps; and the
+     * following pages, whose numbers are loaded a page (list entries: two
+     * pages) before they are needed. */
     Segment pz;
     begin(pz);
-    uint32_t p_at = 0xFFFFFFFFu, left = 0, page_e = 0, off = 0, pos = 0, lp_next = 0, ph_next = 0, lp_then = 0;
+    uint32_t p_at = 0xFFFFFFFFu, left = 0, page_e = 0, off = 0, page_lo = 0, page_hi = 0, lp_next = 0, ph_next = 0, lp_then = 0;
     const uint8_t *kp = nullptr;
     const float *sp = nullptr;
-    bool page_ok = false, turn = false, done = false;
+    bool turn = false, done = false;
     uint32_t whole_slots = 0, fill = 0;                      /* bit per ring slot; slot of the next copies */
+    const size_t page_bytes = 2 * v_off, page_rows = (size_t)2 * a.n_kv_heads * a.page_tokens;
+    auto turn_page = [&]() {                                 /* opens the page at hand, looks up the one after */
+        const bool ok = ph_next < a.n_pages;
+        const uint32_t row = pz.item / a.n_tiles * a.page_tokens + off;          /* of the page */
+        kp = static_cast<const uint8_t *>(a.pool) + (ok ? ph_next : 0u) * page_bytes + (size_t)row * C::kRow + lane * 16;
+        if (kQ8)
+            sp = a.scales + (ok ? ph_next : 0u) * page_rows + row + (lane >> 2) * (a.n_kv_heads * a.page_tokens) + (lane & 3) * 4;
+        const uint32_t first = lp_next * a.page_tokens;
+        page_lo = pz.sq.start > first ? pz.sq.start - first : 0u;
+        page_hi = ok ? min(pz.sq.len - first, a.page_tokens) : 0u;
+        lp_next = lp_then;
+        ph_next = mapped(pz, lp_next);
+        lp_then = entry(pz, page_e + 2);
+        page_e++;
+        turn = false;
+    };
     /* Starts the copies of this warp's next step (tokens that the mask drops
      * become zeros), then, if that was the last of its segment, looks for the
      * next segment and loads the numbers of its first pages. */
     auto advance = [&]() {
         if (left) {
-            constexpr int CPR = C::kRow / 16, N = 16 * CPR;  /* 16-byte chunks of a row, of a group */
-            bool whole = true;
-            #pragma unroll 1
-            for (uint32_t gr = 0; gr < (uint32_t)GR; gr++) {
-                if (turn) {                                  /* open the page at hand, look up the one after */
-                    page_ok = ph_next < a.n_pages;
-                    const size_t row = ((size_t)(page_ok ? ph_next : 0u) * 2 * a.n_kv_heads + pz.item / a.n_tiles) * a.page_tokens + off;
-                    kp = static_cast<const uint8_t *>(a.pool) + row * C::kRow + lane * 16;
-                    if (kQ8) sp = a.scales + row + (lane >> 2) * (size_t)a.n_kv_heads * a.page_tokens + (lane & 3) * 4;
-                    pos = page_ok ? lp_next * a.page_tokens + off : 0u;
-                    lp_next = lp_then;
-                    ph_next = mapped(pz, lp_next);
-                    lp_then = entry(pz, page_e + 2);
-                    page_e++;
-                    turn = false;
-                }
-                const uint32_t to = ring_a + fill * C::kStage + gr * 16 * kPitch;
-                const uint32_t to_s = ring_a + fill * C::kStage + 2 * TS * kPitch + ((lane >> 2) * TS + gr * 16 + (lane & 3) * 4) * 4;
+            constexpr int CPR = C::kRow / 16, N = 16 * CPR;  /* 16-byte chunks of a row, of 16 tokens */
+            const uint32_t to = ring_a + fill * C::kStage;
+            const uint32_t to_s = to + 2 * TS * kPitch + ((lane >> 2) * TS + (lane & 3) * 4) * 4;
+            if (turn) turn_page();
+            bool whole = off >= page_lo && off + TS <= page_hi;
+            if (whole) {
                 const uint8_t *vp = kp + v_off;
-                if (page_ok && pos >= pz.sq.start && pos + 16 <= pz.sq.len) {
+                #pragma unroll
+                for (int c0 = 0; c0 < GR * N; c0 += 32) {
+                    const uint32_t c = c0 + lane;
+                    if (GR * N % 32 != 0 && c >= (uint32_t)(GR * N)) continue;
+                    const uint32_t d = to + (c / CPR) * kPitch + (c % CPR) * 16;
+                    cp_async16(d, kp + c0 * 16);
+                    cp_async16(d + TS * kPitch, vp + c0 * 16);
+                }
+                if (kQ8 && lane < 8) {                       /* scales of K, of V */
                     #pragma unroll
-                    for (int c0 = 0; c0 < N; c0 += 32) {
-                        const uint32_t c = c0 + lane;
-                        if (N % 32 != 0 && c >= (uint32_t)N) continue;
-                        const uint32_t d = to + (c / CPR) * kPitch + (c % CPR) * 16;
-                        cp_async16(d, kp + c0 * 16);
-                        cp_async16(d + TS * kPitch, vp + c0 * 16);
-                    }
-                    if (kQ8 && lane < 8) cp_async16(to_s, sp);           /* 16 scales of K, 16 of V */
-                } else {
-                    whole = false;
-                    const uint32_t lo = pos < pz.sq.start ? pz.sq.start - pos : 0u;      /* tokens [lo, hi) of the group are kept */
-                    const uint32_t hi = !page_ok || pos >= pz.sq.len ? 0u : (pz.sq.len - pos < 16u ? pz.sq.len - pos : 16u);
+                    for (int gr = 0; gr < GR; gr++) cp_async16(to_s + gr * 64, sp + gr * 16);
+                }
+                off += TS;
+                kp += TS * C::kRow;
+                if (kQ8) sp += TS;
+            } else {                                         /* 16 tokens at a time: across pages, or masked */
+                whole = true;
+                #pragma unroll 1
+                for (uint32_t gr = 0; gr < (uint32_t)GR; gr++) {
+                    if (turn || off == a.page_tokens) { if (!turn) off = 0; turn_page(); }
+                    const uint32_t lo = page_lo > off ? page_lo - off : 0u;      /* tokens [lo, hi) are kept */
+                    const uint32_t hi = page_hi > off ? min(page_hi - off, 16u) : 0u;
+                    whole = whole && lo == 0 && hi == 16;
                     #pragma unroll 1
                     for (uint32_t c = lane; c < (uint32_t)N; c += 32) {
-                        const uint32_t row = c / CPR, d = to + row * kPitch + (c % CPR) * 16;
+                        const uint32_t row = c / CPR, d = to + (gr * 16 + row) * kPitch + (c % CPR) * 16;
                         const uint32_t bytes = row >= lo && row < hi ? 16u : 0u;
                         cp_async16_part(d, kp + (c - lane) * 16, bytes);
-                        cp_async16_part(d + TS * kPitch, vp + (c - lane) * 16, bytes);
+                        cp_async16_part(d + TS * kPitch, kp + v_off + (c - lane) * 16, bytes);
                     }
                     if (kQ8 && lane < 8) {
                         const uint32_t tk = (lane & 3) * 4;
-                        cp_async16_part(to_s, sp, (hi > tk ? (hi - tk < 4u ? hi - tk : 4u) : 0u) * 4);
+                        cp_async16_part(to_s + gr * 64, sp, (hi > tk ? min(hi - tk, 4u) : 0u) * 4);
                     }
+                    off += 16;
+                    kp += 16 * C::kRow;
+                    if (kQ8) sp += 16;
                 }
-                pos += 16;
-                kp += 16 * C::kRow;
-                if (kQ8) sp += 16;
-                off += 16;
-                if (off == a.page_tokens) { off = 0; turn = true; }
             }
+            if (off == a.page_tokens) { off = 0; turn = true; }
             whole_slots = whole ? whole_slots | (1u << fill) : whole_slots & ~(1u << fill);
             fill = fill + 1 == S ? 0 : fill + 1;
             left--;
@@ -547,12 +562,13 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, DT, HT>::kMinB) k_gqa_decode(
          * is set anew when a weight would pass 2^15 or when a maximum grew, so
          * a weight keeps its 11 bits down to 2^-22 of the largest one that
          * still counts. */
-        int unit[HT][2];
-        bool renew = true, blank = true;                     /* blank: some head has seen no token yet */
+        float unit[HT][2];                                   /* 2^unit */
+        bool renew = true, blank = true;                     /* blank: some head has seen no token yet, */
+        uint32_t seen = 0;                                   /* bits of those that have */
         #pragma unroll
         for (int t = 0; t < HT; t++)
             #pragma unroll
-            for (int h = 0; h < 2; h++) { m[t][h] = kNoMax; l[t][h] = 0.0f; unit[t][h] = 0; }
+            for (int h = 0; h < 2; h++) { m[t][h] = 0.0f; l[t][h] = 0.0f; unit[t][h] = 1.0f; }
 
         #pragma unroll 1
         for (uint32_t i = z.wb; i < z.we;) {
@@ -567,7 +583,8 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, DT, HT>::kMinB) k_gqa_decode(
             float s[GR][HT][4];
             #pragma unroll
             for (int gr = 0; gr < GR; gr++) {
-                float s2[HT][4];                             /* every other block: two chains of MMAs */
+                constexpr bool kTwo = KB > 4;                /* every other block apart: two chains of MMAs */
+                float s2[HT][4];
                 #pragma unroll
                 for (int t = 0; t < HT; t++)
                     #pragma unroll
@@ -596,27 +613,31 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, DT, HT>::kMinB) k_gqa_decode(
                             q[t][2] = qb[kQS ? 0 : t][b + 1][0]; q[t][3] = qb[kQS ? 0 : t][b + 1][1];
                         }
                         mma16816<kQ8>(s[gr][t], f[0], q[t][0], q[t][1]);
-                        mma16816<kQ8>(s2[t], f[1], q[t][2], q[t][3]);
+                        mma16816<kQ8>(kTwo ? s2[t] : s[gr][t], f[1], q[t][2], q[t][3]);
                     }
                 }
                 #pragma unroll
                 for (int t = 0; t < HT; t++)
                     #pragma unroll
-                    for (int h = 0; h < 4; h++) s[gr][t][h] += s2[t][h];
+                    for (int h = 0; h < 4; h++)
+                        if (kTwo) s[gr][t][h] += s2[t][h];
             }
+            /* log2 of the probabilities, up to the running maxima */
             float vs[GR][2];                                 /* V scales of tokens g, g + 8 */
             #pragma unroll
             for (int gr = 0; gr < GR; gr++) {
-                float ks0 = 1.0f, ks1 = 1.0f;
                 if (kQ8) {
-                    ks0 = scp[gr * 16 + g]; ks1 = scp[gr * 16 + 8 + g];
+                    const float ks[2] = {scp[gr * 16 + g], scp[gr * 16 + 8 + g]};
                     vs[gr][0] = scp[TS + gr * 16 + g]; vs[gr][1] = scp[TS + gr * 16 + 8 + g];
+                    #pragma unroll
+                    for (int t = 0; t < HT; t++)
+                        #pragma unroll
+                        for (int h = 0; h < 4; h++) s[gr][t][h] *= ks[h >> 1];
                 }
                 #pragma unroll
-                for (int t = 0; t < HT; t++) {
-                    s[gr][t][0] *= ks0 * sc[t][0]; s[gr][t][1] *= ks0 * sc[t][1];
-                    s[gr][t][2] *= ks1 * sc[t][0]; s[gr][t][3] *= ks1 * sc[t][1];
-                }
+                for (int t = 0; t < HT; t++)
+                    #pragma unroll
+                    for (int h = 0; h < 4; h++) s[gr][t][h] = fmaf(s[gr][t][h], sc[t][h & 1], -m[t][h & 1]);
             }
             if (!((whole_slots >> slot) & 1u)) {             /* some tokens are not to be attended */
                 #pragma unroll
@@ -640,10 +661,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, DT, HT>::kMinB) k_gqa_decode(
                 #pragma unroll
                 for (int t = 0; t < HT; t++)
                     #pragma unroll
-                    for (int h = 0; h < 4; h++) {
-                        s[gr][t][h] -= m[t][h & 1] == kNoMax ? 0.0f : m[t][h & 1];
-                        top = fmaxf(top, s[gr][t][h]);
-                    }
+                    for (int h = 0; h < 4; h++) top = fmaxf(top, s[gr][t][h]);
             if (__any_sync(0xFFFFFFFFu, blank || top > kGrow)) {
                 renew = true;
                 blank = false;
@@ -651,7 +669,8 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, DT, HT>::kMinB) k_gqa_decode(
                 for (int t = 0; t < HT; t++) {
                     #pragma unroll
                     for (int h = 0; h < 2; h++) {
-                        const bool none = m[t][h] == kNoMax;
+                        const uint32_t bit = 1u << (2 * t + h);
+                        const bool none = (seen & bit) == 0;
                         float by = none ? -INFINITY : 0.0f;  /* how far the maximum moves */
                         #pragma unroll
                         for (int gr = 0; gr < GR; gr++) by = fmaxf(by, fmaxf(s[gr][t][h], s[gr][t][2 + h]));
@@ -659,7 +678,8 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, DT, HT>::kMinB) k_gqa_decode(
                         for (int d = 4; d < 32; d <<= 1) by = fmaxf(by, __shfl_xor_sync(0xFFFFFFFFu, by, d));
                         if (by == -INFINITY) { blank = true; continue; }
                         const float f = none ? 1.0f : ex2(-by);
-                        m[t][h] = none ? by : m[t][h] + by;
+                        seen |= bit;
+                        m[t][h] += by;
                         l[t][h] *= f;
                         #pragma unroll
                         for (int gr = 0; gr < GR; gr++) { s[gr][t][h] -= by; s[gr][t][2 + h] -= by; }
@@ -685,7 +705,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, DT, HT>::kMinB) k_gqa_decode(
                     for (int t = 0; t < HT; t++)
                         #pragma unroll
                         for (int h = 0; h < 4; h++) {
-                            s[gr][t][h] *= vs[gr][h >> 1] * pow2f(unit[t][h & 1]);
+                            s[gr][t][h] *= vs[gr][h >> 1] * unit[t][h & 1];
                             wt = fmaxf(wt, s[gr][t][h]);
                         }
                 if (__any_sync(0xFFFFFFFFu, renew || wt >= kTopWeight)) {
@@ -700,11 +720,12 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, DT, HT>::kMinB) k_gqa_decode(
                             #pragma unroll
                             for (int d = 4; d < 32; d <<= 1) w = fmaxf(w, __shfl_xor_sync(0xFFFFFFFFu, w, d));
                             if (w == 0.0f) { renew = true; continue; }
-                            int to = unit[t][h] + 7 - ((int)(__float_as_uint(w) >> 23) - 127);
+                            const int from = (int)(__float_as_uint(unit[t][h]) >> 23) - 127;
+                            int to = from + 7 - ((int)(__float_as_uint(w) >> 23) - 127);
                             to = to < -100 ? -100 : to > 100 ? 100 : to;
-                            const int by = to - unit[t][h];
+                            const int by = to - from;
                             const float f0 = pow2f(by / 2), f1 = pow2f(by - by / 2);
-                            unit[t][h] = to;
+                            unit[t][h] = pow2f(to);
                             #pragma unroll
                             for (int gr = 0; gr < GR; gr++) { s[gr][t][h] = s[gr][t][h] * f0 * f1; s[gr][t][2 + h] = s[gr][t][2 + h] * f0 * f1; }
                             #pragma unroll
@@ -777,7 +798,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, DT, HT>::kMinB) k_gqa_decode(
             for (int h = 0; h < 2; h++) {
                 #pragma unroll
                 for (int d = 4; d < 32; d <<= 1) l[t][h] += __shfl_xor_sync(0xFFFFFFFFu, l[t][h], d);
-                if (g == 0) { s_ml[warp][t * 8 + 2 * j + h][0] = m[t][h]; s_ml[warp][t * 8 + 2 * j + h][1] = l[t][h]; }
+                if (g == 0) { s_ml[warp][t * 8 + 2 * j + h][0] = (seen >> (2 * t + h)) & 1u ? m[t][h] : kNoMax; s_ml[warp][t * 8 + 2 * j + h][1] = l[t][h]; }
             }
         #pragma unroll
         for (int d0 = 0; d0 < D; d0 += kJoinCols) {
@@ -787,7 +808,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, DT, HT>::kMinB) k_gqa_decode(
                 for (int h = 0; h < 2; h++) {
                     const uint32_t r = t * 8 + 2 * j + h;
                     float *dst = mine + r * kJoin;
-                    const float back = kQ8 ? pow2f(-unit[t][h]) : 1.0f;
+                    const float back = kQ8 ? 1.0f / unit[t][h] : 1.0f;
                     if (r < rows) {
                         #pragma unroll
                         for (int b = 0; b < kJoinCols / 16; b++) {
