@@ -290,6 +290,16 @@ def ptr(a) -> int:
     return a.data_ptr()
 
 
+def _addr(a):
+    """ptr() for calls where a microsecond counts: ints, None and tensors first."""
+    if a is None or type(a) is int:
+        return a
+    try:
+        return a.data_ptr()
+    except AttributeError:
+        return ptr(a)
+
+
 def launch_count() -> int:
     return int(lib().ct_hal_cuda_launch_count())
 
@@ -524,21 +534,27 @@ class GqaKV(PagedKV):
 
 def gqa_write_slots(layout, pool, scales, k, v, dest_slot, n, src_dtype=CT_KV_BF16, k_stride=0, v_stride=0, stream=None):
     """Write n tokens' K and V rows into a grouped-query pool (ct_kv_gqa_write_slots)."""
-    check(lib().ct_kv_gqa_write_slots(C.byref(layout), ptr(pool), ptr(scales), ptr(k), ptr(v), k_stride, v_stride, src_dtype,
-                                      ptr(dest_slot), n, stream), "ct_kv_gqa_write_slots")
+    rc = lib().ct_kv_gqa_write_slots(layout, _addr(pool), _addr(scales), _addr(k), _addr(v), k_stride, v_stride, src_dtype,
+                                     _addr(dest_slot), n, stream)
+    if rc:
+        check(rc, "ct_kv_gqa_write_slots")
 
 
 def gqa_read_slots(layout, pool, scales, src_slot, n, k_out, v_out, out_dtype=CT_KV_BF16, k_stride=0, v_stride=0,
                    stream=None):
     """Read n tokens' K and V rows back from a grouped-query pool (ct_kv_gqa_read_slots)."""
-    check(lib().ct_kv_gqa_read_slots(C.byref(layout), ptr(pool), ptr(scales), ptr(src_slot), n, ptr(k_out), ptr(v_out),
-                                     k_stride, v_stride, out_dtype, stream), "ct_kv_gqa_read_slots")
+    rc = lib().ct_kv_gqa_read_slots(layout, _addr(pool), _addr(scales), _addr(src_slot), n, _addr(k_out), _addr(v_out), k_stride,
+                                    v_stride, out_dtype, stream)
+    if rc:
+        check(rc, "ct_kv_gqa_read_slots")
 
 
 def gqa_page_bounds(layout, pool, scales, pages, counts, n, bounds, bound_scales, stream=None):
     """Bounds of the keys of n pages (ct_kv_gqa_page_bounds)."""
-    check(lib().ct_kv_gqa_page_bounds(C.byref(layout), ptr(pool), ptr(scales), ptr(pages), ptr(counts), n, ptr(bounds),
-                                      ptr(bound_scales), stream), "ct_kv_gqa_page_bounds")
+    rc = lib().ct_kv_gqa_page_bounds(layout, _addr(pool), _addr(scales), _addr(pages), _addr(counts), n, _addr(bounds),
+                                     _addr(bound_scales), stream)
+    if rc:
+        check(rc, "ct_kv_gqa_page_bounds")
 
 
 class GqaPlan:
@@ -571,20 +587,24 @@ class GqaPlan:
         return int(lib().ct_gqa_plan_scratch_bytes(self.h))
 
     def decode(self, q, pool, scales, block_table, seq_lens, out, lse=None, q_stride=0, stream=None):
-        check(lib().ct_attn_gqa_decode_paged(self.h, ptr(q), q_stride, ptr(pool), ptr(scales), ptr(block_table),
-                                             ptr(seq_lens), ptr(out), ptr(lse), stream), "ct_attn_gqa_decode_paged")
+        rc = lib().ct_attn_gqa_decode_paged(self.h, _addr(q), q_stride, _addr(pool), _addr(scales), _addr(block_table),
+                                            _addr(seq_lens), _addr(out), _addr(lse), stream)
+        if rc:
+            check(rc, "ct_attn_gqa_decode_paged")
 
     def select(self, q, bounds, bound_scales, block_table, seq_lens, pages, n_select, n_first=1, n_last=1, q_stride=0,
                stream=None):
-        check(lib().ct_attn_gqa_select_pages(self.h, ptr(q), q_stride, ptr(bounds), ptr(bound_scales), ptr(block_table),
-                                             ptr(seq_lens), n_select, n_first, n_last, ptr(pages), stream),
-              "ct_attn_gqa_select_pages")
+        rc = lib().ct_attn_gqa_select_pages(self.h, _addr(q), q_stride, _addr(bounds), _addr(bound_scales), _addr(block_table),
+                                            _addr(seq_lens), n_select, n_first, n_last, _addr(pages), stream)
+        if rc:
+            check(rc, "ct_attn_gqa_select_pages")
 
     def decode_selected(self, q, pool, scales, block_table, seq_lens, pages, n_select, out, lse=None, q_stride=0,
                         stream=None):
-        check(lib().ct_attn_gqa_decode_selected(self.h, ptr(q), q_stride, ptr(pool), ptr(scales), ptr(block_table),
-                                                ptr(seq_lens), ptr(pages), n_select, ptr(out), ptr(lse), stream),
-              "ct_attn_gqa_decode_selected")
+        rc = lib().ct_attn_gqa_decode_selected(self.h, _addr(q), q_stride, _addr(pool), _addr(scales), _addr(block_table),
+                                               _addr(seq_lens), _addr(pages), n_select, _addr(out), _addr(lse), stream)
+        if rc:
+            check(rc, "ct_attn_gqa_decode_selected")
 
 
 class MlaPlan:

@@ -69,12 +69,47 @@ __global__ void __launch_bounds__(kThreads) k_gqa_write(void *pool, float *scale
         w[i][0] = __ldcs(p);
         if (F32) w[i][F32 ? 1 : 0] = __ldcs(p + 1);
     }
+    /* The four tokens' maxima are reduced together: after two exchanges a lane
+     * keeps that of token u & 3, so the divisions run once, not four times. */
+    uint32_t top[T];                                         /* bits of max|x|: NaN above Inf above every finite value */
+    float d = 0.0f, id = 0.0f;
+    if (DT != CT_KV_BF16) {
+        #pragma unroll
+        for (int i = 0; i < T; i++) {
+            top[i] = 0;
+            if (t0 + i * R >= n || u >= U) continue;
+            if (F32) {
+                const uint32_t ws[8] = {w[i][0].x, w[i][0].y, w[i][0].z, w[i][0].w, w[i][F32 ? 1 : 0].x, w[i][F32 ? 1 : 0].y,
+                                        w[i][F32 ? 1 : 0].z, w[i][F32 ? 1 : 0].w};
+                #pragma unroll
+                for (int e = 0; e < 8; e++) top[i] = max(top[i], ws[e] & 0x7FFFFFFFu);
+            } else {
+                const uint32_t m = __vimax3_u16x2(w[i][0].x & 0x7FFF7FFFu, w[i][0].y & 0x7FFF7FFFu, w[i][0].z & 0x7FFF7FFFu);
+                const uint32_t m2 = __vimax3_u16x2(m, w[i][0].w & 0x7FFF7FFFu, 0u);
+                top[i] = max(m2 << 16, m2 & 0xFFFF0000u);
+            }
+        }
+        uint32_t r = top[0];
+        if (T == 4) {
+            const bool b = u & 1, c = u & 2;
+            const uint32_t r0 = max(b ? top[T - 3] : top[0], __shfl_xor_sync(0xFFFFFFFFu, b ? top[0] : top[T - 3], 1));
+            const uint32_t r1 = max(b ? top[T - 1] : top[T - 2], __shfl_xor_sync(0xFFFFFFFFu, b ? top[T - 2] : top[T - 1], 1));
+            r = max(c ? r1 : r0, __shfl_xor_sync(0xFFFFFFFFu, c ? r0 : r1, 2));
+        }
+        #pragma unroll
+        for (int o = T; o < L; o <<= 1) r = max(r, __shfl_xor_sync(0xFFFFFFFFu, r, o));
+        const bool fine = r < 0x7F800000u;
+        d = fine ? __fdiv_rn(__uint_as_float(r), DT == CT_KV_INT8 ? 127.0f : 448.0f) : __uint_as_float(0x7FC00000u);
+        id = fine && d > 0.0f ? fminf(__fdiv_rn(1.0f, d), FLT_MAX) : 0.0f;
+    }
     #pragma unroll
     for (int i = 0; i < T; i++) {
+        const uint32_t from = (threadIdx.x & (32 - L)) | (i & (L - 1));
+        const float di = T == 1 ? d : __shfl_sync(0xFFFFFFFFu, d, from), idi = T == 1 ? id : __shfl_sync(0xFFFFFFFFu, id, from);
         size_t row = 0;
-        const bool mine = pool_row(slot[i], place, n_kv_heads, page_tokens, n_pages, row) && u < U;
+        if (!pool_row(slot[i], place, n_kv_heads, page_tokens, n_pages, row) || u >= U) continue;
         if (DT == CT_KV_BF16 && !F32) {
-            if (mine) *reinterpret_cast<uint4 *>(static_cast<uint16_t *>(pool) + row * D + u * 8) = w[i][0];
+            *reinterpret_cast<uint4 *>(static_cast<uint16_t *>(pool) + row * D + u * 8) = w[i][0];
             continue;
         }
         float x[8];
@@ -82,24 +117,14 @@ __global__ void __launch_bounds__(kThreads) k_gqa_write(void *pool, float *scale
                                 w[i][F32 ? 1 : 0].z, w[i][F32 ? 1 : 0].w};
         #pragma unroll
         for (int e = 0; e < 8; e++)
-            x[e] = !mine ? 0.0f : F32 ? __uint_as_float(ws[e]) : __uint_as_float((e & 1) ? ws[e >> 1] & 0xFFFF0000u : ws[e >> 1] << 16);
+            x[e] = F32 ? __uint_as_float(ws[e]) : __uint_as_float((e & 1) ? ws[e >> 1] & 0xFFFF0000u : ws[e >> 1] << 16);
         if (DT == CT_KV_BF16) {
-            if (mine)
-                *reinterpret_cast<uint4 *>(static_cast<uint16_t *>(pool) + row * D + u * 8) =
-                    make_uint4(pack2_bf16(x[0], x[1]), pack2_bf16(x[2], x[3]), pack2_bf16(x[4], x[5]), pack2_bf16(x[6], x[7]));
+            *reinterpret_cast<uint4 *>(static_cast<uint16_t *>(pool) + row * D + u * 8) =
+                make_uint4(pack2_bf16(x[0], x[1]), pack2_bf16(x[2], x[3]), pack2_bf16(x[4], x[5]), pack2_bf16(x[6], x[7]));
             continue;
         }
-        uint32_t top = 0;                                    /* bits of max|x|: NaN above Inf above every finite value */
-        #pragma unroll
-        for (int e = 0; e < 8; e++) top = max(top, __float_as_uint(x[e]) & 0x7FFFFFFFu);
-        #pragma unroll
-        for (int o = 1; o < L; o <<= 1) top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
-        if (!mine) continue;
-        const bool fine = top < 0x7F800000u;
-        const float d = __fdiv_rn(__uint_as_float(top), DT == CT_KV_INT8 ? 127.0f : 448.0f);
-        const float id = fine && d > 0.0f ? fminf(__fdiv_rn(1.0f, d), FLT_MAX) : 0.0f;
         uint32_t c[2] = {0u, 0u};
-        if (fine) {
+        if (di == di) {                                      /* a NaN or an infinity in the row: codes 0 */
             #pragma unroll
             for (int k = 0; k < 2; k++) {
                 if (DT == CT_KV_INT8) {
@@ -108,16 +133,16 @@ __global__ void __launch_bounds__(kThreads) k_gqa_write(void *pool, float *scale
                     uint32_t q[4];
                     #pragma unroll
                     for (int e = 0; e < 4; e++)
-                        q[e] = __float_as_uint(__fadd_rd(__fadd_rn(__fmul_rn(x[4 * k + e], id), 0.5f), 12582912.0f));
+                        q[e] = __float_as_uint(__fadd_rd(__fadd_rn(__fmul_rn(x[4 * k + e], idi), 0.5f), 12582912.0f));
                     c[k] = __byte_perm(__byte_perm(q[0], q[1], 0x0040), __byte_perm(q[2], q[3], 0x0040), 0x5410);
                 } else {
-                    c[k] = (uint32_t)ct_e4m3x2_code(x[4 * k], x[4 * k + 1], id) |
-                           ((uint32_t)ct_e4m3x2_code(x[4 * k + 2], x[4 * k + 3], id) << 16);
+                    c[k] = (uint32_t)ct_e4m3x2_code(x[4 * k], x[4 * k + 1], idi) |
+                           ((uint32_t)ct_e4m3x2_code(x[4 * k + 2], x[4 * k + 3], idi) << 16);
                 }
             }
         }
         *reinterpret_cast<uint2 *>(static_cast<uint8_t *>(pool) + row * D + u * 8) = make_uint2(c[0], c[1]);
-        if (u == 0) scales[row] = fine ? d : __uint_as_float(0x7FC00000u);
+        if (u == 0) scales[row] = di;
     }
 }
 

@@ -45,10 +45,7 @@
 
 namespace ct_gqa {
 
-#ifndef GQ_WARPS
-#define GQ_WARPS 4
-#endif
-constexpr int kWarps = GQ_WARPS;
+constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
@@ -56,42 +53,23 @@ constexpr float kGrow = 8.0f;           /* log2 growth of a maximum that is foll
 constexpr float kNoMax = -3.402823466e38f;  /* maximum of no tokens: finite, so that no difference of maxima is NaN */
 constexpr float kTopWeight = 32768.0f;  /* fp16 weights stay below this */
 constexpr uint32_t kItemCost = 4;       /* steps that an item's start and end are counted as */
-#ifndef GQ_CMIN
-#define GQ_CMIN 12u
-#endif
-#ifndef GQ_CDIV
-#define GQ_CDIV 4
-#endif
-#ifndef GQ_CMAX
-#define GQ_CMAX 40u
-#endif
-#define GQ_CUT max(GQ_CMIN, min(Q / GQ_CDIV, GQ_CMAX))
-#ifndef GQ_SOLO
-#define GQ_SOLO 16
-#endif
-constexpr uint32_t kSoloMost = GQ_SOLO; /* longest item of one warp: longer ones would leave the others idle at the end */
+constexpr uint32_t kSoloMost = 16; /* longest item of one warp: longer ones would leave the others idle at the end */
 constexpr uint32_t kSoloCost = 3;       /* start and end of an item, in steps of one warp, */
 constexpr uint32_t kShareCost = 10;     /* and of one that the warps share */
-constexpr uint32_t kWhole = 8;          /* items of at most so many steps are not cut between CTAs */
-constexpr uint32_t kFewSteps = 32;      /* steps a CTA up to which a part of one item each is the better split */
 constexpr uint32_t kFan = 16;           /* workers whose parts are joined at a time, when an item has more than 2 kFan */
 
-/* Tokens of a warp's step, steps in its ring, CTAs that an SM holds. */
-#ifndef GQ_TS
-#define GQ_TS (kRow <= 64 ? 32 : 16)
-#endif
-#ifndef GQ_S
-#define GQ_S (kElt == 1 && HT * D == 512 ? 2 : 3)
-#endif
-#ifndef GQ_MINB
-#define GQ_MINB (HT == 1 && D <= 128 && (kElt == 1 || D <= 64) ? 3 : 1)
-#endif
+/* Tokens of a warp's step (2 to 17 KB of K and V), steps in its ring, and the
+ * CTAs that an SM shall hold.  Three steps of 16 tokens a warp leave 2 CTAs of
+ * bf16 x 128 (140 KB of copies in flight), 3 of 8-bit x 128; a third CTA is
+ * worth the registers' limit of 168 where it spills nothing: int8 x 128, 256
+ * sequences of 256 tokens 53 -> 47 us.  Two steps only where that lets a
+ * second CTA in (8-bit x 256, groups above 8: 75 -> 57 us). */
 template <int D, int DT, int HT> struct Cfg {
     static constexpr int kElt = DT == CT_KV_BF16 ? 2 : 1;
     static constexpr int kRow = D * kElt;
-    static constexpr int TS = GQ_TS;
-    static constexpr int kStages = GQ_S;
-    static constexpr int kMinB = GQ_MINB;
+    static constexpr int TS = kRow <= 64 ? 32 : 16;
+    static constexpr int kStages = kElt == 1 && HT * D == 512 ? 2 : 3;
+    static constexpr int kMinB = HT == 1 && D <= 128 && (kElt == 1 || D <= 64) ? 3 : 1;
     static constexpr int kPitch = kRow + 16;                  /* odd number of 16-B units: conflict-free ldmatrix */
     static constexpr int kScaleBytes = DT == CT_KV_BF16 ? 0 : TS * 8;
     static constexpr int kStage = 2 * TS * kPitch + kScaleBytes;
@@ -143,6 +121,16 @@ template <bool F16> CT_DEV void mma16816(float *c, const uint32_t *a, uint32_t b
 CT_DEV float ex2(float x) {
     float y;
     asm("ex2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+CT_DEV float rcp(float x) {
+    float y;
+    asm("rcp.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+CT_DEV float lg2(float x) {
+    float y;
+    asm("lg2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
 /* Two floats -> packed (lo in the low half), round to nearest even. */
@@ -205,8 +193,11 @@ template <int TS> CT_DEV Seq sequence(const ct_gqa_args_t &a, uint32_t s) {
     return r;
 }
 
-/* HT: column tiles of 8 query heads. */
-template <int D, int DT, int HT>
+/* HT: column tiles of 8 query heads.  FEW: fewer than half as many items as
+ * CTAs, each CTA takes a part of one; this form has no more code than that
+ * needs, since a call of a few microseconds runs every line of it from a cold
+ * instruction cache. */
+template <int D, int DT, int HT, bool FEW>
 __global__ void __launch_bounds__(kThreads, Cfg<D, DT, HT>::kMinB) k_gqa_decode(const ct_gqa_args_t a) {
     using C = Cfg<D, DT, HT>;
     constexpr int TS = C::TS, GR = TS / 16, kPitch = C::kPitch, KB = D / 16, S = C::kStages;
@@ -219,7 +210,9 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, DT, HT>::kMinB) k_gqa_decode(
     static_assert(kHeads * kJoin * 4 <= C::kStage && kJoinCols % 16 == 0, "half the sums of a warp fit a slot");
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ uint32_t s_scan[kWarps];
-    struct End { uint32_t ordinal, step, first, last; };     /* an end of the CTA's range; its item's first and last worker */
+    /* An end of the CTA's range: an item (and its ordinal in the batch), a step
+     * of it, the first and last worker that hold steps of it. */
+    struct End { uint32_t seq, head, tile, step, first, last, ordinal; };
     __shared__ End s_end[2];
     __shared__ float s_ml[kWarps][kHeads][2];
     __shared__ uint32_t s_free[kWarps], s_last;
@@ -227,40 +220,37 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, DT, HT>::kMinB) k_gqa_decode(
     const uint32_t HV = a.n_kv_heads * a.n_tiles;
     ct_gqa_enter();
 
-    /* ---- this CTA's range of steps: from step s_end[0].step of item
-     * s_end[0].ordinal to before step s_end[1].step of s_end[1].ordinal ---- */
-    bool few = 2ull * a.n_seq * HV <= gridDim.x;
-    if (few) {                                               /* each warp for itself: no barrier */
-        uint32_t sum = 0;
+    /* ---- this CTA's range of steps: from s_end[0] to before s_end[1] ---- */
+    auto end_at = [&](uint32_t s, uint32_t item, uint32_t step, uint32_t first, uint32_t last) -> End {
+        const uint32_t head = item / a.n_tiles;
+        return {s, head, item - head * a.n_tiles, step, first, last, s * HV + item};
+    };
+    if (FEW) {                                               /* each warp for itself; the last barrier shares the result */
+        uint32_t sum = 0, before = 0;
         #pragma unroll 1
         for (uint32_t s = lane; s < a.n_seq; s += 32) sum += sequence<TS>(a, s).steps;
         sum = __reduce_add_sync(0xFFFFFFFFu, sum);
-        few = (uint64_t)sum * HV <= (uint64_t)kFewSteps * gridDim.x;
-        if (few) {
-            const uint32_t Q = max(a.min_steps, (sum * HV - 1) / (gridDim.x - a.n_seq * HV) + 1);
-            uint32_t at = 0, all = 0;                        /* parts before the sequences at hand */
-            #pragma unroll 1
-            for (uint32_t s0 = 0; s0 < a.n_seq; s0 += 32) {
-                const uint32_t s = s0 + lane, steps = s < a.n_seq ? sequence<TS>(a, s).steps : 0u, n = (steps + Q - 1) / Q;
-                uint32_t incl = n * HV;
-                #pragma unroll
-                for (int o = 1; o < 32; o <<= 1) {
-                    const uint32_t y = __shfl_up_sync(0xFFFFFFFFu, incl, o);
-                    if (lane >= (uint32_t)o) incl += y;
-                }
-                const uint32_t x = blockIdx.x - (all + incl - n * HV);
-                if (n && blockIdx.x >= all + incl - n * HV && x < n * HV && warp == 0) {
-                    const uint32_t item = x / n, part = x - item * n, first = blockIdx.x - part;
-                    s_end[0] = {s * HV + item, steps * part / n, first, first + n - 1};
-                    s_end[1] = {s * HV + item, steps * (part + 1) / n, first, first + n - 1};
-                }
-                all += __shfl_sync(0xFFFFFFFFu, incl, 31);
-                at = all;
+        const uint32_t spare = gridDim.x - a.n_seq * HV;     /* every item's last part may be a short one */
+        const uint32_t Q = max(a.min_steps, (uint32_t)__umul64hi((uint64_t)sum * HV + spare - 1, a.spare_magic));
+        #pragma unroll 1
+        for (uint32_t s0 = 0; s0 < a.n_seq; s0 += 32) {
+            const uint32_t s = s0 + lane, steps = s < a.n_seq ? sequence<TS>(a, s).steps : 0u, n = min((steps + Q - 1) / Q, a.most_parts);
+            uint32_t incl = n * HV;                          /* parts of the sequence's items */
+            #pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const uint32_t y = __shfl_up_sync(0xFFFFFFFFu, incl, o);
+                if (lane >= (uint32_t)o) incl += y;
             }
-            if (blockIdx.x >= at) return;
+            const uint32_t x = blockIdx.x - (before + incl - n * HV);
+            if (warp == 0 && x < n * HV) {
+                const uint32_t item = x / n, part = x - item * n, first = blockIdx.x - part, each = steps / n, over = steps - each * n;
+                s_end[0] = end_at(s, item, part * each + min(part, over), first, first + n - 1);
+                s_end[1].step = (part + 1) * each + min(part + 1, over);
+            }
+            before += __shfl_sync(0xFFFFFFFFu, incl, 31);
         }
-    }
-    if (!few) {
+        if (blockIdx.x >= before) return;
+    } else {
         const uint32_t per = (a.n_seq + kThreads - 1) / kThreads;
         uint32_t sum = 0;
         #pragma unroll 1
@@ -286,7 +276,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, DT, HT>::kMinB) k_gqa_decode(
         const uint32_t Q = max(a.min_steps, (uint32_t)__umul64hi(total + gridDim.x - 1, a.worker_magic));
         const uint64_t x0 = (uint64_t)blockIdx.x * Q;
         if (x0 >= total) return;
-        if (tid == 0 && x0 + Q >= total) s_end[1] = {a.n_seq * HV, 0u, 0u, 0u};
+        if (tid == 0 && x0 + Q >= total) s_end[1] = end_at(a.n_seq, 0u, 0u, 0u, 0u);
         #pragma unroll 1
         for (uint32_t b = 0; b < 2; b++) {                   /* where the range begins, where the next one does */
             const uint64_t x = x0 + b * Q;
@@ -301,17 +291,19 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, DT, HT>::kMinB) k_gqa_decode(
             }
             const uint32_t rel = (uint32_t)(x - at), item = rel / width;          /* below 2^32: see the plan */
             uint32_t in = rel - item * width;
-            if (width <= GQ_CUT) in = 0;                     /* a short item goes to the later CTA as a whole */
+            /* An item that is short against the CTA's share goes to the later
+             * CTA as a whole: cutting it costs both of them a shared start and
+             * end, and the join. */
+            if (width <= max(12u, min(Q / 4, 40u))) in = 0;
             const uint32_t step = in > kItemCost ? in - kItemCost : 0u;
             /* workers that hold steps of the item: from the one of its first
              * step (this one if the item begins here) to that of its last */
             const uint32_t here = blockIdx.x + b;
-            s_end[b] = {s * HV + item, step, here - (step + Q - 1) / Q, here + (width - 1 - in) / Q};
+            s_end[b] = end_at(s, item, step, here - (step + Q - 1) / Q, here + (width - 1 - in) / Q);
         }
     }
     __syncthreads();
-    const uint32_t o0 = s_end[0].ordinal;
-    const uint32_t range = s_end[1].ordinal - o0 + (s_end[1].step ? 1u : 0u);      /* items */
+    const uint32_t range = FEW ? 1u : s_end[1].ordinal - s_end[0].ordinal + (s_end[1].step ? 1u : 0u);     /* items */
     if (range == 0) return;
 
     uint8_t *ring = smem + warp * (S * C::kStage);
@@ -325,26 +317,35 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, DT, HT>::kMinB) k_gqa_decode(
     /* A segment: the part of an item inside the range, and this warp's run of
      * its steps [wb, we). */
     struct Segment {
-        uint32_t seq, item;
+        uint32_t seq, head, tile;
         Seq sq;
         uint32_t sb, se, wb, we;
         bool solo;
     };
-    auto begin = [&](Segment &z) {
-        z.seq = o0 / HV;
-        z.item = o0 % HV;
-        z.sq = sequence<TS>(a, z.seq);
-    };
-    auto bounds = [&](Segment &z, uint32_t at) {             /* of item o0 + at, which z.seq and z.item name */
+    /* The range's at-th item; called with at = 0, 1, 2, ... */
+    auto segment = [&](Segment &z, uint32_t at) {
+        bool next = at == 0;
+        if (at == 0) {
+            z.seq = s_end[0].seq;
+            z.head = s_end[0].head;
+            z.tile = s_end[0].tile;
+        } else if (++z.tile == a.n_tiles) {
+            z.tile = 0;
+            if (++z.head == a.n_kv_heads) { z.head = 0; z.seq++; next = true; }
+        }
+        if (next) z.sq = sequence<TS>(a, z.seq);
         z.sb = at == 0 ? s_end[0].step : 0u;
         z.se = at + 1 == range && s_end[1].step ? s_end[1].step : z.sq.steps;
         const uint32_t n = z.se - z.sb;
-        /* A whole item is one warp's if there is nothing to share, or if the
-         * range's whole items, handed out one by one, take
-         * less of the warps' time so than shared. */
-        const uint32_t items = range - (s_end[0].step ? 1u : 0u) - (s_end[1].step ? 1u : 0u), rounds = (items + kWarps - 1) / kWarps;
-        z.solo = n == z.sq.steps && (n == 1 || (n <= kSoloMost && items > 1 &&
-                                                kWarps * rounds * (n + kSoloCost) <= items * (n + kShareCost)));
+        z.solo = false;
+        if (!FEW) {
+            /* A whole item is one warp's if there is nothing to share, or if the
+             * range's whole items, handed out one by one, take less of the
+             * warps' time so than shared. */
+            const uint32_t items = range - (s_end[0].step ? 1u : 0u) - (s_end[1].step ? 1u : 0u), rounds = (items + kWarps - 1) / kWarps;
+            z.solo = n == z.sq.steps && (n == 1 || (n <= kSoloMost && items > 1 &&
+                                                    kWarps * rounds * (n + kSoloCost) <= items * (n + kShareCost)));
+        }
         if (z.solo) {
             z.wb = z.sb;
             z.we = (at & (kWarps - 1)) == warp ? z.se : z.sb;
@@ -353,18 +354,11 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, DT, HT>::kMinB) k_gqa_decode(
             z.we = z.sb + n * (warp + 1) / kWarps;
         }
     };
-    auto step_on = [&](Segment &z) {
-        if (++z.item == HV) {
-            z.item = 0;
-            z.sq = sequence<TS>(a, ++z.seq);
-        }
-    };
     auto first_token = [&](const Seq &q) -> uint32_t { return a.picked ? 0u : (q.start & ~15u); };
     /* Logical page of the e-th page stepped over (0xFFFFFFFF: none). */
     auto entry = [&](const Segment &z, uint32_t e) -> uint32_t {
         if (!a.picked) return e;
-        const uint32_t head = z.item / a.n_tiles;
-        return e < z.sq.n_list ? (uint32_t)__ldg(a.picked + ((size_t)z.seq * a.n_kv_heads + head) * a.n_pick + e) : 0xFFFFFFFFu;
+        return e < z.sq.n_list ? (uint32_t)__ldg(a.picked + ((size_t)z.seq * a.n_kv_heads + z.head) * a.n_pick + e) : 0xFFFFFFFFu;
     };
     /* Its physical page (>= n_pages: nothing to read). */
     auto mapped = [&](const Segment &z, uint32_t lp) -> uint32_t {
@@ -377,8 +371,8 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, DT, HT>::kMinB) k_gqa_decode(
      * and the page's slots [page_lo, page_hi) that the mask keeps; and the
      * following pages, whose numbers are loaded a page (list entries: two
      * pages) before they are needed. */
-    Segment pz;
-    begin(pz);
+    Segment z = {}, pz = {};
+    if (FEW) { segment(z, 0); pz = z; }
     uint32_t p_at = 0xFFFFFFFFu, left = 0, page_e = 0, off = 0, page_lo = 0, page_hi = 0, lp_next = 0, ph_next = 0, lp_then = 0;
     const uint8_t *kp = nullptr;
     const float *sp = nullptr;
@@ -387,7 +381,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, DT, HT>::kMinB) k_gqa_decode(
     const size_t page_bytes = 2 * v_off, page_rows = (size_t)2 * a.n_kv_heads * a.page_tokens;
     auto turn_page = [&]() {                                 /* opens the page at hand, looks up the one after */
         const bool ok = ph_next < a.n_pages;
-        const uint32_t row = pz.item / a.n_tiles * a.page_tokens + off;          /* of the page */
+        const uint32_t row = pz.head * a.page_tokens + off;  /* of the page */
         kp = static_cast<const uint8_t *>(a.pool) + (ok ? ph_next : 0u) * page_bytes + (size_t)row * C::kRow + lane * 16;
         if (kQ8)
             sp = a.scales + (ok ? ph_next : 0u) * page_rows + row + (lane >> 2) * (a.n_kv_heads * a.page_tokens) + (lane & 3) * 4;
@@ -461,8 +455,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, DT, HT>::kMinB) k_gqa_decode(
             #pragma unroll 1
             do {
                 if (++p_at == range) { done = true; break; }
-                if (p_at) step_on(pz);
-                bounds(pz, p_at);
+                if (!FEW) segment(pz, p_at);
                 left = pz.we - pz.wb;
             } while (left == 0);
             if (left) {
@@ -480,14 +473,11 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, DT, HT>::kMinB) k_gqa_decode(
     int prime = S;                                           /* the first call looks for a segment, S - 1 fill the ring */
 
     /* ---- arithmetic ---- */
-    Segment z;
-    begin(z);
     #pragma unroll 1
     for (uint32_t at = 0; at < range; at++) {
-        if (at) step_on(z);
-        bounds(z, at);
+        if (!FEW) segment(z, at);
         if (z.solo && z.we == z.wb) continue;                /* another warp's */
-        const uint32_t seq = z.seq, tile = z.item % a.n_tiles, head = z.item / a.n_tiles;
+        const uint32_t seq = z.seq, tile = z.tile, head = z.head;
         const uint32_t rows = a.group - tile * 16 < 16 ? a.group - tile * 16 : 16;
         const bool cut = z.sb > 0 || z.se < z.sq.steps;
         auto query_head = [&](uint32_t r) -> uint32_t {
@@ -782,12 +772,9 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, DT, HT>::kMinB) k_gqa_decode(
         const uint32_t part = 2 * blockIdx.x + (z.sb > 0 ? 0u : 1u);
         float *po = a.part_o + (size_t)part * 16 * D;
         float *pml = a.part_ml + (size_t)part * 32;
-        auto finish = [&](uint32_t r, uint32_t d, float M, float L, const float4 &acc) {
-            const float inv = L == 0.0f ? 0.0f : 1.0f / L;
-            const size_t row = (size_t)seq * a.n_q_heads + query_head(r);
-            *reinterpret_cast<uint2 *>(a.out + row * D + d) =
-                make_uint2(pack_bf16(acc.x * inv, acc.y * inv), pack_bf16(acc.z * inv, acc.w * inv));
-            if (a.lse && d == 0) a.lse[row] = (M + log2f(L)) * kLn2;
+        auto write = [&](uint32_t r, uint32_t d, float f, const float4 &v) {
+            *reinterpret_cast<uint2 *>(a.out + ((size_t)seq * a.n_q_heads + query_head(r)) * D + d) =
+                make_uint2(pack_bf16(v.x * f, v.y * f), pack_bf16(v.z * f, v.w * f));
         };
         const uint32_t freed = slot == 0 ? S - 1 : slot - 1;
         float *mine = reinterpret_cast<float *>(ring + freed * C::kStage);
@@ -808,7 +795,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, DT, HT>::kMinB) k_gqa_decode(
                 for (int h = 0; h < 2; h++) {
                     const uint32_t r = t * 8 + 2 * j + h;
                     float *dst = mine + r * kJoin;
-                    const float back = kQ8 ? 1.0f / unit[t][h] : 1.0f;
+                    const float back = kQ8 ? rcp(unit[t][h]) : 1.0f;      /* a power of two: exact */
                     if (r < rows) {
                         #pragma unroll
                         for (int b = 0; b < kJoinCols / 16; b++) {
@@ -847,7 +834,8 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, DT, HT>::kMinB) k_gqa_decode(
                     __stcg(reinterpret_cast<float4 *>(po + r * D + d), acc);
                     if (d == 0) __stcg(reinterpret_cast<float2 *>(pml + 2 * r), make_float2(M, L));
                 } else {
-                    finish(r, d, M, L, acc);
+                    write(r, d, L == 0.0f ? 0.0f : rcp(L), acc);
+                    if (a.lse && d == 0) a.lse[(size_t)seq * a.n_q_heads + query_head(r)] = (M + lg2(L)) * kLn2;
                 }
             }
             if (z.solo) __syncwarp(); else __syncthreads();              /* the slots and s_ml are free again */
@@ -857,7 +845,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, DT, HT>::kMinB) k_gqa_decode(
              * An item of more than 2 kFan workers (few items in the batch)
              * is joined in two rounds: each aligned run of kFan workers by
              * its last one, into the run's first part, then the runs. */
-            const End &end = s_end[z.sb > 0 ? 0 : 1];
+            const End &end = s_end[FEW || z.sb > 0 ? 0 : 1];
             const uint32_t first = end.first, last = end.last;
             const bool tree = last - first >= 2 * kFan;
             uint32_t lo = first, hi = last, by = 1;
@@ -885,55 +873,65 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, DT, HT>::kMinB) k_gqa_decode(
                 __syncthreads();
                 last_here = s_last != 0;
                 if (!last_here) break;
-                /* part k of the join: worker w_k, its slot */
-                auto slot_of = [&](uint32_t k) -> uint32_t {
-                    uint32_t w = lo + k;
-                    if (by != 1) w = k == 0 ? first : (first / kFan + k) * kFan;
-                    return 2 * w + (w == first ? 1u : 0u);
-                };
-                /* (max, sum) of part k and row r: entries c = r n + k in the
-                 * warps' free slots, each kStage / 8 of them */
-                constexpr uint32_t kPer = C::kStage / 8;
-                auto s_part = [&](uint32_t k, uint32_t r) -> float2 & {
-                    const uint32_t c = r * n + k;
-                    return reinterpret_cast<float2 *>(smem + s_free[c / kPer])[c % kPer];
+                /* part k of the join: of worker lo + k, or of the k-th run of
+                 * workers, in its first slot (in the item's first worker: its
+                 * second) */
+                const uint32_t from = by == 1 ? lo : first / kFan * kFan, to = by == 1 && lo != first ? 2 * lo : 2 * first + 1;
+                auto slot_of = [&](uint32_t k) -> uint32_t { return k ? 2 * (from + k * by) : to; };
+                const bool more = tree && round == 0;
+                /* weights of the parts (at most 65), a row a warp, in the
+                 * warps' free slots; 1 / sum in place of the warps' maxima */
+                auto s_weight = [&](uint32_t r, uint32_t k) -> float & {
+                    return reinterpret_cast<float *>(smem + s_free[r & (kWarps - 1)])[r / kWarps * n + k];
                 };
                 #pragma unroll 1
-                for (uint32_t c = tid; c < n * rows; c += kThreads) {
-                    const uint32_t r = c / n, k = c % n;
-                    s_part(k, r) = __ldcg(reinterpret_cast<const float2 *>(a.part_ml + (size_t)slot_of(k) * 32) + r);
+                for (uint32_t r = warp; r < rows; r += kWarps) {
+                    float M = kNoMax, L = 0.0f;
+                    float2 ml[3];
+                    #pragma unroll
+                    for (int i = 0; i < 3; i++) {
+                        const uint32_t k = lane + 32 * i;
+                        ml[i] = make_float2(kNoMax, 0.0f);
+                        if (k < n) ml[i] = __ldcg(reinterpret_cast<const float2 *>(a.part_ml + slot_of(k) * 32) + r);
+                        M = fmaxf(M, ml[i].x);
+                    }
+                    #pragma unroll
+                    for (int d = 1; d < 32; d <<= 1) M = fmaxf(M, __shfl_xor_sync(0xFFFFFFFFu, M, d));
+                    #pragma unroll
+                    for (int i = 0; i < 3; i++) {
+                        const float f = ex2(ml[i].x - M);
+                        L += ml[i].y * f;
+                        if (lane + 32 * i < n) s_weight(r, lane + 32 * i) = f;
+                    }
+                    #pragma unroll
+                    for (int d = 1; d < 32; d <<= 1) L += __shfl_xor_sync(0xFFFFFFFFu, L, d);
+                    if (lane == 0) {
+                        s_ml[0][r][0] = more ? 1.0f : L == 0.0f ? 0.0f : rcp(L);
+                        if (more) __stcg(reinterpret_cast<float2 *>(a.part_ml + (size_t)to * 32) + r, make_float2(M, L));
+                        else if (a.lse) a.lse[(size_t)seq * a.n_q_heads + query_head(r)] = (M + lg2(L)) * kLn2;
+                    }
                 }
                 __syncthreads();
-                const uint32_t to = slot_of(0);
-                const bool more = tree && round == 0;
                 #pragma unroll 1
                 for (uint32_t c = tid; c < rows * (D / 4); c += kThreads) {
                     const uint32_t r = c / (D / 4), d = (c % (D / 4)) * 4;
-                    float M = kNoMax, L = 0.0f;
-                    #pragma unroll 1
-                    for (uint32_t k = 0; k < n; k++) M = fmaxf(M, s_part(k, r).x);
                     float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
                     #pragma unroll 1
                     for (uint32_t k0 = 0; k0 < n; k0 += 8) {
                         float4 v[8];
                         #pragma unroll
-                        for (int k = 0; k < 8; k++)
-                            if (k0 + k < n) v[k] = __ldcg(reinterpret_cast<const float4 *>(a.part_o + ((size_t)slot_of(k0 + k) * 16 + r) * D + d));
+                        for (int k = 0; k < 8; k++)          /* 32-bit offsets: the parts are a few MB */
+                            if (k0 + k < n)
+                                v[k] = __ldcg(reinterpret_cast<const float4 *>(a.part_o + ((slot_of(k0 + k) * 16 + r) * D + d)));
                         #pragma unroll
                         for (int k = 0; k < 8; k++) {
-                            if (k0 + k >= n) continue;
-                            const float2 ml = s_part(k0 + k, r);
-                            const float f = ex2(ml.x - M);
-                            L += ml.y * f;
+                            if (k0 + k >= n) break;
+                            const float f = s_weight(r, k0 + k);
                             acc.x += v[k].x * f; acc.y += v[k].y * f; acc.z += v[k].z * f; acc.w += v[k].w * f;
                         }
                     }
-                    if (more) {
-                        __stcg(reinterpret_cast<float4 *>(a.part_o + ((size_t)to * 16 + r) * D + d), acc);
-                        if (d == 0) __stcg(reinterpret_cast<float2 *>(a.part_ml + (size_t)to * 32) + r, make_float2(M, L));
-                    } else {
-                        finish(r, d, M, L, acc);
-                    }
+                    if (more) __stcg(reinterpret_cast<float4 *>(a.part_o + ((size_t)to * 16 + r) * D + d), acc);
+                    else write(r, d, s_ml[0][r][0], acc);
                 }
                 by = kFan;
             }

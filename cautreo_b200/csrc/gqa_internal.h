@@ -28,8 +28,10 @@ typedef struct {
     uint32_t n_seq, n_q_heads, n_kv_heads, group, n_tiles;   /* group = query heads a kv head, tiles of 16 of them */
     uint32_t page_tokens, max_pages, n_pages, n_pick, window, blocked;
     uint32_t min_steps;          /* least steps a worker takes */
+    uint32_t most_parts;         /* parts of an item, when every worker takes one part */
     float scale_log2;            /* scale x log2(e) */
     uint64_t worker_magic;       /* floor(2^64 / n_workers) + 1: division of less than 2^64 / n_workers */
+    uint64_t spare_magic;        /* the same of n_workers less the batch's items, where that is positive */
     uint32_t page_magic;         /* floor(2^32 / (page_tokens / 16)) + 1; 0 for pages of 16 */
 #ifdef __CUDACC__
     /* Page of token v (below 2^31, page_tokens a multiple of 16 up to 512): a

@@ -10,19 +10,20 @@ namespace ct_gqa {
 
 template <int D, int DT, int HT> static int ctas() {
     using C = Cfg<D, DT, HT>;
-    int n = 0;
-    int rc = ct__cuda_status(cudaFuncSetAttribute(k_gqa_decode<D, DT, HT>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem),
-                             "gqa decode");
-    if (!rc)
-        rc = ct__cuda_status(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, k_gqa_decode<D, DT, HT>, kThreads, C::kSmem),
-                             "gqa decode");
-    return rc ? 0 : n;
+    int n[2] = {0, 0}, rc = CT_OK;
+    for (int few = 0; few < 2 && !rc; few++) {
+        auto kernel = few ? k_gqa_decode<D, DT, HT, true> : k_gqa_decode<D, DT, HT, false>;
+        rc = ct__cuda_status(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem), "gqa decode");
+        if (!rc) rc = ct__cuda_status(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n[few], kernel, kThreads, C::kSmem), "gqa decode");
+    }
+    return rc ? 0 : n[0] < n[1] ? n[0] : n[1];
 }
 
 template <int D, int DT, int HT> static int run(const ct_gqa_args_t *a, uint32_t n_workers, cudaStream_t st) {
+    const bool few = 2ull * a->n_seq * a->n_kv_heads * a->n_tiles <= n_workers;
     ct__count_launches(1);
-    return ct__cuda_status(ct_gqa_launch(k_gqa_decode<D, DT, HT>, dim3(n_workers), dim3(kThreads), Cfg<D, DT, HT>::kSmem, st, 1, *a),
-                           "gqa decode");
+    return ct__cuda_status(ct_gqa_launch(few ? k_gqa_decode<D, DT, HT, true> : k_gqa_decode<D, DT, HT, false>, dim3(n_workers),
+                                         dim3(kThreads), Cfg<D, DT, HT>::kSmem, st, 1, *a), "gqa decode");
 }
 
 /* Groups of up to 8 query heads take one column tile, larger ones two. */

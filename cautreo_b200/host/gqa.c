@@ -216,6 +216,7 @@ static int decode(ct_gqa_plan_t *p, const void *q, uint64_t q_stride, const void
     if (!block_table || !seq_lens || !out || misaligned(out, 8)) return bad("gqa: table, lengths or out");
     if (p->n_seq == 0) return CT_OK;
     const uint32_t group = p->shape.n_q_heads / l->n_kv_heads;
+    const uint64_t items = (uint64_t)p->n_seq * l->n_kv_heads * ((group + 15) / 16);
     const uint32_t page_groups = l->page_tokens / 16;
     const ct_gqa_args_t a = {
         .q = (const uint16_t *)q, .pool = pool, .scales = scales, .block_table = block_table, .seq_lens = seq_lens,
@@ -223,9 +224,14 @@ static int decode(ct_gqa_plan_t *p, const void *q, uint64_t q_stride, const void
         .counters = p->counters, .q_stride = q_stride, .n_seq = p->n_seq, .n_q_heads = p->shape.n_q_heads,
         .n_kv_heads = l->n_kv_heads, .group = group, .n_tiles = (group + 15) / 16, .page_tokens = l->page_tokens,
         .max_pages = l->max_pages_per_seq, .n_pages = l->n_pages, .n_pick = n_select, .window = p->shape.window_tokens,
-        .blocked = p->shape.head_order == CT_GQA_BLOCKED, .min_steps = getenv("GQMIN") ? (uint32_t)atoi(getenv("GQMIN")) : 8,
+        .blocked = p->shape.head_order == CT_GQA_BLOCKED, .min_steps = 8,
+        /* up to 32 parts are joined at once: somewhat fewer workers than there
+         * are beat a second round of joins (one sequence of 8000 tokens,
+         * 8 heads: 32 parts of 13.6 us, 37 of 14.7) */
+        .most_parts = items && p->n_workers / items <= 64 ? 32u : 0xFFFFFFFFu,
         .scale_log2 = p->shape.scale * 1.4426950408889634f,
         .worker_magic = UINT64_MAX / p->n_workers + 1,
+        .spare_magic = items < p->n_workers ? UINT64_MAX / (p->n_workers - items) + 1 : 0,
         .page_magic = page_groups == 1 ? 0u : (uint32_t)(0x100000000ull / page_groups) + 1u,
     };
     int prev = 0;
