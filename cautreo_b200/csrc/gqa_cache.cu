@@ -38,8 +38,9 @@ CT_DEV uint32_t pack2_bf16(float lo, float hi) {
  * tokens; all its loads are in flight before the first is used. */
 
 /* Row of the pool for a token's slot, or none. */
-CT_DEV bool pool_row(int32_t slot, uint32_t place, uint32_t n_kv_heads, uint32_t page_tokens, uint32_t n_pages, size_t &row) {
-    const uint32_t page = (uint32_t)slot / page_tokens;
+CT_DEV bool pool_row(int32_t slot, uint32_t place, uint32_t n_kv_heads, uint32_t page_tokens, uint32_t page_magic, uint32_t n_pages,
+                     size_t &row) {
+    const uint32_t page = ct_gqa_page_of((uint32_t)slot, page_magic);
     if (slot < 0 || page >= n_pages) return false;
     row = ((size_t)page * 2 * n_kv_heads + place) * page_tokens + ((uint32_t)slot - page * page_tokens);
     return true;
@@ -48,7 +49,7 @@ CT_DEV bool pool_row(int32_t slot, uint32_t place, uint32_t n_kv_heads, uint32_t
 template <int D, int DT, bool F32, int T>
 __global__ void __launch_bounds__(kThreads) k_gqa_write(void *pool, float *scales, const void *ks, const void *vs, size_t k_stride,
                                                         size_t v_stride, const int32_t *slots, uint32_t n, uint32_t n_kv_heads,
-                                                        uint32_t page_tokens, uint32_t n_pages) {
+                                                        uint32_t page_tokens, uint32_t page_magic, uint32_t n_pages) {
     constexpr int L = lanes_of(D), U = D / 8, R = kThreads / L;
     const uint32_t u = threadIdx.x % L, place = blockIdx.y;
     const bool is_v = place >= n_kv_heads;
@@ -107,7 +108,7 @@ __global__ void __launch_bounds__(kThreads) k_gqa_write(void *pool, float *scale
         const uint32_t from = (threadIdx.x & (32 - L)) | (i & (L - 1));
         const float di = T == 1 ? d : __shfl_sync(0xFFFFFFFFu, d, from), idi = T == 1 ? id : __shfl_sync(0xFFFFFFFFu, id, from);
         size_t row = 0;
-        if (!pool_row(slot[i], place, n_kv_heads, page_tokens, n_pages, row) || u >= U) continue;
+        if (!pool_row(slot[i], place, n_kv_heads, page_tokens, page_magic, n_pages, row) || u >= U) continue;
         if (DT == CT_KV_BF16 && !F32) {
             *reinterpret_cast<uint4 *>(static_cast<uint16_t *>(pool) + row * D + u * 8) = w[i][0];
             continue;
@@ -175,7 +176,7 @@ template <int D, int DT> CT_DEV uint4 load8(const void *pool, size_t row, uint32
 
 template <int D, int DT, bool F32, int T>
 __global__ void __launch_bounds__(kThreads) k_gqa_read(const void *pool, const float *scales, const int32_t *slots, uint32_t n,
-                                                       uint32_t n_kv_heads, uint32_t page_tokens, uint32_t n_pages, void *ko,
+                                                       uint32_t n_kv_heads, uint32_t page_tokens, uint32_t page_magic, uint32_t n_pages, void *ko,
                                                        void *vo, size_t k_stride, size_t v_stride) {
     constexpr int L = lanes_of(D), U = D / 8, R = kThreads / L;
     const uint32_t u = threadIdx.x % L, place = blockIdx.y;
@@ -194,7 +195,7 @@ __global__ void __launch_bounds__(kThreads) k_gqa_read(const void *pool, const f
     #pragma unroll
     for (int i = 0; i < T; i++) {
         size_t row = 0;
-        ok[i] = pool_row(slot[i], place, n_kv_heads, page_tokens, n_pages, row);
+        ok[i] = pool_row(slot[i], place, n_kv_heads, page_tokens, page_magic, n_pages, row);
         sc[i] = 1.0f;
         if (!ok[i]) continue;
         w[i] = load8<D, DT>(pool, row, u);
@@ -318,7 +319,7 @@ struct WriteCall {
     }
     template <class K> cudaError_t launch(K k_, uint32_t tokens) const {
         return ct_gqa_launch(k_, dim3((n + tokens - 1) / tokens, 2 * heads), dim3(kThreads), 0, st, 1, pool, scales, k, v, ks, vs,
-                             slots, n, heads, pt, np);
+                             slots, n, heads, pt, ct_gqa_page_magic(pt), np);
     }
 };
 
@@ -333,7 +334,7 @@ struct ReadCall {
     }
     template <class K> cudaError_t launch(K k_, uint32_t tokens) const {
         return ct_gqa_launch(k_, dim3((n + tokens - 1) / tokens, 2 * heads), dim3(kThreads), 0, st, 1, pool, scales, slots, n, heads,
-                             pt, np, k, v, ks, vs);
+                             pt, ct_gqa_page_magic(pt), np, k, v, ks, vs);
     }
 };
 

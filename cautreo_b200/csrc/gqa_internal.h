@@ -12,6 +12,12 @@
 extern "C" {
 #endif
 
+/* For dividing tokens by page_tokens (a multiple of 16 up to 512):
+ * floor(2^32 / (page_tokens / 16)) + 1; 0 for pages of 16. */
+static inline uint32_t ct_gqa_page_magic(uint32_t page_tokens) {
+    return page_tokens == 16 ? 0u : (uint32_t)(0x100000000ull / (page_tokens / 16)) + 1u;
+}
+
 /* One decode launch.  All pointers are device pointers. */
 typedef struct {
     const uint16_t *q;           /* bf16 [n_seq][n_q_heads][D], rows q_stride values apart */
@@ -32,13 +38,9 @@ typedef struct {
     float scale_log2;            /* scale x log2(e) */
     uint64_t worker_magic;       /* floor(2^64 / n_workers) + 1: division of less than 2^64 / n_workers */
     uint64_t spare_magic;        /* the same of n_workers less the batch's items, where that is positive */
-    uint32_t page_magic;         /* floor(2^32 / (page_tokens / 16)) + 1; 0 for pages of 16 */
+    uint32_t page_magic;         /* ct_gqa_page_magic(page_tokens) */
 #ifdef __CUDACC__
-    /* Page of token v (below 2^31, page_tokens a multiple of 16 up to 512): a
-     * product instead of a division; exact while v / 16 < 2^32 / (page_tokens / 16). */
-    __device__ __forceinline__ uint32_t page_of(uint32_t v) const {
-        return page_magic ? __umulhi(v >> 4, page_magic) : v >> 4;
-    }
+    __device__ __forceinline__ uint32_t page_of(uint32_t v) const;
 #endif
 } ct_gqa_args_t;
 
@@ -89,6 +91,12 @@ int ct__launch_gqa_bounds(const void *pool, const float *scales, uint32_t dtype,
 
 #ifdef __CUDACC__
 #include <cuda_runtime.h>
+/* Page of token v (below 2^31): a product instead of a division; exact while
+ * v / 16 < 2^32 / (page_tokens / 16). */
+static __device__ __forceinline__ uint32_t ct_gqa_page_of(uint32_t v, uint32_t magic) {
+    return magic ? __umulhi(v >> 4, magic) : v >> 4;
+}
+__device__ __forceinline__ uint32_t ct_gqa_args_t::page_of(uint32_t v) const { return ct_gqa_page_of(v, page_magic); }
 /* These kernels are launched while the kernel before them on the stream still
  * drains (programmatic stream serialization): each first lets its own
  * successor do the same, then waits until everything before it has finished

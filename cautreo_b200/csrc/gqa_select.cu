@@ -13,8 +13,8 @@
  *
  * Bound: HBM, 2 D + 4 bytes a page and head.  A CTA per (sequence, kv head),
  * or a cluster of up to 8 when that leaves SMs idle: its warps take 16 pages
- * at a time, 8 as the columns of a mma.sync m16n8k32 (int8), the heads of the
- * group being the rows, with the next pages' numbers loaded ahead.  The scores
+ * at a time, as the rows of mma.sync m16n8k32 (int8), 8 heads of the group
+ * being the columns, with the next pages' numbers loaded ahead.  The scores
  * become ordered 32-bit keys in the first CTA's shared memory; a radix select
  * over the bits that differ finds the key of the last page chosen, and a scan
  * writes the pages in ascending order.
@@ -34,7 +34,7 @@ namespace cg = cooperative_groups;
 
 constexpr int kThreads = 256, kWarps = kThreads / 32;
 constexpr uint32_t kMaxPages = 49152;                        /* keys in shared memory: 192 KB */
-constexpr int kTiles = 2;                                    /* 8-page tiles a warp takes at a time */
+constexpr int kTiles = 2;                                    /* runs of 8 pages a warp takes at a time: the rows of an MMA */
 constexpr uint32_t kKeyInf = 0xFF800000u, kKeyForced = 0xFFFFFFFFu;
 
 CT_DEV void mma_s8(int *c, const uint32_t *a, uint32_t b0, uint32_t b1) {
@@ -105,13 +105,12 @@ __global__ void __launch_bounds__(kThreads, D <= 128 ? 4 : 2) k_gqa_select(const
                 s_q[r][D + lane + 32 * i] = (int8_t)min(c, 0);
             }
             if (lane == 0) {
-                s_e[r] = e;
+                s_e[r] = live ? e : -1.0f;
                 if (top >= 0x7F800000u) s_bad = 1;
             }
         }
         __syncthreads();
         const uint32_t rows = a.group - tile * 16 < 16 ? a.group - tile * 16 : 16;
-        const float e0 = s_e[g], e1 = s_e[g + 8];
         const bool bad = s_bad != 0;
         constexpr uint32_t kStep = kTiles * 8;
         const uint32_t pb = (uint32_t)((uint64_t)have * rank / ranks), pe = (uint32_t)((uint64_t)have * (rank + 1) / ranks);
@@ -139,37 +138,38 @@ __global__ void __launch_bounds__(kThreads, D <= 128 ? 4 : 2) k_gqa_select(const
                 const uint32_t p = p0 + kWarps * kStep + t * 8 + g;
                 ph[t] = p < pe ? __ldg(table + p) : -1;
             }
-            int c[kTiles][4];
+            /* rows = pages p0 + g and p0 + 8 + g, columns = heads 2j, 2j + 1 of a
+             * tile; lane j owns bytes 16 j .. 16 j + 15 of each 64 */
+            float m[2] = {-INFINITY, -INFINITY};
             #pragma unroll
-            for (int t = 0; t < kTiles; t++) c[t][0] = c[t][1] = c[t][2] = c[t][3] = 0;
-            #pragma unroll
-            for (int b = 0; b < D / 32; b++) {               /* 64 bytes of a row: lane j owns bytes 16 j .. 16 j + 15 */
-                const uint4 q0 = *reinterpret_cast<const uint4 *>(&s_q[g][b * 64 + 16 * j]);
-                const uint4 q1 = rows > 8 ? *reinterpret_cast<const uint4 *>(&s_q[g + 8][b * 64 + 16 * j]) : make_uint4(0u, 0u, 0u, 0u);
-                const uint32_t a0[4] = {q0.x, q1.x, q0.y, q1.y}, a1[4] = {q0.z, q1.z, q0.w, q1.w};
+            for (int ht = 0; ht < 2; ht++) {
+                if (8 * ht >= (int)rows) break;
+                int c[4] = {0, 0, 0, 0};
                 #pragma unroll
-                for (int t = 0; t < kTiles; t++) {
-                    mma_s8(c[t], a0, w[t][b].x, w[t][b].y);
-                    mma_s8(c[t], a1, w[t][b].z, w[t][b].w);
+                for (int b = 0; b < D / 32; b++) {
+                    const uint4 q = *reinterpret_cast<const uint4 *>(&s_q[8 * ht + g][b * 64 + 16 * j]);
+                    const uint32_t a0[4] = {w[0][b].x, w[1][b].x, w[0][b].y, w[1][b].y};
+                    const uint32_t a1[4] = {w[0][b].z, w[1][b].z, w[0][b].w, w[1][b].w};
+                    mma_s8(c, a0, q.x, q.y);
+                    mma_s8(c, a1, q.z, q.w);
+                }
+                #pragma unroll
+                for (int h = 0; h < 2; h++) {                /* heads past the group have e = -1 */
+                    const float e = s_e[8 * ht + 2 * j + h];
+                    #pragma unroll
+                    for (int t = 0; t < 2; t++) m[t] = fmaxf(m[t], e < 0.0f ? -INFINITY : __fmul_rn((float)c[2 * t + h], e));
                 }
             }
             #pragma unroll
             for (int t = 0; t < kTiles; t++) {
-                #pragma unroll
-                for (int h = 0; h < 2; h++) {                /* pages p0 + 8t + 2j + h */
-                    float m = g < rows ? __fmul_rn((float)c[t][h], e0) : -INFINITY;
-                    if (g + 8 < rows) m = fmaxf(m, __fmul_rn((float)c[t][2 + h], e1));
-                    #pragma unroll
-                    for (int o = 4; o < 32; o <<= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
-                    const float pscale = __shfl_sync(0xFFFFFFFFu, ps[t], (2 * j + h) * 4);
-                    const bool pok = __shfl_sync(0xFFFFFFFFu, ok[t] ? 1 : 0, (2 * j + h) * 4) != 0;
-                    const uint32_t pp = p0 + t * 8 + 2 * j + h;
-                    if (g == 0 && pp < pe) {
-                        uint32_t key = bad ? kKeyInf : key_of(__fmul_rn(m, pscale));
-                        if (pp < a.n_first || pp + a.n_last >= have) key = kKeyForced;
-                        if (!pok) key = 0;
-                        lead[pp] = tile ? max(lead[pp], key) : key;
-                    }
+                m[t] = fmaxf(m[t], __shfl_xor_sync(0xFFFFFFFFu, m[t], 1));
+                m[t] = fmaxf(m[t], __shfl_xor_sync(0xFFFFFFFFu, m[t], 2));
+                const uint32_t pp = p0 + t * 8 + g;
+                if (j == 0 && pp < pe) {
+                    uint32_t key = bad ? kKeyInf : key_of(__fmul_rn(m[t], ps[t]));
+                    if (pp < a.n_first || pp + a.n_last >= have) key = kKeyForced;
+                    if (!ok[t]) key = 0;
+                    lead[pp] = tile ? max(lead[pp], key) : key;
                 }
             }
         }

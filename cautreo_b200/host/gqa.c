@@ -217,7 +217,6 @@ static int decode(ct_gqa_plan_t *p, const void *q, uint64_t q_stride, const void
     if (p->n_seq == 0) return CT_OK;
     const uint32_t group = p->shape.n_q_heads / l->n_kv_heads;
     const uint64_t items = (uint64_t)p->n_seq * l->n_kv_heads * ((group + 15) / 16);
-    const uint32_t page_groups = l->page_tokens / 16;
     const ct_gqa_args_t a = {
         .q = (const uint16_t *)q, .pool = pool, .scales = scales, .block_table = block_table, .seq_lens = seq_lens,
         .picked = pages, .out = (uint16_t *)out, .lse = lse, .part_o = p->part_o, .part_ml = p->part_ml,
@@ -232,7 +231,7 @@ static int decode(ct_gqa_plan_t *p, const void *q, uint64_t q_stride, const void
         .scale_log2 = p->shape.scale * 1.4426950408889634f,
         .worker_magic = UINT64_MAX / p->n_workers + 1,
         .spare_magic = items < p->n_workers ? UINT64_MAX / (p->n_workers - items) + 1 : 0,
-        .page_magic = page_groups == 1 ? 0u : (uint32_t)(0x100000000ull / page_groups) + 1u,
+        .page_magic = ct_gqa_page_magic(l->page_tokens),
     };
     int prev = 0;
     if ((rc = enter(p->device, &prev))) return rc;
