@@ -219,79 +219,147 @@ __global__ void __launch_bounds__(kThreads) k_gqa_read(const void *pool, const f
     }
 }
 
+/* Running maxima and minima of a thread's 8 values, over rows w (as load8
+ * gives them) with scales sc, and whether any row held a NaN or an infinity.
+ * bf16 stays packed: a maximum of bf16 values is one of them. */
+template <int DT> struct Range8 {
+    float hi[8], lo[8];
+    bool bad;
+    CT_DEV void start() {
+        bad = false;
+        #pragma unroll
+        for (int e = 0; e < 8; e++) { hi[e] = -INFINITY; lo[e] = INFINITY; }
+    }
+    CT_DEV void take(const uint4 &w, float sc) {
+        bad = bad || !(fabsf(sc) < INFINITY);                /* 8-bit pools: only a scale can be NaN */
+        const uint32_t ws[2] = {w.x, w.y};
+        #pragma unroll
+        for (int i = 0; i < 8; i += 2) {
+            float2 f;
+            if (DT == CT_KV_INT8) {                          /* byte + 128 under the exponent of 2^23, minus 2^23 + 128 */
+                const uint32_t b = ws[i >> 2] ^ 0x80808080u;
+                f.x = __uint_as_float(__byte_perm(b, 0x4B000000u, 0x7540 | (i & 3))) - 8388736.0f;
+                f.y = __uint_as_float(__byte_perm(b, 0x4B000000u, 0x7540 | ((i & 3) + 1))) - 8388736.0f;
+            } else {
+                f = ct_e4m3x2_to_f32x2((uint16_t)(ws[i >> 2] >> (8 * (i & 3))));
+            }
+            f.x = __fmul_rn(f.x, sc);
+            f.y = __fmul_rn(f.y, sc);
+            hi[i] = fmaxf(hi[i], f.x); lo[i] = fminf(lo[i], f.x);
+            hi[i + 1] = fmaxf(hi[i + 1], f.y); lo[i + 1] = fminf(lo[i + 1], f.y);
+        }
+    }
+    CT_DEV void finish() {}
+};
+template <> struct Range8<CT_KV_BF16> {
+    float hi[8], lo[8];
+    bool bad;
+    __nv_bfloat162 ph[4], pl[4];
+    uint32_t top;
+    CT_DEV void start() {
+        top = 0;
+        #pragma unroll
+        for (int e = 0; e < 4; e++) {
+            ph[e] = __nv_bfloat162(__nv_bfloat162_raw{0xFF80, 0xFF80});
+            pl[e] = __nv_bfloat162(__nv_bfloat162_raw{0x7F80, 0x7F80});
+        }
+    }
+    CT_DEV void take(const uint4 &w, float) {
+        const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
+        #pragma unroll
+        for (int e = 0; e < 4; e++) {
+            const __nv_bfloat162 v = *reinterpret_cast<const __nv_bfloat162 *>(&ws[e]);
+            ph[e] = __hmax2(ph[e], v);
+            pl[e] = __hmin2(pl[e], v);
+        }
+        top = __vimax3_u16x2(top, ws[0] & 0x7FFF7FFFu, ws[1] & 0x7FFF7FFFu);
+        top = __vimax3_u16x2(top, ws[2] & 0x7FFF7FFFu, ws[3] & 0x7FFF7FFFu);
+    }
+    CT_DEV void finish() {
+        bad = max(top & 0xFFFFu, top >> 16) >= 0x7F80u;
+        #pragma unroll
+        for (int e = 0; e < 4; e++) {
+            const float2 h = __bfloat1622float2(ph[e]), l = __bfloat1622float2(pl[e]);
+            hi[2 * e] = h.x; hi[2 * e + 1] = h.y;
+            lo[2 * e] = l.x; lo[2 * e + 1] = l.y;
+        }
+    }
+};
+
 /* Bounds of a page's keys, one CTA per (listed page, head):
  *   hi_d = max_t k_td, lo_d = min_t k_td over the page's first `count` tokens,
  *   s = max_d max(|hi_d|, |lo_d|) / 127, codes ceil(hi / s) and floor(lo / s).
  * Maxima and minima have no order, so a page's bounds are the same whichever
- * way its tokens came.  A NaN or an infinity among the keys: scale NaN. */
+ * way its tokens came.  A NaN or an infinity among the keys: scale NaN.
+ * Bound by instructions when many pages are new (their keys are still in L2):
+ * see Range8; by latency when few are. */
+constexpr int kBoundThreads = 128;
 template <int D, int DT>
-__global__ void __launch_bounds__(128) k_gqa_bounds(const void *pool, const float *scales, uint32_t n_kv_heads, uint32_t page_tokens,
-                                                    uint32_t n_pages, const int32_t *pages, const int32_t *counts, int8_t *bounds,
-                                                    float *bound_scales) {
-    constexpr int U = D / 8, R = 128 / U;                    /* threads along the row, tokens at a time */
+__global__ void __launch_bounds__(kBoundThreads) k_gqa_bounds(const void *pool, const float *scales, uint32_t n_kv_heads,
+                                                              uint32_t page_tokens, uint32_t n_pages, const int32_t *pages,
+                                                              const int32_t *counts, int8_t *bounds, float *bound_scales) {
+    constexpr int U = D / 8, R = kBoundThreads / U, W = kBoundThreads / 32;      /* threads along the row, tokens at a time */
     __shared__ float s_hi[R][D], s_lo[R][D];
-    __shared__ uint32_t s_top[4], s_bad;
+    __shared__ float s_top[W];
     ct_gqa_enter();
-    const uint32_t i = blockIdx.x / n_kv_heads, head = blockIdx.x % n_kv_heads;
-    const int32_t page = pages[i];
+    const uint32_t i = blockIdx.x / n_kv_heads, head = blockIdx.x - i * n_kv_heads;
+    const int32_t page = __ldg(pages + i), ct = __ldg(counts + i);
     if (page < 0 || (uint32_t)page >= n_pages) return;
-    const int32_t ct = counts[i];
-    const uint32_t count = ct < 0 ? 0u : ((uint32_t)ct > page_tokens ? page_tokens : (uint32_t)ct);
+    const uint32_t count = ct < 0 ? 0u : min((uint32_t)ct, page_tokens);
     const uint32_t u = threadIdx.x % U, r = threadIdx.x / U;
     const size_t row0 = ((size_t)page * 2 * n_kv_heads + head) * page_tokens;
-    if (threadIdx.x == 0) s_bad = 0;
-    __syncthreads();
-    float hi[8], lo[8];
-    uint32_t top = 0;
-    #pragma unroll
-    for (int e = 0; e < 8; e++) { hi[e] = -INFINITY; lo[e] = INFINITY; }
+    Range8<DT> range;
+    range.start();
     if (r < R) {
-        for (uint32_t t = r; t < count; t += 4 * R) {        /* four rows' loads in flight */
-            uint4 w[4];
-            float sc[4];
+        #pragma unroll 1
+        for (uint32_t t = r; t < count; t += 8 * R) {        /* eight rows' loads in flight */
+            uint4 w[8];
+            float sc[8];
             #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const size_t row = row0 + min(t + i * R, count - 1);     /* past the end: the last token once more */
-                w[i] = load8<D, DT>(pool, row, u);
-                sc[i] = DT == CT_KV_BF16 ? 1.0f : __ldg(scales + row);
+            for (int k = 0; k < 8; k++) {
+                const size_t row = row0 + min(t + k * R, count - 1);     /* past the end: the last token once more */
+                w[k] = load8<D, DT>(pool, row, u);
+                sc[k] = DT == CT_KV_BF16 ? 1.0f : __ldg(scales + row);
             }
             #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                float x[8];
-                values8<DT>(w[i], sc[i], x);
-                #pragma unroll
-                for (int e = 0; e < 8; e++) {
-                    top = max(top, __float_as_uint(x[e]) & 0x7FFFFFFFu);
-                    hi[e] = fmaxf(hi[e], x[e]);
-                    lo[e] = fminf(lo[e], x[e]);
-                }
-            }
+            for (int k = 0; k < 8; k++) range.take(w[k], sc[k]);
         }
+    }
+    range.finish();
+    if (r < R) {
         #pragma unroll
-        for (int e = 0; e < 8; e++) { s_hi[r][u * 8 + e] = hi[e]; s_lo[r][u * 8 + e] = lo[e]; }
-    }
-    if (top >= 0x7F800000u) s_bad = 1;
-    #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
-    if ((threadIdx.x & 31) == 0) s_top[threadIdx.x >> 5] = top;
-    __syncthreads();
-    top = max(max(s_top[0], s_top[1]), max(s_top[2], s_top[3]));
-    const bool bad = s_bad != 0;
-    const float s = __fdiv_rn(__uint_as_float(top), 127.0f);
-    const size_t out = (size_t)page * n_kv_heads + head;
-    for (uint32_t d = threadIdx.x; d < (uint32_t)D; d += 128) {
-        float h = s_hi[0][d], l = s_lo[0][d];
-        #pragma unroll 4
-        for (int k = 1; k < R; k++) { h = fmaxf(h, s_hi[k][d]); l = fminf(l, s_lo[k][d]); }
-        int ch = 0, cl = 0;
-        if (!bad && s > 0.0f) {
-            ch = max(-127, min(127, __float2int_ru(__fdiv_rn(h, s))));
-            cl = max(-127, min(127, __float2int_rd(__fdiv_rn(l, s))));
+        for (int e = 0; e < 8; e += 4) {
+            *reinterpret_cast<float4 *>(&s_hi[r][u * 8 + e]) = make_float4(range.hi[e], range.hi[e + 1], range.hi[e + 2], range.hi[e + 3]);
+            *reinterpret_cast<float4 *>(&s_lo[r][u * 8 + e]) = make_float4(range.lo[e], range.lo[e + 1], range.lo[e + 2], range.lo[e + 3]);
         }
-        bounds[out * 2 * D + d] = (int8_t)ch;
-        bounds[out * 2 * D + D + d] = (int8_t)cl;
     }
-    if (threadIdx.x == 0) bound_scales[out] = bad ? __uint_as_float(0x7FC00000u) : s;
+    float top = 0.0f;
+    #pragma unroll
+    for (int e = 0; e < 8; e++) top = fmaxf(top, fmaxf(fabsf(range.hi[e]), fabsf(range.lo[e])));
+    if (r >= R || count <= r) top = 0.0f;                    /* a thread without tokens */
+    top = ct_warp_max(top);
+    if ((threadIdx.x & 31) == 0) s_top[threadIdx.x >> 5] = top;
+    const bool fine = !__syncthreads_or(r < R && range.bad);
+    #pragma unroll
+    for (int k = 0; k < W; k++) top = fmaxf(top, s_top[k]);
+    const float s = __fdiv_rn(top, 127.0f);
+    const size_t out = (size_t)page * n_kv_heads + head;
+    /* a bound a thread at a time: the upper ones, then the lower ones */
+    #pragma unroll 1
+    for (uint32_t c = threadIdx.x; c < 2 * D; c += kBoundThreads) {
+        const bool lower = c >= D;
+        const float *from = lower ? &s_lo[0][c - D] : &s_hi[0][c];
+        float b = from[0];
+        #pragma unroll 8
+        for (int k = 1; k < R; k++) b = lower ? fminf(b, from[k * D]) : fmaxf(b, from[k * D]);
+        int code = 0;
+        if (fine && s > 0.0f) {
+            const float y = __fdiv_rn(b, s);
+            code = max(-127, min(127, lower ? __float2int_rd(y) : __float2int_ru(y)));
+        }
+        bounds[out * 2 * D + c] = (int8_t)code;
+    }
+    if (threadIdx.x == 0) bound_scales[out] = fine ? s : __uint_as_float(0x7FC00000u);
 }
 
 #define CT_BY_DIM(call)                            \
@@ -353,8 +421,8 @@ int bounds_of(const void *pool, const float *scales, uint32_t dtype, uint32_t he
     auto kernel = dtype == CT_KV_BF16 ? k_gqa_bounds<D, CT_KV_BF16> : dtype == CT_KV_INT8 ? k_gqa_bounds<D, CT_KV_INT8>
                                                                                      : k_gqa_bounds<D, CT_KV_E4M3>;
     ct__count_launches(1);
-    return ct__cuda_status(ct_gqa_launch(kernel, dim3(n * heads), dim3(128), 0, st, 1, pool, scales, heads, pt, np, pages, counts,
-                                         bounds, bs), "gqa bounds");
+    return ct__cuda_status(ct_gqa_launch(kernel, dim3(n * heads), dim3(kBoundThreads), 0, st, 1, pool, scales, heads, pt, np, pages,
+                                         counts, bounds, bs), "gqa bounds");
 }
 
 }  // namespace
