@@ -6,7 +6,7 @@
  * Math (sequence s, query head h of kv head c, tokens t that the mask keeps):
  *   x_t = scale * q_h . k_t,  out_h = sum_t softmax(x)_t v_t,  lse_h = ln sum_t exp x_t
  * as one pass over the tokens with a running maximum and sum in the log2
- * domain; a maximum is only followed when it grows by more than 2^8, so the
+ * domain; a maximum is only followed when it grows by more than 2^3, so the
  * accumulators are rescaled a few times per sequence.
  *
  * Bound: HBM.  A token of a head is 4 D bytes (bf16) for 4 G D flops, G <= 16
@@ -23,7 +23,7 @@
  * as large as the rounding of the output).  8-bit pools: codes are widened to
  * fp16 (exact), queries are brought to fp16 by a power of two a head (exact
  * down to 2^-29 of the head's largest value), and probability x V scale is
- * one fp16 digit (11 bits) of a running power-of-two unit; see `unit`.
+ * one fp16 digit (11 bits) in a running power-of-two unit; see `unit`.
  *
  * Split: an item is a (sequence, kv head, group of 16 heads); a step of it
  * TS tokens.  The steps of the whole batch lie end to end, each item with
@@ -49,9 +49,8 @@ constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
-constexpr float kGrow = 8.0f;           /* log2 growth of a maximum that is followed */
+constexpr float kGrow = 3.0f;           /* log2 growth of a maximum that is followed */
 constexpr float kNoMax = -3.402823466e38f;  /* maximum of no tokens: finite, so that no difference of maxima is NaN */
-constexpr float kTopWeight = 32768.0f;  /* fp16 weights stay below this */
 constexpr uint32_t kItemCost = 4;       /* steps that an item's start and end are counted as */
 constexpr uint32_t kSoloMost = 16; /* longest item of one warp: longer ones would leave the others idle at the end */
 constexpr uint32_t kSoloCost = 3;       /* start and end of an item, in steps of one warp, */
@@ -146,6 +145,7 @@ CT_DEV uint32_t pack_f16(float lo, float hi) {
 }
 CT_DEV float bf16_lo(uint32_t w) { return __uint_as_float(w << 16); }
 CT_DEV float bf16_hi(uint32_t w) { return __uint_as_float(w & 0xFFFF0000u); }
+CT_DEV float inverse_pow2(float x) { return __uint_as_float(0x7F000000u - __float_as_uint(x)); }
 CT_DEV float pow2f(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }   /* -126 <= e <= 127 */
 
 /* Four codes (a 32-bit word) -> two fp16 pairs, exact: bytes (0, 1), (2, 3),
@@ -547,18 +547,18 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, DT, HT>::kMinB) k_gqa_decode(
             #pragma unroll
             for (int t = 0; t < HT; t++) o[b][t][0] = o[b][t][1] = o[b][t][2] = o[b][t][3] = 0.0f;
         float m[HT][2], l[HT][2];
-        /* 8-bit pools: the fp16 weights are probability x V scale x 2^unit.
-         * The unit brought the largest weight of some step to [2^7, 2^8); it
-         * is set anew when a weight would pass 2^15 or when a maximum grew, so
-         * a weight keeps its 11 bits down to 2^-22 of the largest one that
-         * still counts. */
-        float unit[HT][2];                                   /* 2^unit */
-        bool renew = true, blank = true;                     /* blank: some head has seen no token yet, */
+        /* 8-bit pools: the fp16 weights are probability (at most 2^kGrow) x V
+         * scale x unit, a power of two that brought the largest V scale of
+         * some step to [2^11, 2^12) and falls when one would pass that; so a
+         * weight is below 2^15, and keeps its 11 bits where its V scale is
+         * 2^-25 of the largest or more. */
+        float unit = 1.0f;
+        bool blank = true, renew = true;                     /* blank: some head has seen no token yet, */
         uint32_t seen = 0;                                   /* bits of those that have */
         #pragma unroll
         for (int t = 0; t < HT; t++)
             #pragma unroll
-            for (int h = 0; h < 2; h++) { m[t][h] = 0.0f; l[t][h] = 0.0f; unit[t][h] = 1.0f; }
+            for (int h = 0; h < 2; h++) m[t][h] = l[t][h] = 0.0f;
 
         #pragma unroll 1
         for (uint32_t i = z.wb; i < z.we;) {
@@ -653,29 +653,45 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, DT, HT>::kMinB) k_gqa_decode(
                     #pragma unroll
                     for (int h = 0; h < 4; h++) top = fmaxf(top, s[gr][t][h]);
             if (__any_sync(0xFFFFFFFFu, blank || top > kGrow)) {
-                renew = true;
-                blank = false;
+                float by[HT][2];                             /* how far the maxima move */
                 #pragma unroll
-                for (int t = 0; t < HT; t++) {
+                for (int t = 0; t < HT; t++)
                     #pragma unroll
                     for (int h = 0; h < 2; h++) {
-                        const uint32_t bit = 1u << (2 * t + h);
-                        const bool none = (seen & bit) == 0;
-                        float by = none ? -INFINITY : 0.0f;  /* how far the maximum moves */
+                        by[t][h] = (seen >> (2 * t + h)) & 1u ? 0.0f : -INFINITY;
                         #pragma unroll
-                        for (int gr = 0; gr < GR; gr++) by = fmaxf(by, fmaxf(s[gr][t][h], s[gr][t][2 + h]));
-                        #pragma unroll
-                        for (int d = 4; d < 32; d <<= 1) by = fmaxf(by, __shfl_xor_sync(0xFFFFFFFFu, by, d));
-                        if (by == -INFINITY) { blank = true; continue; }
-                        const float f = none ? 1.0f : ex2(-by);
-                        seen |= bit;
-                        m[t][h] += by;
-                        l[t][h] *= f;
-                        #pragma unroll
-                        for (int gr = 0; gr < GR; gr++) { s[gr][t][h] -= by; s[gr][t][2 + h] -= by; }
-                        #pragma unroll
-                        for (int b = 0; b < KB; b++) { o[b][t][h] *= f; o[b][t][2 + h] *= f; }
+                        for (int gr = 0; gr < GR; gr++) by[t][h] = fmaxf(by[t][h], fmaxf(s[gr][t][h], s[gr][t][2 + h]));
                     }
+                #pragma unroll
+                for (int d = 4; d < 32; d <<= 1)
+                    #pragma unroll
+                    for (int t = 0; t < HT; t++)
+                        #pragma unroll
+                        for (int h = 0; h < 2; h++) by[t][h] = fmaxf(by[t][h], __shfl_xor_sync(0xFFFFFFFFu, by[t][h], d));
+                const uint32_t was = seen;
+                blank = false;
+                #pragma unroll
+                for (int t = 0; t < HT; t++)
+                    #pragma unroll
+                    for (int h = 0; h < 2; h++) {
+                        const bool none = by[t][h] == -INFINITY;         /* still no token */
+                        blank = blank || none;
+                        by[t][h] = none ? 0.0f : by[t][h];
+                        seen |= none ? 0u : 1u << (2 * t + h);
+                        m[t][h] += by[t][h];
+                        #pragma unroll
+                        for (int gr = 0; gr < GR; gr++) { s[gr][t][h] -= by[t][h]; s[gr][t][2 + h] -= by[t][h]; }
+                    }
+                if (was) {                                   /* a head without tokens has no sums */
+                    #pragma unroll
+                    for (int t = 0; t < HT; t++)
+                        #pragma unroll
+                        for (int h = 0; h < 2; h++) {
+                            const float f = (was >> (2 * t + h)) & 1u ? ex2(-by[t][h]) : 1.0f;
+                            l[t][h] *= f;
+                            #pragma unroll
+                            for (int b = 0; b < KB; b++) { o[b][t][h] *= f; o[b][t][2 + h] *= f; }
+                        }
                 }
             }
             #pragma unroll
@@ -688,40 +704,31 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, DT, HT>::kMinB) k_gqa_decode(
                         l[t][h & 1] += s[gr][t][h];
                     }
             if (kQ8) {
-                float wt = 0.0f;
+                float vm = 0.0f;
                 #pragma unroll
-                for (int gr = 0; gr < GR; gr++)
+                for (int gr = 0; gr < GR; gr++) vm = fmaxf(vm, fmaxf(vs[gr][0], vs[gr][1]));
+                if (__any_sync(0xFFFFFFFFu, vm * unit >= 4096.0f || (renew && vm > 0.0f))) {
+                    #pragma unroll
+                    for (int d = 4; d < 32; d <<= 1) vm = fmaxf(vm, __shfl_xor_sync(0xFFFFFFFFu, vm, d));
+                    int to = 11 - ((int)(__float_as_uint(vm) >> 23) - 127);
+                    to = to < -120 ? -120 : to > 100 ? 100 : to;
+                    const float f = pow2f(to) * inverse_pow2(unit);
+                    unit = pow2f(to);
+                    if (!renew) {
+                        #pragma unroll
+                        for (int t = 0; t < HT; t++)
+                            #pragma unroll
+                            for (int b = 0; b < KB; b++) { o[b][t][0] *= f; o[b][t][1] *= f; o[b][t][2] *= f; o[b][t][3] *= f; }
+                    }
+                    renew = false;
+                }
+                #pragma unroll
+                for (int gr = 0; gr < GR; gr++) {
+                    const float w0 = vs[gr][0] * unit, w1 = vs[gr][1] * unit;
                     #pragma unroll
                     for (int t = 0; t < HT; t++)
                         #pragma unroll
-                        for (int h = 0; h < 4; h++) {
-                            s[gr][t][h] *= vs[gr][h >> 1] * unit[t][h & 1];
-                            wt = fmaxf(wt, s[gr][t][h]);
-                        }
-                if (__any_sync(0xFFFFFFFFu, renew || wt >= kTopWeight)) {
-                    renew = false;
-                    #pragma unroll
-                    for (int t = 0; t < HT; t++) {
-                        #pragma unroll
-                        for (int h = 0; h < 2; h++) {
-                            float w = 0.0f;
-                            #pragma unroll
-                            for (int gr = 0; gr < GR; gr++) w = fmaxf(w, fmaxf(s[gr][t][h], s[gr][t][2 + h]));
-                            #pragma unroll
-                            for (int d = 4; d < 32; d <<= 1) w = fmaxf(w, __shfl_xor_sync(0xFFFFFFFFu, w, d));
-                            if (w == 0.0f) { renew = true; continue; }
-                            const int from = (int)(__float_as_uint(unit[t][h]) >> 23) - 127;
-                            int to = from + 7 - ((int)(__float_as_uint(w) >> 23) - 127);
-                            to = to < -100 ? -100 : to > 100 ? 100 : to;
-                            const int by = to - from;
-                            const float f0 = pow2f(by / 2), f1 = pow2f(by - by / 2);
-                            unit[t][h] = pow2f(to);
-                            #pragma unroll
-                            for (int gr = 0; gr < GR; gr++) { s[gr][t][h] = s[gr][t][h] * f0 * f1; s[gr][t][2 + h] = s[gr][t][2 + h] * f0 * f1; }
-                            #pragma unroll
-                            for (int b = 0; b < KB; b++) { o[b][t][h] = o[b][t][h] * f0 * f1; o[b][t][2 + h] = o[b][t][2 + h] * f0 * f1; }
-                        }
-                    }
+                        for (int h = 0; h < 4; h++) s[gr][t][h] *= h < 2 ? w0 : w1;
                 }
             }
             #pragma unroll
@@ -795,7 +802,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, DT, HT>::kMinB) k_gqa_decode(
                 for (int h = 0; h < 2; h++) {
                     const uint32_t r = t * 8 + 2 * j + h;
                     float *dst = mine + r * kJoin;
-                    const float back = kQ8 ? rcp(unit[t][h]) : 1.0f;      /* a power of two: exact */
+                    const float back = kQ8 ? inverse_pow2(unit) : 1.0f;
                     if (r < rows) {
                         #pragma unroll
                         for (int b = 0; b < kJoinCols / 16; b++) {
