@@ -58,16 +58,23 @@ constexpr uint32_t kShareCost = 10;     /* and of one that the warps share */
 constexpr uint32_t kFan = 16;           /* workers whose parts are joined at a time, when an item has more than 2 kFan */
 
 /* Tokens of a warp's step (2 to 17 KB of K and V), steps in its ring, and the
- * CTAs that an SM shall hold.  Three steps of 16 tokens a warp leave 2 CTAs of
- * bf16 x 128 (140 KB of copies in flight), 3 of 8-bit x 128; a third CTA is
- * worth the registers' limit of 168 where it spills nothing: int8 x 128, 256
- * sequences of 256 tokens 53 -> 47 us.  Two steps only where that lets a
- * second CTA in (8-bit x 256, groups above 8: 75 -> 57 us). */
+ * CTAs that an SM shall hold.  What bounds a long batch is how evenly the SMs
+ * share the memory, and that gets worse with the copies in flight: from 100
+ * to 140 KB an SM hides the latency, more lets the SMs nearest to the memory
+ * take more than their part.  So rings have two steps, and CTAs that would
+ * bring more than kInFlight are kept out (32 sequences of 4096 tokens, 8 kv
+ * heads: int8 x 128 170 -> 110 KB 58.0 -> 54.0 us, bf16 x 192 143 -> 135,
+ * bf16 x 256 186 -> 181, and bf16 x 128 208 -> 140 KB 16 sequences 52.0 ->
+ * 51.0).  Rows of 64 bytes or fewer are bound by their instructions and gain
+ * from a third step (8-bit x 64, 16 x 4096 tokens 24.7 -> 22.2 us).  A third
+ * CTA is worth the registers' limit of 168 where it spills nothing: int8 x
+ * 128, 256 sequences of 256 tokens 53 -> 47 us. */
+constexpr int kInFlight = 142 * 1024;
 template <int D, int DT, int HT> struct Cfg {
     static constexpr int kElt = DT == CT_KV_BF16 ? 2 : 1;
     static constexpr int kRow = D * kElt;
     static constexpr int TS = kRow <= 64 ? 32 : 16;
-    static constexpr int kStages = kElt == 1 && HT * D == 512 ? 2 : 3;
+    static constexpr int kStages = kRow <= 64 ? 3 : 2;
     static constexpr int kMinB = HT == 1 && D <= 128 && (kElt == 1 || D <= 64) ? 3 : 1;
     static constexpr int kPitch = kRow + 16;                  /* odd number of 16-B units: conflict-free ldmatrix */
     static constexpr int kScaleBytes = DT == CT_KV_BF16 ? 0 : TS * 8;
@@ -79,7 +86,10 @@ template <int D, int DT, int HT> struct Cfg {
     static constexpr int kQPitch = 2 * D + 16;
     static constexpr int kQBytes = kWarps * HT * 8 * kQPitch;
     static constexpr bool kQueriesInSmem = HT * D >= 192 && kRing + kQBytes <= 226 * 1024;
-    static constexpr int kSmem = kRing + (kQueriesInSmem ? kQBytes : 0);
+    static constexpr int kUsed = kRing + (kQueriesInSmem ? kQBytes : 0);
+    static constexpr int kMost = kRow <= 64 ? 32 : kRing < kInFlight ? kInFlight / kRing : 1;
+    static constexpr int kShare = 227 * 1024 / (kMost + 1);      /* as much as keeps one CTA more out */
+    static constexpr int kSmem = kUsed > kShare ? kUsed : kShare;
 };
 
 CT_DEV uint32_t smem_u32(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
