@@ -8,8 +8,7 @@
  *   d = max|x| / 127 (int8) or / 448 (e4m3),  code = floor(x (1/d) + 1/2) or
  *   e4m3(x (1/d)), every operation rounded once to fp32;
  * a row that holds a NaN or an infinity has scale NaN and codes 0, so that
- * what is read back says so instead of a finite value (and e4m3's NaN code is
- * never stored, which the decode's widening relies on).
+ * what is read back says so instead of a finite value.
  */
 #include <cuda_runtime.h>
 #include <float.h>
@@ -231,8 +230,10 @@ template <int DT> struct Range8 {
         for (int e = 0; e < 8; e++) { hi[e] = -INFINITY; lo[e] = INFINITY; }
     }
     CT_DEV void take(const uint4 &w, float sc) {
-        bad = bad || !(fabsf(sc) < INFINITY);                /* 8-bit pools: only a scale can be NaN */
+        bad = bad || !(fabsf(sc) < INFINITY);
         const uint32_t ws[2] = {w.x, w.y};
+        if (DT == CT_KV_E4M3)                                /* a byte of seven ones is NaN (this cache stores none) */
+            bad = bad || ((((w.x & 0x7F7F7F7Fu) + 0x01010101u) | ((w.y & 0x7F7F7F7Fu) + 0x01010101u)) & 0x80808080u) != 0;
         #pragma unroll
         for (int i = 0; i < 8; i += 2) {
             float2 f;

@@ -662,3 +662,122 @@ def test_plan_refusals_on_the_device():
     assert L.ct_attn_gqa_decode_selected(plan.h, a, 0, a, a, a, a, a, 0, a, None, None) == ct.CT_ERR_ARG
     far = ct.GqaPlan(ct.GqaLayout(1, 64, 16, BF16, 4, 49153), 1, 1)
     assert L.ct_attn_gqa_select_pages(far.h, a, 0, a, a, a, a, 2, 1, 1, a, None) == ct.CT_ERR_UNSUPPORTED
+
+
+def test_page_bounds_see_not_a_number_codes():
+    """An e4m3 pool that another program filled may hold the format's NaN codes."""
+    g = gen(81)
+    heads, dim, page = 2, 96, 32
+    pool, scales = G.make_pool(4, heads, page, dim, E4M3, g)
+    raw = pool.view(torch.uint8)
+    raw[1, 0, 0, 3, 95] = 0x7F                                # page 1, head 0
+    raw[2, 0, 1, 31, 0] = 0xFF                                # page 2, head 1
+    raw[3, 0, 0, 20, 1] = 0x7F                                # behind the count
+    raw[3, 1, 1, 0, 1] = 0x7F                                 # a value, not a key
+    bounds = torch.zeros(4, heads, 2, dim, dtype=torch.int8, device="cuda")
+    bs = torch.zeros(4, heads, device="cuda")
+    ct.gqa_page_bounds(ct.GqaLayout(heads, dim, page, E4M3, 4, 4), pool, scales,
+                       torch.arange(4, dtype=torch.int32, device="cuda"),
+                       torch.tensor([32, 32, 32, 20], dtype=torch.int32, device="cuda"), 4, bounds, bs, stream=stream())
+    torch.cuda.synchronize()
+    assert torch.isnan(bs).tolist() == [[False, False], [True, False], [False, True], [False, False]]
+    assert (bounds[1, 0] == 0).all() and (bounds[2, 1] == 0).all()
+
+
+@pytest.mark.parametrize("dtype,dim,group", [(BF16, 128, 4), (INT8, 128, 16), (E4M3, 64, 1)])
+def test_decode_one_long_sequence_among_many_short(dtype, dim, group):
+    """The long one's items span so many CTAs that their parts are joined in two rounds, beside whole items."""
+    lens = [(i * 7) % 20 for i in range(150)] + [60000] + [(i * 5) % 33 for i in range(150)]
+    decode(lens, 2, group, dim, 64, dtype, seed=82)
+
+
+def test_decode_thousands_of_sequences():
+    lens = [(i * 29) % 41 for i in range(5000)]
+    decode(lens, 2, 2, 64, 16, INT8, seed=83)
+    decode(lens[:3000], 1, 8, 128, 32, BF16, seed=84)
+
+
+def test_selection_shared_by_a_cluster():
+    """Few rows of many pages: several CTAs score one row, for groups of one and of several head tiles."""
+    selection([16 * 4000 + 3, 16 * 700], 1, 33, 128, 16, 40, seed=85)
+    selection([16 * 3000], 2, 5, 64, 16, 9, first=0, last=3, window=16 * 2000 + 5, seed=86)
+
+
+@pytest.mark.parametrize("dtype", [BF16, INT8])
+def test_captured_calls_share_a_plan_and_follow_the_lengths(dtype):
+    """Two graphs over one plan, replayed in turn on one stream after the lengths changed, rows of the padded batch empty;
+    and one graph of another plan beside them on a second stream."""
+    g = gen(87)
+    heads, group, dim, page, S = 2, 4, 128, 64, 5
+    hq = heads * group
+    longest = [9000, 600, 64, 3000, 1]
+    table, n_pages = G.make_table(longest, page, g)
+    pool, scales = G.make_pool(n_pages, heads, page, dim, dtype, g)
+    layout = ct.GqaLayout(heads, dim, page, dtype, n_pages, table.shape[1])
+    plan, other = ct.GqaPlan(layout, S, hq), ct.GqaPlan(layout, S, hq)
+    q = torch.randn(3, S, hq, dim, generator=g, device="cuda").bfloat16()
+    lens = torch.tensor(longest, dtype=torch.int32, device="cuda")
+    out = torch.zeros(3, S, hq, dim, device="cuda").bfloat16()
+    lse = torch.zeros(3, S, hq, device="cuda")
+    side = torch.cuda.Stream()
+    graphs = []
+    for i, p in enumerate((plan, plan, other)):
+        torch.cuda.synchronize()
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            for _ in range(3):
+                p.decode(q[i], pool, scales, table, lens, out[i], lse[i], stream=torch.cuda.current_stream().cuda_stream)
+    for now in ([9000, 600, 64, 3000, 1], [0, 0, 0, 17, 0], [8999, 0, 0, 0, 0], [0] * 5, [5, 600, 1, 2999, 0]):
+        lens.copy_(torch.tensor(now, dtype=torch.int32))
+        out.fill_(7.0)
+        torch.cuda.synchronize()
+        for _ in range(4):
+            graphs[0].replay()
+            graphs[1].replay()
+            with torch.cuda.stream(side):
+                graphs[2].replay()
+        torch.cuda.synchronize()
+        for i in range(3):
+            G.check_attention(out[i], lse[i], G.attend(q[i], pool, scales, table, now, dtype, hq, MOD), dim, max(max(now), 1),
+                              dtype)
+
+
+def test_captured_write_bounds_and_read_follow_the_slots():
+    """One token a sequence as in a decode step, captured once; the padded rows' slots are outside the pool."""
+    g = gen(88)
+    heads, dim, page, n_pages, S = 3, 64, 32, 6, 4
+    layout = ct.GqaLayout(heads, dim, page, INT8, n_pages, 4)
+    pool = torch.zeros(n_pages, 2, heads, page, dim, dtype=torch.int8, device="cuda")
+    scales = torch.zeros(n_pages, 2, heads, page, device="cuda")
+    bounds = torch.zeros(n_pages, heads, 2, dim, dtype=torch.int8, device="cuda")
+    bs = torch.zeros(n_pages, heads, device="cuda")
+    x = torch.zeros(S, 2 * heads * dim, device="cuda").bfloat16()
+    back = torch.full((2, S, heads * dim), 5.0, device="cuda").bfloat16()
+    slots = torch.full((S,), -1, dtype=torch.int32, device="cuda")
+    pages, counts = (torch.full((S,), -1, dtype=torch.int32, device="cuda") for _ in range(2))
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        st = torch.cuda.current_stream().cuda_stream
+        ct.gqa_write_slots(layout, pool, scales, x, x[:, heads * dim:], slots, S, k_stride=2 * heads * dim,
+                           v_stride=2 * heads * dim, stream=st)
+        ct.gqa_page_bounds(layout, pool, scales, pages, counts, S, bounds, bs, stream=st)
+        ct.gqa_read_slots(layout, pool, scales, slots, S, back[0], back[1], stream=st)
+    kept = torch.zeros(2 * page, heads, dim)
+    for step in range(2 * page):                              # sequence 0 fills page 4, then page 1
+        x.copy_(torch.randn(x.shape, generator=g, device="cuda"))
+        page_now, at = (4, step) if step < page else (1, step - page)
+        slots.copy_(torch.tensor([page_now * page + at, -1, n_pages * page, -7], dtype=torch.int32))
+        pages.copy_(torch.tensor([page_now, -1, n_pages, -2], dtype=torch.int32))
+        counts.copy_(torch.tensor([at + 1, 3, 3, 3], dtype=torch.int32))
+        graph.replay()
+        torch.cuda.synchronize()
+        codes, sc = G.encode(x[0].float().cpu().numpy().reshape(2 * heads, dim), INT8)
+        want = np.asarray(codes, dtype=np.float32).reshape(2, heads, dim) * np.asarray(sc, dtype=np.float32).reshape(2, heads, 1)
+        kept[step] = torch.from_numpy(want[0])
+        assert torch.equal(back[:, 0].cpu(), torch.from_numpy(want).bfloat16().reshape(2, heads * dim))
+        assert (back[:, 1:] == 5.0).all()
+        for h in range(heads):
+            run = kept[step - at:step + 1, h].numpy()
+            want_codes, want_s = G.bounds_of(run)
+            assert np.array_equal(bounds[page_now, h].cpu().numpy(), want_codes) and bs[page_now, h].item() == want_s
