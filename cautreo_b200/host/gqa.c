@@ -158,11 +158,14 @@ ct_gqa_plan_t *ct_gqa_plan_create(const ct_gqa_shape_t *shape, uint32_t n_seq, i
         ct__set_error("ct_gqa_plan_create: bad shape");
         return NULL;
     }
-    /* the kernel counts the batch's steps of 16 tokens or more, and the steps
-     * of a sequence's items, in 32 bits (5: an item's overhead, rounding) */
+    /* the kernel counts the sequences' steps of 16 tokens or more, the steps
+     * of a sequence's items, the batch's items and a worker's part of all
+     * their steps in 32 bits (5: an item's overhead, rounding; 64: fewer
+     * workers than any B200 has) */
     const uint64_t most = (uint64_t)l.max_pages_per_seq * l.page_tokens / 16 + 5;
-    if ((uint64_t)n_seq * most > 0xFFFFFFFFu || most * shape->n_q_heads > 0xFFFFFFFFu ||
-        (uint64_t)n_seq * l.n_kv_heads > 0x7FFFFFFFu) {
+    const uint64_t items = (uint64_t)l.n_kv_heads * ((shape->n_q_heads / l.n_kv_heads + 15) / 16);     /* of a sequence */
+    if (n_seq * most > 0xFFFFFFFFu || most * shape->n_q_heads > 0xFFFFFFFFu || n_seq * items > 0x7FFFFFFFu ||
+        n_seq * most > (64ull << 31) / items) {
         ct__set_error("ct_gqa_plan_create: too many sequences for their longest length");
         return NULL;
     }

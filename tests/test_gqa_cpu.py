@@ -100,3 +100,13 @@ def test_tables_without_a_device(tmp_path):
     plain.save(tmp_path / "p.bin")
     with pytest.raises(RuntimeError):
         ct.GqaKV.load(tmp_path / "p.bin", device=-1)
+
+
+def test_plans_of_too_many_steps_refused():
+    """More steps in all than a worker's 32-bit share of them holds, although each sequence's and each head's are few enough."""
+    for n_seq, hq in ((1 << 18, 256), (3000, 65280)):
+        s = ct.GqaShape(ct.GqaLayout(256, 64, 16, BF16, 4, 1 << 13), hq, 0, 0, 0.0)
+        if hq > 256:
+            s.kv.max_pages_per_seq = 60000
+        assert not ct.lib().ct_gqa_plan_create(C.byref(s), n_seq, 0)
+        assert b"too many" in ct.lib().ct_hal_cuda_last_error()
