@@ -196,7 +196,7 @@ template <int TS> CT_DEV Seq sequence(const ct_gqa_args_t &a, uint32_t s) {
         r.n_list = have < a.n_pick ? have : a.n_pick;
         v = r.n_list * a.page_tokens;
     } else {
-        v = r.len - (r.start & ~15u);
+        v = r.len - (r.start & ~(TS - 1u));           /* whole steps: pages of a multiple of TS are not straddled */
     }
     const uint32_t st = (v + TS - 1) / TS;
     r.steps = st ? st : 1u;                                  /* an empty item still writes its zeros */
@@ -364,7 +364,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, DT, HT>::kMinB) k_gqa_decode(
             z.we = z.sb + n * (warp + 1) / kWarps;
         }
     };
-    auto first_token = [&](const Seq &q) -> uint32_t { return a.picked ? 0u : (q.start & ~15u); };
+    auto first_token = [&](const Seq &q) -> uint32_t { return a.picked ? 0u : (q.start & ~(TS - 1u)); };
     /* Logical page of the e-th page stepped over (0xFFFFFFFF: none). */
     auto entry = [&](const Segment &z, uint32_t e) -> uint32_t {
         if (!a.picked) return e;
