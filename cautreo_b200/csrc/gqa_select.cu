@@ -56,7 +56,7 @@ __global__ void __launch_bounds__(kThreads, D <= 128 ? 4 : 2) k_gqa_select(const
     constexpr int kPitch = 2 * D + 64;                       /* rows g, g + 1 in different halves of the banks */
     __shared__ __align__(16) int8_t s_q[16][kPitch];         /* (positive, negative) parts of 16 heads' codes */
     __shared__ float s_e[16];
-    __shared__ uint32_t s_bad, s_hist[256], s_scan[2][kWarps], s_thr, s_left, s_nz, s_all, s_any;
+    __shared__ uint32_t s_bad, s_hist[256], s_scan[2][kWarps], s_thr, s_left, s_most, s_nz, s_all, s_any;
     const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, j = lane & 3;
     const cg::cluster_group cluster = cg::this_cluster();
     const uint32_t ranks = cluster.num_blocks(), rank = cluster.block_rank();
@@ -78,7 +78,18 @@ __global__ void __launch_bounds__(kThreads, D <= 128 ? 4 : 2) k_gqa_select(const
     if (tid == 0) { s_bad = 0; s_nz = 0; s_all = 0xFFFFFFFFu; s_any = 0; }
     __syncthreads();
 
+    constexpr uint32_t kStep = kTiles * 8;
+    const uint32_t pb = (uint32_t)((uint64_t)have * rank / ranks), pe = (uint32_t)((uint64_t)have * (rank + 1) / ranks);
+    int32_t ph[kTiles];
+    auto numbers = [&](uint32_t p0) {                        /* of the pages that a warp takes from p0 on */
+        #pragma unroll
+        for (int t = 0; t < kTiles; t++) {
+            const uint32_t p = p0 + t * 8 + g;
+            ph[t] = p < pe ? __ldg(table + p) : -1;
+        }
+    };
     const uint32_t n_tiles = (a.group + 15) / 16;
+    if (choose) numbers(pb + warp * kStep);                  /* on their way while the queries are rounded */
     for (uint32_t tile = 0; choose && tile < n_tiles; tile++) {
         /* the tile's heads as whole numbers: two rows a warp */
         for (uint32_t r = warp; r < 16; r += kWarps) {
@@ -112,14 +123,7 @@ __global__ void __launch_bounds__(kThreads, D <= 128 ? 4 : 2) k_gqa_select(const
         __syncthreads();
         const uint32_t rows = a.group - tile * 16 < 16 ? a.group - tile * 16 : 16;
         const bool bad = s_bad != 0;
-        constexpr uint32_t kStep = kTiles * 8;
-        const uint32_t pb = (uint32_t)((uint64_t)have * rank / ranks), pe = (uint32_t)((uint64_t)have * (rank + 1) / ranks);
-        int32_t ph[kTiles];
-        #pragma unroll
-        for (int t = 0; t < kTiles; t++) {
-            const uint32_t p = pb + warp * kStep + t * 8 + g;
-            ph[t] = p < pe ? __ldg(table + p) : -1;
-        }
+        if (tile) numbers(pb + warp * kStep);
         for (uint32_t p0 = pb + warp * kStep; p0 < pe; p0 += kWarps * kStep) {
             uint4 w[kTiles][D / 32];
             float ps[kTiles];
@@ -133,11 +137,7 @@ __global__ void __launch_bounds__(kThreads, D <= 128 ? 4 : 2) k_gqa_select(const
                 for (int b = 0; b < D / 32; b++) w[t][b] = ok[t] ? __ldg(src + b * 4) : make_uint4(0u, 0u, 0u, 0u);
                 ps[t] = ok[t] ? __ldg(a.bound_scales + at) : 0.0f;
             }
-            #pragma unroll
-            for (int t = 0; t < kTiles; t++) {
-                const uint32_t p = p0 + kWarps * kStep + t * 8 + g;
-                ph[t] = p < pe ? __ldg(table + p) : -1;
-            }
+            numbers(p0 + kWarps * kStep);
             /* rows = pages p0 + g and p0 + 8 + g, columns = heads 2j, 2j + 1 of a
              * tile; lane j owns bytes 16 j .. 16 j + 15 of each 64 */
             float m[2] = {-INFINITY, -INFINITY};
@@ -228,16 +228,18 @@ __global__ void __launch_bounds__(kThreads, D <= 128 ? 4 : 2) k_gqa_select(const
                     __syncthreads();
                     s_hist[tid] = 0;
                     for (uint32_t w = 0; w < warp; w++) inc += s_scan[0][w];
-                    if (inc >= want && inc - cnt < want) { s_thr = 255 - tid; s_left = want - (inc - cnt); }
+                    if (inc >= want && inc - cnt < want) { s_thr = 255 - tid; s_left = want - (inc - cnt); s_most = cnt; }
                     __syncthreads();
                     known = 0xFFFFFFFFu << lo;
                     prefix = (prefix & ~(255u << lo)) | (s_thr << lo);
                     want = s_left;
-                    if (lo == 0) break;
+                    /* nothing to tell apart below this digit if all of its keys are chosen */
+                    if (lo == 0 || (want == s_most && (prefix & known))) break;
                     shift -= 8;
                 }
-                thr = prefix;
-                left = want;
+                const bool all_of = shift > 0;
+                thr = all_of ? (prefix & known) - 1 : prefix;
+                left = all_of ? 0u : want;
             }
         }
     }
