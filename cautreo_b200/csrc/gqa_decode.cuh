@@ -929,11 +929,12 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, DT, HT>::kMinB) k_gqa_decode(
                     }
                 }
                 __syncthreads();
-                /* Loads in flight: 8 of a thread; 16 in the form that has the
-                 * registers, of four columns where a thread has as many
-                 * (selected pages, 16 heads of 256 in three parts: 43.9 ->
-                 * 42.7 us; one sequence of 8000 tokens 13.8 -> 13.2). */
-                constexpr int kCols = FEW && HT * D >= 512 ? 4 : 1, kParts = FEW ? 16 / kCols : 8;
+                /* Loads in flight: 8 of a thread, 16 in the form that has the
+                 * registers (one sequence of 8000 tokens 13.8 -> 13.2 us),
+                 * spread over the columns that a thread has with 9 to 16 heads
+                 * (one sequence of 500 tokens, 4 kv heads of 16 query heads,
+                 * 128 values: 12.2 -> 11.6). */
+                constexpr int kCols = HT == 1 ? 1 : D >= 96 ? 4 : 2, kParts = (FEW ? 16 : 8) / kCols;
                 const uint32_t cols = rows * (D / 4);
                 #pragma unroll 1
                 for (uint32_t c0 = tid; c0 < cols; c0 += kCols * kThreads) {
