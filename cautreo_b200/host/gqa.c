@@ -21,7 +21,7 @@ struct ct_gqa_plan {
     ct_gqa_shape_t shape;
     uint32_t n_seq, n_workers, n_sms;
     int device;
-    float *part_o, *part_ml;
+    float *part_o, *part_ml;     /* one allocation: partial results, their (max, sum), counters */
     uint32_t *counters;
     size_t scratch_bytes;
 };
@@ -143,7 +143,7 @@ static void leave(int device, int prev) {
 
 void ct_gqa_plan_destroy(ct_gqa_plan_t *p) {
     if (!p) return;
-    cudaFree(p->part_o); cudaFree(p->part_ml); cudaFree(p->counters);
+    cudaFree(p->part_o);
     free(p);
 }
 
@@ -187,11 +187,17 @@ ct_gqa_plan_t *ct_gqa_plan_create(const ct_gqa_shape_t *shape, uint32_t n_seq, i
         p->n_workers = (uint32_t)(n_sms * ctas);
         const size_t po = (size_t)2 * p->n_workers * 16 * l.head_dim * sizeof(float);
         const size_t pm = (size_t)2 * p->n_workers * 32 * sizeof(float), pc = (size_t)3 * p->n_workers * sizeof(uint32_t);
-        rc = ct__cuda_status(cudaMalloc((void **)&p->part_o, po), "gqa scratch");
-        if (!rc) rc = ct__cuda_status(cudaMalloc((void **)&p->part_ml, pm), "gqa scratch");
-        if (!rc) rc = ct__cuda_status(cudaMalloc((void **)&p->counters, pc), "gqa scratch");
-        if (!rc) rc = ct__cuda_status(cudaMemset(p->counters, 0, pc), "gqa scratch");
-        if (!rc) rc = ct__cuda_status(cudaStreamSynchronize(0), "gqa scratch");    /* streams of any kind may come next */
+        /* zeroed on a stream of its own: the caller's may be busy, and of any kind */
+        cudaStream_t st = NULL;
+        rc = ct__cuda_status(cudaMalloc((void **)&p->part_o, po + pm + pc), "gqa scratch");
+        if (!rc) rc = ct__cuda_status(cudaStreamCreateWithFlags(&st, cudaStreamNonBlocking), "gqa scratch");
+        if (!rc) {
+            p->part_ml = p->part_o + po / sizeof(float);
+            p->counters = (uint32_t *)(p->part_ml + pm / sizeof(float));
+            rc = ct__cuda_status(cudaMemsetAsync(p->counters, 0, pc, st), "gqa scratch");
+            if (!rc) rc = ct__cuda_status(cudaStreamSynchronize(st), "gqa scratch");
+            cudaStreamDestroy(st);
+        }
         p->scratch_bytes = po + pm + pc;
     }
     leave(device, prev);
