@@ -52,30 +52,36 @@ constexpr float kLn2 = 0.6931471805599453f;
 constexpr float kGrow = 3.0f;           /* log2 growth of a maximum that is followed */
 constexpr float kNoMax = -3.402823466e38f;  /* maximum of no tokens: finite, so that no difference of maxima is NaN */
 constexpr uint32_t kItemCost = 4;       /* steps that an item's start and end are counted as */
-constexpr uint32_t kSoloMost = 16; /* longest item of one warp: longer ones would leave the others idle at the end */
+constexpr uint32_t kWhole = 32;         /* longest item, start and end counted, that is never cut between CTAs: 64
+                                         * sequences of 300 tokens, 8 kv heads, bf16 x 128 24.8 -> 20.3 us */
+constexpr uint32_t kSoloMost = 16;      /* longest item of one warp: longer ones would leave the others idle at the end */
 constexpr uint32_t kSoloCost = 3;       /* start and end of an item, in steps of one warp, */
 constexpr uint32_t kShareCost = 10;     /* and of one that the warps share */
 constexpr uint32_t kFan = 16;           /* workers whose parts are joined at a time, when an item has more than 2 kFan */
 
 /* Tokens of a warp's step (2 to 17 KB of K and V), steps in its ring, and the
- * CTAs that an SM shall hold.  What bounds a long batch is how evenly the SMs
- * share the memory, and that gets worse with the copies in flight: from 100
- * to 140 KB an SM hides the latency, more lets the SMs nearest to the memory
- * take more than their part.  So rings have two steps, and CTAs that would
- * bring more than kInFlight are kept out (32 sequences of 4096 tokens, 8 kv
- * heads: int8 x 128 170 -> 110 KB 58.0 -> 54.0 us, bf16 x 192 143 -> 135,
- * bf16 x 256 186 -> 181, and bf16 x 128 208 -> 140 KB 16 sequences 52.0 ->
- * 51.0).  Rows of 64 bytes or fewer are bound by their instructions and gain
- * from a third step (8-bit x 64, 16 x 4096 tokens 24.7 -> 22.2 us).  A third
- * CTA is worth the registers' limit of 168 where it spills nothing: int8 x
- * 128, 256 sequences of 256 tokens 53 -> 47 us. */
-constexpr int kInFlight = 142 * 1024;
+ * CTAs that an SM shall hold.
+ * Rows of up to 128 bytes take 32 tokens: the instructions that a step costs
+ * whatever its size count half, and a long batch, which runs at the power
+ * limit, keeps a higher clock (int8 x 128, 256 sequences of 256 tokens 39.5
+ * -> 34.6 us, 64 of 16384 ragged, for a second, 217 -> 209; pages of 16, two
+ * a step, 77 -> 79).
+ * What bounds a long batch is how evenly the SMs share the memory, and that
+ * gets worse with the copies in flight: from 100 to 150 KB an SM hides the
+ * latency, more lets the SMs nearest to the memory take more than their part.
+ * So rings have two steps, and CTAs that would bring more than kInFlight are
+ * kept out (32 sequences of 4096 tokens, 8 kv heads, bf16: x 192 143 -> 135
+ * us, x 256 186 -> 181; x 128 208 -> 140 KB, 16 sequences 52.0 -> 51.0).
+ * Rows of 64 bytes or fewer are bound by their instructions and gain from a
+ * third step (8-bit x 64, 16 x 4096 tokens 24.7 -> 22.2 us) and a third CTA,
+ * which limits them to 168 registers. */
+constexpr int kInFlight = 156 * 1024;
 template <int D, int DT, int HT> struct Cfg {
     static constexpr int kElt = DT == CT_KV_BF16 ? 2 : 1;
     static constexpr int kRow = D * kElt;
-    static constexpr int TS = kRow <= 64 ? 32 : 16;
+    static constexpr int TS = kRow <= 128 ? 32 : 16;
     static constexpr int kStages = kRow <= 64 ? 3 : 2;
-    static constexpr int kMinB = HT == 1 && D <= 128 && (kElt == 1 || D <= 64) ? 3 : 1;
+    static constexpr int kMinB = HT > 1 || kRow > 128 ? 1 : kRow <= 64 ? 3 : 2;
     static constexpr int kPitch = kRow + 16;                  /* odd number of 16-B units: conflict-free ldmatrix */
     static constexpr int kScaleBytes = DT == CT_KV_BF16 ? 0 : TS * 8;
     static constexpr int kStage = 2 * TS * kPitch + kScaleBytes;
@@ -213,6 +219,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, DT, HT>::kMinB) k_gqa_decode(
     constexpr int TS = C::TS, GR = TS / 16, kPitch = C::kPitch, KB = D / 16, S = C::kStages;
     constexpr int kHeads = 8 * HT;
     constexpr bool kQ8 = DT != CT_KV_BF16;
+    constexpr uint32_t kLeast = 128 / TS;                    /* least steps of a part: one a warp or two */
     /* a segment's end: each warp leaves its [head][value] sums in the ring slot
      * that it consumed last, all values at once or half of them at a time */
     constexpr int kJoinCols = kHeads * (D + 4) * 4 <= C::kStage ? D : D / 2;
@@ -240,11 +247,23 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, DT, HT>::kMinB) k_gqa_decode(
         #pragma unroll 1
         for (uint32_t s = lane; s < a.n_seq; s += 32) sum += sequence<TS>(a, s).steps;
         sum = __reduce_add_sync(0xFFFFFFFFu, sum);
+        /* Parts of an item: as many as there are CTAs for, but with 9 to 16
+         * heads, whose sums are long to join, few where a part would be short:
+         * none of up to 256 tokens, else about as many as make a part's steps
+         * and the join take equal time (4 kv heads of 16 query heads, bf16 x
+         * 256: 4000 tokens 30.4 -> 24.0 us; 30 sequences of 239 tokens, 1 kv
+         * head, 14.4 -> 11.9). */
         const uint32_t spare = gridDim.x - a.n_seq * HV;     /* every item's last part may be a short one */
-        const uint32_t Q = max(a.min_steps, (uint32_t)__umul64hi((uint64_t)sum * HV + spare - 1, a.spare_magic));
+        const uint32_t Q = max(kLeast, (uint32_t)__umul64hi((uint64_t)sum * HV + spare - 1, a.spare_magic));
         #pragma unroll 1
         for (uint32_t s0 = 0; s0 < a.n_seq; s0 += 32) {
-            const uint32_t s = s0 + lane, steps = s < a.n_seq ? sequence<TS>(a, s).steps : 0u, n = min((steps + Q - 1) / Q, a.most_parts);
+            const uint32_t s = s0 + lane, steps = s < a.n_seq ? sequence<TS>(a, s).steps : 0u;
+            uint32_t n = min((steps + Q - 1) / Q, a.most_parts);
+            if (HT == 2) {
+                n = min(n, max(2 * kFan, steps / 8));        /* more are joined in two rounds */
+                if (steps <= kLeast * HT) n = min(steps, 1u);
+                else if (n <= 2 * kFan) n = min(n, max(1u, (uint32_t)sqrtf((float)steps * (19.0f * TS / (HT * D)))));
+            }
             uint32_t incl = n * HV;                          /* parts of the sequence's items */
             #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
@@ -283,7 +302,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, DT, HT>::kMinB) k_gqa_decode(
             all += s_scan[w];
         }
         const uint64_t total = (uint64_t)all * HV, excl = (uint64_t)(before + incl - sum) * HV, next = excl + (uint64_t)sum * HV;
-        const uint32_t Q = max(a.min_steps, (uint32_t)__umul64hi(total + gridDim.x - 1, a.worker_magic));
+        const uint32_t Q = max(kLeast, (uint32_t)__umul64hi(total + gridDim.x - 1, a.worker_magic));
         const uint64_t x0 = (uint64_t)blockIdx.x * Q;
         if (x0 >= total) return;
         if (tid == 0 && x0 + Q >= total) s_end[1] = end_at(a.n_seq, 0u, 0u, 0u, 0u);
@@ -301,10 +320,9 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, DT, HT>::kMinB) k_gqa_decode(
             }
             const uint32_t rel = (uint32_t)(x - at), item = rel / width;          /* below 2^32: see the plan */
             uint32_t in = rel - item * width;
-            /* An item that is short against the CTA's share goes to the later
-             * CTA as a whole: cutting it costs both of them a shared start and
-             * end, and the join. */
-            if (width <= max(12u, min(Q / 4, 40u))) in = 0;
+            /* A short item goes to the later CTA as a whole: cutting it costs
+             * both of them a shared start and end, and the join. */
+            if (width <= kWhole) in = 0;
             const uint32_t step = in > kItemCost ? in - kItemCost : 0u;
             /* workers that hold steps of the item: from the one of its first
              * step (this one if the item begins here) to that of its last */
@@ -378,30 +396,32 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, DT, HT>::kMinB) k_gqa_decode(
 
     /* ---- copies: S - 1 steps ahead of the arithmetic ----
      * Cursor of the next tokens to copy: their address, the slot in their page
-     * and the page's slots [page_lo, page_hi) that the mask keeps; and the
-     * following pages, whose numbers are loaded a page (list entries: two
-     * pages) before they are needed. */
+     * and the page's slots [page_lo, page_hi) that the mask keeps.  Page
+     * numbers are loaded 32 at a time, one a lane, 16 pages ahead. */
     Segment z = {}, pz = {};
     if (FEW) { segment(z, 0); pz = z; }
-    uint32_t p_at = 0xFFFFFFFFu, left = 0, page_e = 0, off = 0, page_lo = 0, page_hi = 0, lp_next = 0, ph_next = 0, lp_then = 0;
+    uint32_t p_at = 0xFFFFFFFFu, left = 0, page_e = 0, off = 0, page_lo = 0, page_hi = 0;
+    uint32_t turned = 0, lps = 0, phs = 0, lps_then = 0, phs_then = 0;       /* pages opened; logical, physical numbers */
     const uint8_t *kp = nullptr;
     const float *sp = nullptr;
     bool turn = false, done = false;
     uint32_t whole_slots = 0, fill = 0;                      /* bit per ring slot; slot of the next copies */
     const size_t page_bytes = 2 * v_off, page_rows = (size_t)2 * a.n_kv_heads * a.page_tokens;
-    auto turn_page = [&]() {                                 /* opens the page at hand, looks up the one after */
-        const bool ok = ph_next < a.n_pages;
+    auto turn_page = [&]() {                                 /* opens the next page */
+        const uint32_t i = turned & 31;
+        if (i == 0 && turned) { lps = lps_then; phs = phs_then; }
+        if (i == 16) { lps_then = entry(pz, page_e + 16 + lane); phs_then = mapped(pz, lps_then); }
+        const uint32_t lp = __shfl_sync(0xFFFFFFFFu, lps, i), ph = __shfl_sync(0xFFFFFFFFu, phs, i);
+        const bool ok = ph < a.n_pages;
         const uint32_t row = pz.head * a.page_tokens + off;  /* of the page */
-        kp = static_cast<const uint8_t *>(a.pool) + (ok ? ph_next : 0u) * page_bytes + (size_t)row * C::kRow + lane * 16;
+        kp = static_cast<const uint8_t *>(a.pool) + (ok ? ph : 0u) * page_bytes + (size_t)row * C::kRow + lane * 16;
         if (kQ8)
-            sp = a.scales + (ok ? ph_next : 0u) * page_rows + row + (lane >> 2) * (a.n_kv_heads * a.page_tokens) + (lane & 3) * 4;
-        const uint32_t first = lp_next * a.page_tokens;
+            sp = a.scales + (ok ? ph : 0u) * page_rows + row + (lane >> 2) * (a.n_kv_heads * a.page_tokens) + (lane & 3) * 4;
+        const uint32_t first = lp * a.page_tokens;
         page_lo = pz.sq.start > first ? pz.sq.start - first : 0u;
         page_hi = ok ? min(pz.sq.len - first, a.page_tokens) : 0u;
-        lp_next = lp_then;
-        ph_next = mapped(pz, lp_next);
-        lp_then = entry(pz, page_e + 2);
         page_e++;
+        turned++;
         turn = false;
     };
     /* Starts the copies of this warp's next step (tokens that the mask drops
@@ -438,17 +458,29 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, DT, HT>::kMinB) k_gqa_decode(
                     if (turn || off == a.page_tokens) { if (!turn) off = 0; turn_page(); }
                     const uint32_t lo = page_lo > off ? page_lo - off : 0u;      /* tokens [lo, hi) are kept */
                     const uint32_t hi = page_hi > off ? min(page_hi - off, 16u) : 0u;
-                    whole = whole && lo == 0 && hi == 16;
-                    #pragma unroll 1
-                    for (uint32_t c = lane; c < (uint32_t)N; c += 32) {
-                        const uint32_t row = c / CPR, d = to + (gr * 16 + row) * kPitch + (c % CPR) * 16;
-                        const uint32_t bytes = row >= lo && row < hi ? 16u : 0u;
-                        cp_async16_part(d, kp + (c - lane) * 16, bytes);
-                        cp_async16_part(d + TS * kPitch, kp + v_off + (c - lane) * 16, bytes);
-                    }
-                    if (kQ8 && lane < 8) {
-                        const uint32_t tk = (lane & 3) * 4;
-                        cp_async16_part(to_s + gr * 64, sp, (hi > tk ? min(hi - tk, 4u) : 0u) * 4);
+                    if (lo == 0 && hi == 16) {
+                        #pragma unroll
+                        for (int c0 = 0; c0 < N; c0 += 32) {
+                            const uint32_t c = c0 + lane;
+                            if (N % 32 != 0 && c >= (uint32_t)N) continue;
+                            const uint32_t d = to + (gr * 16 + c / CPR) * kPitch + (c % CPR) * 16;
+                            cp_async16(d, kp + c0 * 16);
+                            cp_async16(d + TS * kPitch, kp + v_off + c0 * 16);
+                        }
+                        if (kQ8 && lane < 8) cp_async16(to_s + gr * 64, sp);
+                    } else {
+                        whole = false;
+                        #pragma unroll 1
+                        for (uint32_t c = lane; c < (uint32_t)N; c += 32) {
+                            const uint32_t row = c / CPR, d = to + (gr * 16 + row) * kPitch + (c % CPR) * 16;
+                            const uint32_t bytes = row >= lo && row < hi ? 16u : 0u;
+                            cp_async16_part(d, kp + (c - lane) * 16, bytes);
+                            cp_async16_part(d + TS * kPitch, kp + v_off + (c - lane) * 16, bytes);
+                        }
+                        if (kQ8 && lane < 8) {
+                            const uint32_t tk = (lane & 3) * 4;
+                            cp_async16_part(to_s + gr * 64, sp, (hi > tk ? min(hi - tk, 4u) : 0u) * 4);
+                        }
                     }
                     off += 16;
                     kp += 16 * C::kRow;
@@ -472,9 +504,9 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, DT, HT>::kMinB) k_gqa_decode(
                 const uint32_t v = first_token(pz.sq) + pz.wb * TS;
                 page_e = a.page_of(v);
                 off = v - page_e * a.page_tokens;
-                lp_next = entry(pz, page_e);
-                lp_then = entry(pz, page_e + 1);
-                ph_next = mapped(pz, lp_next);
+                lps = entry(pz, page_e + lane);
+                phs = mapped(pz, lps);
+                turned = 0;
                 turn = true;
             }
         }

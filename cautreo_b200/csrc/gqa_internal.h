@@ -33,7 +33,6 @@ typedef struct {
     uint64_t q_stride;
     uint32_t n_seq, n_q_heads, n_kv_heads, group, n_tiles;   /* group = query heads a kv head, tiles of 16 of them */
     uint32_t page_tokens, max_pages, n_pages, n_pick, window, blocked;
-    uint32_t min_steps;          /* least steps a worker takes */
     uint32_t most_parts;         /* parts of an item, when every worker takes one part */
     float scale_log2;            /* scale x log2(e) */
     uint64_t worker_magic;       /* floor(2^64 / n_workers) + 1: division of less than 2^64 / n_workers */

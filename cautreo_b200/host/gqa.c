@@ -232,7 +232,7 @@ static int decode(ct_gqa_plan_t *p, const void *q, uint64_t q_stride, const void
         .counters = p->counters, .q_stride = q_stride, .n_seq = p->n_seq, .n_q_heads = p->shape.n_q_heads,
         .n_kv_heads = l->n_kv_heads, .group = group, .n_tiles = (group + 15) / 16, .page_tokens = l->page_tokens,
         .max_pages = l->max_pages_per_seq, .n_pages = l->n_pages, .n_pick = n_select, .window = p->shape.window_tokens,
-        .blocked = p->shape.head_order == CT_GQA_BLOCKED, .min_steps = 8,
+        .blocked = p->shape.head_order == CT_GQA_BLOCKED,
         /* up to 32 parts are joined at once: somewhat fewer workers than there
          * are beat a second round of joins (one sequence of 8000 tokens,
          * 8 heads: 32 parts of 13.6 us, 37 of 14.7) */
