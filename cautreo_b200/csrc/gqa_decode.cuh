@@ -18,6 +18,10 @@
  * 9 to 16 take two column tiles over the same K and V fragments, more run as
  * further items.  Scores come out as [token][head] and are needed as
  * [token][head] operands: two movmatrix per 16 tokens.
+ * Measured, 8 kv heads of 4 query heads, 128 values: 32 sequences of 4096
+ * tokens, bf16 94 us (5.7 TB/s), int8 54 us (5.1 TB/s); 64 of 8192 bf16 341 us
+ * (6.3 TB/s); one of 777 tokens 8.2 us, most of it the launch, the dependent
+ * loads up to the first tokens and the join.
  *
  * bf16 pools: probabilities enter as two bf16 digits (one would add an error
  * as large as the rounding of the output).  8-bit pools: codes are widened to

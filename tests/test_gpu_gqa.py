@@ -781,3 +781,37 @@ def test_captured_write_bounds_and_read_follow_the_slots():
             run = kept[step - at:step + 1, h].numpy()
             want_codes, want_s = G.bounds_of(run)
             assert np.array_equal(bounds[page_now, h].cpu().numpy(), want_codes) and bs[page_now, h].item() == want_s
+
+
+@pytest.mark.parametrize("dtype,dim", [(BF16, 128), (INT8, 128), (E4M3, 64)])
+def test_decode_warps_that_pass_many_pages(dtype, dim):
+    """Small pages and enough items that each warp's run of tokens goes over more than 64 of them, holes among them."""
+    lens = [2900 + 13 * i for i in range(48)]
+    holes = {(s, p) for s in range(0, 48, 5) for p in range(20, 80, 7)}
+    decode(lens, 8, 1, dim, 16, dtype, holes=holes, seed=89)
+
+
+@pytest.mark.parametrize("dtype,window", [(BF16, 0), (INT8, 3999)])
+def test_decode_many_selected_pages(dtype, window):
+    """Long lists of small pages: more entries than a warp loads at a time, sequences shorter than their list among them."""
+    g = gen(90)
+    heads, group, dim, page, pick, S = 4, 4, 128, 16, 220, 40
+    lens = [5000 + 3 * i for i in range(S - 2)] + [700, 0]
+    table, n_pages = G.make_table(lens, page, g, window)
+    pool, scales = G.make_pool(n_pages, heads, page, dim, dtype, g)
+    q = torch.randn(S, heads * group, dim, generator=g, device="cuda").bfloat16()
+    pages = np.full((S, heads, pick), -1, np.int32)
+    rng = np.random.default_rng(5)
+    for s, n in enumerate(lens):
+        first, last = (max(0, n - window) // page if window else 0), -(-n // page)
+        for h in range(heads):
+            k = min(pick, last - first)
+            pages[s, h, :k] = np.sort(rng.permutation(np.arange(first, last))[:k])
+    plan = ct.GqaPlan(ct.GqaLayout(heads, dim, page, dtype, n_pages, table.shape[1]), S, heads * group, window_tokens=window)
+    out = torch.empty(S, heads * group, dim, device="cuda").bfloat16()
+    lse = torch.empty(S, heads * group, device="cuda")
+    plan.decode_selected(q, pool, scales, table, torch.tensor(lens, dtype=torch.int32, device="cuda"),
+                         torch.from_numpy(pages).cuda(), pick, out, lse, stream=stream())
+    torch.cuda.synchronize()
+    G.check_attention(out, lse, G.attend(q, pool, scales, table, lens, dtype, heads * group, MOD, window, pages=pages), dim,
+                      max(lens), dtype)
