@@ -34,18 +34,32 @@ CT_DEV uint32_t pack2_bf16(float lo, float hi) {
 /* Both directions: blockIdx.y is the row's place in a token (K heads, then V
  * heads), blockIdx.x a run of tokens, so a block reads or writes a head's
  * consecutive slots as one contiguous run.  A thread moves 8 values of T
- * tokens; all its loads are in flight before the first is used.  Bound by HBM
- * in large calls (16384 tokens, 8 heads of 128, bf16 <-> int8: written in
- * 20.1 us, 5.0 TB/s of bytes read and written, read back in 19.4), by the
- * launch in small ones (64 tokens with their pages' bounds 4.5 us). */
+ * tokens; all its loads are in flight before the first is used, and the lanes
+ * of a row find the tokens' rows once between them.  Bound by HBM in large
+ * calls (16384 tokens, 8 heads of 128, bf16 -> int8 18.5 us, 5.5 TB/s of bytes
+ * read and written; read back at once, the pool still in L2, 12), by the
+ * launch in small ones (64 tokens with their pages' bounds 4.5 to 5 us). */
 
-/* Row of the pool for a token's slot, or none. */
-CT_DEV bool pool_row(int32_t slot, uint32_t place, uint32_t n_kv_heads, uint32_t page_tokens, uint32_t page_magic, uint32_t n_pages,
-                     size_t &row) {
+/* Row of the pool for a token's slot, or kNoRow. */
+constexpr size_t kNoRow = ~(size_t)0;
+CT_DEV size_t pool_row(int32_t slot, uint32_t place, uint32_t n_kv_heads, uint32_t page_tokens, uint32_t page_magic, uint32_t n_pages) {
     const uint32_t page = ct_gqa_page_of((uint32_t)slot, page_magic);
-    if (slot < 0 || page >= n_pages) return false;
-    row = ((size_t)page * 2 * n_kv_heads + place) * page_tokens + ((uint32_t)slot - page * page_tokens);
-    return true;
+    if (slot < 0 || page >= n_pages) return kNoRow;
+    return ((size_t)page * 2 * n_kv_heads + place) * page_tokens + ((uint32_t)slot - page * page_tokens);
+}
+CT_DEV size_t shfl_row(size_t row, uint32_t from) {
+    return ((size_t)__shfl_sync(0xFFFFFFFFu, (uint32_t)(row >> 32), from) << 32) | __shfl_sync(0xFFFFFFFFu, (uint32_t)row, from);
+}
+
+/* floor(x id + 1/2) of two values in the low bytes of lo and hi: by a
+ * round-down addition into the bits of 1.5 x 2^23; two values an instruction,
+ * since the 8-bit write issues as many as it can. */
+CT_DEV void floor2(float x0, float x1, float id, uint32_t &lo, uint32_t &hi) {
+    asm("{ .reg .b64 x, i, h, m;\n\t"
+        "mov.b64 x, {%2, %3};\n\tmov.b64 i, {%4, %4};\n\tmov.b64 h, {%5, %5};\n\tmov.b64 m, {%6, %6};\n\t"
+        "mul.rn.f32x2 x, x, i;\n\tadd.rn.f32x2 x, x, h;\n\tadd.rm.f32x2 x, x, m;\n\t"
+        "mov.b64 {%0, %1}, x; }"
+        : "=r"(lo), "=r"(hi) : "f"(x0), "f"(x1), "f"(id), "f"(0.5f), "f"(12582912.0f));
 }
 
 template <int D, int DT, bool F32, int T>
@@ -60,11 +74,12 @@ __global__ void __launch_bounds__(kThreads) k_gqa_write(void *pool, float *scale
     const size_t col = (size_t)(is_v ? place - n_kv_heads : place) * D + u * 8, stride = is_v ? v_stride : k_stride;
     const void *from = is_v ? vs : ks;
     uint4 w[T][F32 ? 2 : 1];
-    int32_t slot[T];
+    /* lane u finds the row of token u & (T - 1) for the lanes that share it */
+    const uint32_t own = t0 + (u & (T - 1)) * R;
+    const int32_t slot = own < n ? __ldg(slots + own) : -1;
     #pragma unroll
     for (int i = 0; i < T; i++) {
         const uint32_t t = t0 + i * R;
-        slot[i] = t < n ? __ldg(slots + t) : -1;
         if (t >= n || u >= U) continue;
         const size_t at = (size_t)t * stride + col;
         const uint4 *p = F32 ? reinterpret_cast<const uint4 *>(static_cast<const float *>(from) + at)
@@ -72,6 +87,7 @@ __global__ void __launch_bounds__(kThreads) k_gqa_write(void *pool, float *scale
         w[i][0] = __ldcs(p);
         if (F32) w[i][F32 ? 1 : 0] = __ldcs(p + 1);
     }
+    const size_t mine = pool_row(slot, place, n_kv_heads, page_tokens, page_magic, n_pages);
     /* The four tokens' maxima are reduced together: after two exchanges a lane
      * keeps that of token u & 3, so the divisions run once, not four times. */
     uint32_t top[T];                                         /* bits of max|x|: NaN above Inf above every finite value */
@@ -109,8 +125,8 @@ __global__ void __launch_bounds__(kThreads) k_gqa_write(void *pool, float *scale
     for (int i = 0; i < T; i++) {
         const uint32_t from = (threadIdx.x & (32 - L)) | (i & (L - 1));
         const float di = T == 1 ? d : __shfl_sync(0xFFFFFFFFu, d, from), idi = T == 1 ? id : __shfl_sync(0xFFFFFFFFu, id, from);
-        size_t row = 0;
-        if (!pool_row(slot[i], place, n_kv_heads, page_tokens, page_magic, n_pages, row) || u >= U) continue;
+        const size_t row = T == 1 ? mine : shfl_row(mine, from);
+        if (row == kNoRow || u >= U) continue;
         if (DT == CT_KV_BF16 && !F32) {
             *reinterpret_cast<uint4 *>(static_cast<uint16_t *>(pool) + row * D + u * 8) = w[i][0];
             continue;
@@ -131,12 +147,10 @@ __global__ void __launch_bounds__(kThreads) k_gqa_write(void *pool, float *scale
             #pragma unroll
             for (int k = 0; k < 2; k++) {
                 if (DT == CT_KV_INT8) {
-                    /* floor by a round-down addition into the bits of 1.5 x 2^23;
-                     * |x id| <= 127 (1 + 2^-21), so no code passes +-127 */
+                    /* |x id| <= 127 (1 + 2^-21), so no code passes +-127 */
                     uint32_t q[4];
-                    #pragma unroll
-                    for (int e = 0; e < 4; e++)
-                        q[e] = __float_as_uint(__fadd_rd(__fadd_rn(__fmul_rn(x[4 * k + e], idi), 0.5f), 12582912.0f));
+                    floor2(x[4 * k], x[4 * k + 1], idi, q[0], q[1]);
+                    floor2(x[4 * k + 2], x[4 * k + 3], idi, q[2], q[3]);
                     c[k] = __byte_perm(__byte_perm(q[0], q[1], 0x0040), __byte_perm(q[2], q[3], 0x0040), 0x5410);
                 } else {
                     c[k] = (uint32_t)ct_e4m3x2_code(x[4 * k], x[4 * k + 1], idi) |
@@ -183,21 +197,19 @@ __global__ void __launch_bounds__(kThreads) k_gqa_read(const void *pool, const f
     constexpr int L = lanes_of(D), U = D / 8, R = kThreads / L;
     const uint32_t u = threadIdx.x % L, place = blockIdx.y;
     ct_gqa_enter();
-    if (u >= U) return;
     const bool is_v = place >= n_kv_heads;
     const uint32_t t0 = blockIdx.x * (R * T) + threadIdx.x / L;
     const size_t col = (size_t)(is_v ? place - n_kv_heads : place) * D + u * 8, stride = is_v ? v_stride : k_stride;
     void *to = is_v ? vo : ko;
-    int32_t slot[T];
     uint4 w[T];
     float sc[T];
     bool ok[T];
-    #pragma unroll
-    for (int i = 0; i < T; i++) slot[i] = t0 + i * R < n ? __ldg(slots + t0 + i * R) : -1;
+    const uint32_t own = t0 + (u & (T - 1)) * R;             /* as in the write */
+    const size_t mine = pool_row(own < n ? __ldg(slots + own) : -1, place, n_kv_heads, page_tokens, page_magic, n_pages);
     #pragma unroll
     for (int i = 0; i < T; i++) {
-        size_t row = 0;
-        ok[i] = pool_row(slot[i], place, n_kv_heads, page_tokens, page_magic, n_pages, row);
+        const size_t row = T == 1 ? mine : shfl_row(mine, (threadIdx.x & (32 - L)) | (i & (L - 1)));
+        ok[i] = row != kNoRow && u < U;
         sc[i] = 1.0f;
         if (!ok[i]) continue;
         w[i] = load8<D, DT>(pool, row, u);
