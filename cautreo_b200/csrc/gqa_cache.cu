@@ -14,6 +14,8 @@
 #include <float.h>
 #include <math.h>
 
+#include <type_traits>
+
 #include "../../include/hal.h"
 #include "../../include/kv_cache.h"
 #include "ct_internal.h"
@@ -244,26 +246,39 @@ template <int DT> struct Range8 {
         #pragma unroll
         for (int e = 0; e < 8; e++) { hi[e] = -INFINITY; lo[e] = INFINITY; }
     }
-    CT_DEV void take(const uint4 &w, float sc) {
-        bad = bad || !(fabsf(sc) < INFINITY);
+    /* Two rows: 8-bit values in fp32, products and sums two an instruction,
+     * extremes of three. */
+    CT_DEV static void row(const uint4 &w, float sc, uint64_t *x) {
         const uint32_t ws[2] = {w.x, w.y};
-        if (DT == CT_KV_E4M3)                                /* a byte of seven ones is NaN (this cache stores none) */
-            bad = bad || ((((w.x & 0x7F7F7F7Fu) + 0x01010101u) | ((w.y & 0x7F7F7F7Fu) + 0x01010101u)) & 0x80808080u) != 0;
         #pragma unroll
-        for (int i = 0; i < 8; i += 2) {
+        for (int i = 0; i < 4; i++) {
             float2 f;
             if (DT == CT_KV_INT8) {                          /* byte + 128 under the exponent of 2^23, minus 2^23 + 128 */
-                const uint32_t b = ws[i >> 2] ^ 0x80808080u;
-                f.x = __uint_as_float(__byte_perm(b, 0x4B000000u, 0x7540 | (i & 3))) - 8388736.0f;
-                f.y = __uint_as_float(__byte_perm(b, 0x4B000000u, 0x7540 | ((i & 3) + 1))) - 8388736.0f;
+                const uint32_t b = ws[i >> 1] ^ 0x80808080u;
+                f.x = __uint_as_float(__byte_perm(b, 0x4B000000u, 0x7540 | (2 * i & 3)));
+                f.y = __uint_as_float(__byte_perm(b, 0x4B000000u, 0x7540 | ((2 * i & 3) + 1)));
+                asm("{ .reg .b64 m; mov.b64 m, {%3, %3}; mov.b64 %0, {%1, %2}; add.rn.f32x2 %0, %0, m; }"
+                    : "=l"(x[i]) : "f"(f.x), "f"(f.y), "f"(-8388736.0f));
             } else {
-                f = ct_e4m3x2_to_f32x2((uint16_t)(ws[i >> 2] >> (8 * (i & 3))));
+                f = ct_e4m3x2_to_f32x2((uint16_t)(ws[i >> 1] >> (16 * (i & 1))));
+                asm("mov.b64 %0, {%1, %2};" : "=l"(x[i]) : "f"(f.x), "f"(f.y));
             }
-            f.x = __fmul_rn(f.x, sc);
-            f.y = __fmul_rn(f.y, sc);
-            hi[i] = fmaxf(hi[i], f.x); lo[i] = fminf(lo[i], f.x);
-            hi[i + 1] = fmaxf(hi[i + 1], f.y); lo[i + 1] = fminf(lo[i + 1], f.y);
+            asm("{ .reg .b64 m; mov.b64 m, {%1, %1}; mul.rn.f32x2 %0, %0, m; }" : "+l"(x[i]) : "f"(sc));
         }
+    }
+    CT_DEV void take(const uint4 &w0, const uint4 &w1, float sc0, float sc1) {
+        bad = bad || !(fabsf(sc0) < INFINITY) || !(fabsf(sc1) < INFINITY);
+        if (DT == CT_KV_E4M3)                                /* a byte of seven ones is NaN (this cache stores none) */
+            bad = bad || ((((w0.x & 0x7F7F7F7Fu) + 0x01010101u) | ((w0.y & 0x7F7F7F7Fu) + 0x01010101u) |
+                           ((w1.x & 0x7F7F7F7Fu) + 0x01010101u) | ((w1.y & 0x7F7F7F7Fu) + 0x01010101u)) & 0x80808080u) != 0;
+        uint64_t x[4], y[4];
+        row(w0, sc0, x);
+        row(w1, sc1, y);
+        #pragma unroll
+        for (int i = 0; i < 4; i++)
+            asm("{ .reg .f32 a, b, c, d; mov.b64 {a, b}, %4; mov.b64 {c, d}, %5;\n\t"
+                "max.f32 %0, %0, a, c; min.f32 %1, %1, a, c; max.f32 %2, %2, b, d; min.f32 %3, %3, b, d; }"
+                : "+f"(hi[2 * i]), "+f"(lo[2 * i]), "+f"(hi[2 * i + 1]), "+f"(lo[2 * i + 1]) : "l"(x[i]), "l"(y[i]));
     }
     CT_DEV void finish() {}
 };
@@ -280,7 +295,7 @@ template <> struct Range8<CT_KV_BF16> {
             pl[e] = __nv_bfloat162(__nv_bfloat162_raw{0x7F80, 0x7F80});
         }
     }
-    CT_DEV void take(const uint4 &w, float) {
+    CT_DEV void one(const uint4 &w) {
         const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
         #pragma unroll
         for (int e = 0; e < 4; e++) {
@@ -290,6 +305,10 @@ template <> struct Range8<CT_KV_BF16> {
         }
         top = __vimax3_u16x2(top, ws[0] & 0x7FFF7FFFu, ws[1] & 0x7FFF7FFFu);
         top = __vimax3_u16x2(top, ws[2] & 0x7FFF7FFFu, ws[3] & 0x7FFF7FFFu);
+    }
+    CT_DEV void take(const uint4 &w0, const uint4 &w1, float, float) {
+        one(w0);
+        one(w1);
     }
     CT_DEV void finish() {
         bad = max(top & 0xFFFFu, top >> 16) >= 0x7F80u;
@@ -309,7 +328,7 @@ template <> struct Range8<CT_KV_BF16> {
  * way its tokens came.  A NaN or an infinity among the keys: scale NaN.
  * Bound by instructions when many pages are new (their keys are still in L2):
  * see Range8; by latency when few are.  256 pages of 64 tokens, 8 heads of
- * 128, int8: 9.9 us. */
+ * 128, int8: 8 us; 1024 of 16 tokens, 8 heads of 64: 14. */
 constexpr int kBoundThreads = 128;
 template <int D, int DT>
 __global__ void __launch_bounds__(kBoundThreads) k_gqa_bounds(const void *pool, const float *scales, uint32_t n_kv_heads,
@@ -327,19 +346,30 @@ __global__ void __launch_bounds__(kBoundThreads) k_gqa_bounds(const void *pool, 
     const size_t row0 = ((size_t)page * 2 * n_kv_heads + head) * page_tokens;
     Range8<DT> range;
     range.start();
+    /* `n` rows from token t + r on, in flight together; past the end: the last token once more */
+    auto rows = [&](uint32_t t, auto n) {
+        constexpr int N = decltype(n)::value;
+        uint4 w[N];
+        float sc[N];
+        #pragma unroll
+        for (int k = 0; k < N; k++) {
+            const size_t row = row0 + min(t + r + k * R, count - 1);
+            w[k] = load8<D, DT>(pool, row, u);
+            sc[k] = DT == CT_KV_BF16 ? 1.0f : __ldg(scales + row);
+        }
+        #pragma unroll
+        for (int k = 0; k < N; k += 2) range.take(w[k], w[k + 1], sc[k], sc[k + 1]);
+    };
     if (r < R) {
         #pragma unroll 1
-        for (uint32_t t = r; t < count; t += 8 * R) {        /* eight rows' loads in flight */
-            uint4 w[8];
-            float sc[8];
-            #pragma unroll
-            for (int k = 0; k < 8; k++) {
-                const size_t row = row0 + min(t + k * R, count - 1);     /* past the end: the last token once more */
-                w[k] = load8<D, DT>(pool, row, u);
-                sc[k] = DT == CT_KV_BF16 ? 1.0f : __ldg(scales + row);
+        for (uint32_t t = 0; t < count;) {
+            if (count - t > 2 * R) {
+                rows(t, std::integral_constant<int, 8>());
+                t += 8 * R;
+            } else {
+                rows(t, std::integral_constant<int, 2>());
+                t += 2 * R;
             }
-            #pragma unroll
-            for (int k = 0; k < 8; k++) range.take(w[k], sc[k]);
         }
     }
     range.finish();
