@@ -91,11 +91,10 @@ template <int D, int DT, int HT> struct Cfg {
     static constexpr int kStage = 2 * TS * kPitch + kScaleBytes;
     static constexpr int kRing = kWarps * kStages * kStage;
     /* Queries as operands: in registers, or (2 D / 16 registers a tile would
-     * spill) in shared memory behind the ring, a copy for each warp, where an
-     * SM has the room (1 KB of its 227 is for the joins' statics). */
+     * spill) in shared memory behind the ring, a copy for each warp. */
     static constexpr int kQPitch = 2 * D + 16;
     static constexpr int kQBytes = kWarps * HT * 8 * kQPitch;
-    static constexpr bool kQueriesInSmem = HT * D >= 192 && kRing + kQBytes <= 226 * 1024;
+    static constexpr bool kQueriesInSmem = HT * D >= 192;
     static constexpr int kUsed = kRing + (kQueriesInSmem ? kQBytes : 0);
     static constexpr int kMost = kRow <= 64 ? 32 : kRing < kInFlight ? kInFlight / kRing : 1;
     static constexpr int kShare = 227 * 1024 / (kMost + 1);      /* as much as keeps one CTA more out */
