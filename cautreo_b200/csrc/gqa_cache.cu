@@ -78,7 +78,7 @@ __global__ void __launch_bounds__(kThreads) k_gqa_write(void *pool, float *scale
     uint4 w[T][F32 ? 2 : 1];
     /* lane u finds the row of token u & (T - 1) for the lanes that share it */
     const uint32_t own = t0 + (u & (T - 1)) * R;
-    const int32_t slot = own < n ? __ldg(slots + own) : -1;
+    const int32_t slot = own < n ? slots[own] : -1;
     #pragma unroll
     for (int i = 0; i < T; i++) {
         const uint32_t t = t0 + i * R;
@@ -86,8 +86,8 @@ __global__ void __launch_bounds__(kThreads) k_gqa_write(void *pool, float *scale
         const size_t at = (size_t)t * stride + col;
         const uint4 *p = F32 ? reinterpret_cast<const uint4 *>(static_cast<const float *>(from) + at)
                              : reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(from) + at);
-        w[i][0] = __ldcs(p);
-        if (F32) w[i][F32 ? 1 : 0] = __ldcs(p + 1);
+        w[i][0] = ct_gqa_load_once(p);
+        if (F32) w[i][F32 ? 1 : 0] = ct_gqa_load_once(p + 1);
     }
     const size_t mine = pool_row(slot, place, n_kv_heads, page_tokens, page_magic, n_pages);
     /* The four tokens' maxima are reduced together: after two exchanges a lane
@@ -187,8 +187,8 @@ template <int DT> CT_DEV void values8(const uint4 &w, float sc, float *x) {
     }
 }
 template <int D, int DT> CT_DEV uint4 load8(const void *pool, size_t row, uint32_t u) {
-    if (DT == CT_KV_BF16) return __ldg(reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(pool) + row * D + u * 8));
-    const uint2 a = __ldg(reinterpret_cast<const uint2 *>(static_cast<const uint8_t *>(pool) + row * D + u * 8));
+    if (DT == CT_KV_BF16) return *reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(pool) + row * D + u * 8);
+    const uint2 a = *reinterpret_cast<const uint2 *>(static_cast<const uint8_t *>(pool) + row * D + u * 8);
     return make_uint4(a.x, a.y, 0u, 0u);
 }
 
@@ -207,7 +207,7 @@ __global__ void __launch_bounds__(kThreads) k_gqa_read(const void *pool, const f
     float sc[T];
     bool ok[T];
     const uint32_t own = t0 + (u & (T - 1)) * R;             /* as in the write */
-    const size_t mine = pool_row(own < n ? __ldg(slots + own) : -1, place, n_kv_heads, page_tokens, page_magic, n_pages);
+    const size_t mine = pool_row(own < n ? slots[own] : -1, place, n_kv_heads, page_tokens, page_magic, n_pages);
     #pragma unroll
     for (int i = 0; i < T; i++) {
         const size_t row = T == 1 ? mine : shfl_row(mine, (threadIdx.x & (32 - L)) | (i & (L - 1)));
@@ -215,7 +215,7 @@ __global__ void __launch_bounds__(kThreads) k_gqa_read(const void *pool, const f
         sc[i] = 1.0f;
         if (!ok[i]) continue;
         w[i] = load8<D, DT>(pool, row, u);
-        if (DT != CT_KV_BF16) sc[i] = __ldg(scales + row);
+        if (DT != CT_KV_BF16) sc[i] = scales[row];
     }
     #pragma unroll
     for (int i = 0; i < T; i++) {
@@ -339,7 +339,7 @@ __global__ void __launch_bounds__(kBoundThreads) k_gqa_bounds(const void *pool, 
     __shared__ float s_top[W];
     ct_gqa_enter();
     const uint32_t i = blockIdx.x / n_kv_heads, head = blockIdx.x - i * n_kv_heads;
-    const int32_t page = __ldg(pages + i), ct = __ldg(counts + i);
+    const int32_t page = pages[i], ct = counts[i];
     if (page < 0 || (uint32_t)page >= n_pages) return;
     const uint32_t count = ct < 0 ? 0u : min((uint32_t)ct, page_tokens);
     const uint32_t u = threadIdx.x % U, r = threadIdx.x / U;
@@ -355,7 +355,7 @@ __global__ void __launch_bounds__(kBoundThreads) k_gqa_bounds(const void *pool, 
         for (int k = 0; k < N; k++) {
             const size_t row = row0 + min(t + r + k * R, count - 1);
             w[k] = load8<D, DT>(pool, row, u);
-            sc[k] = DT == CT_KV_BF16 ? 1.0f : __ldg(scales + row);
+            sc[k] = DT == CT_KV_BF16 ? 1.0f : scales[row];
         }
         #pragma unroll
         for (int k = 0; k < N; k += 2) range.take(w[k], w[k + 1], sc[k], sc[k + 1]);

@@ -193,7 +193,7 @@ struct Seq {
 };
 template <int TS> CT_DEV Seq sequence(const ct_gqa_args_t &a, uint32_t s) {
     Seq r;
-    const int32_t n = __ldg(a.seq_lens + s);
+    const int32_t n = a.seq_lens[s];
     const uint32_t cap = a.max_pages * a.page_tokens;
     r.len = n < 0 ? 0u : ((uint32_t)n > cap ? cap : (uint32_t)n);
     r.start = a.window && r.len > a.window ? r.len - a.window : 0u;
@@ -389,12 +389,11 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, DT, HT>::kMinB) k_gqa_decode(
     /* Logical page of the e-th page stepped over (0xFFFFFFFF: none). */
     auto entry = [&](const Segment &z, uint32_t e) -> uint32_t {
         if (!a.picked) return e;
-        return e < z.sq.n_list ? (uint32_t)__ldg(a.picked + ((size_t)z.seq * a.n_kv_heads + z.head) * a.n_pick + e) : 0xFFFFFFFFu;
+        return e < z.sq.n_list ? (uint32_t)a.picked[((size_t)z.seq * a.n_kv_heads + z.head) * a.n_pick + e] : 0xFFFFFFFFu;
     };
     /* Its physical page (>= n_pages: nothing to read). */
     auto mapped = [&](const Segment &z, uint32_t lp) -> uint32_t {
-        return lp < z.sq.pages ? (uint32_t)__ldg(a.block_table + (size_t)z.seq * a.max_pages + lp)
-                                                                 : 0xFFFFFFFFu;
+        return lp < z.sq.pages ? (uint32_t)a.block_table[(size_t)z.seq * a.max_pages + lp] : 0xFFFFFFFFu;
     };
 
     /* ---- copies: S - 1 steps ahead of the arithmetic ----
@@ -543,11 +542,11 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, DT, HT>::kMinB) k_gqa_decode(
             #pragma unroll
             for (int b = 0; b < KB; b++) {
                 if (kQ8) {                                   /* values 4j .. 4j+3 of the block */
-                    const uint2 w = r < rows ? __ldg(reinterpret_cast<const uint2 *>(qp + b * 16 + 4 * j)) : make_uint2(0u, 0u);
+                    const uint2 w = r < rows ? *reinterpret_cast<const uint2 *>(qp + b * 16 + 4 * j) : make_uint2(0u, 0u);
                     qt[b][0] = w.x; qt[b][1] = w.y;
                 } else {
-                    qt[b][0] = r < rows ? __ldg(reinterpret_cast<const uint32_t *>(qp + b * 16 + 2 * j)) : 0u;
-                    qt[b][1] = r < rows ? __ldg(reinterpret_cast<const uint32_t *>(qp + b * 16 + 8 + 2 * j)) : 0u;
+                    qt[b][0] = r < rows ? *reinterpret_cast<const uint32_t *>(qp + b * 16 + 2 * j) : 0u;
+                    qt[b][1] = r < rows ? *reinterpret_cast<const uint32_t *>(qp + b * 16 + 8 + 2 * j) : 0u;
                 }
             }
             sc[t][0] = sc[t][1] = a.scale_log2;
@@ -944,7 +943,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, DT, HT>::kMinB) k_gqa_decode(
                     for (int i = 0; i < 3; i++) {
                         const uint32_t k = lane + 32 * i;
                         ml[i] = make_float2(kNoMax, 0.0f);
-                        if (k < n) ml[i] = __ldcg(reinterpret_cast<const float2 *>(a.part_ml + slot_of(k) * 32) + r);
+                        if (k < n) ml[i] = ct_gqa_load_l2(reinterpret_cast<const float2 *>(a.part_ml + slot_of(k) * 32) + r);
                         M = fmaxf(M, ml[i].x);
                     }
                     #pragma unroll
@@ -984,7 +983,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, DT, HT>::kMinB) k_gqa_decode(
                             const float4 *from = reinterpret_cast<const float4 *>(a.part_o + slot_of(k0 + k) * (16 * D));
                             #pragma unroll
                             for (int x = 0; x < kCols; x++)
-                                if (k0 + k < n && c0 + x * kThreads < cols) v[x][k] = __ldcg(from + c0 + x * kThreads);
+                                if (k0 + k < n && c0 + x * kThreads < cols) v[x][k] = ct_gqa_load_l2(from + c0 + x * kThreads);
                         }
                         #pragma unroll
                         for (int k = 0; k < kParts; k++) {

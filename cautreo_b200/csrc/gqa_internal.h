@@ -100,10 +100,33 @@ __device__ __forceinline__ uint32_t ct_gqa_args_t::page_of(uint32_t v) const { r
  * drains (programmatic stream serialization): each first lets its own
  * successor do the same, then waits until everything before it has finished
  * and its writes are visible.  Nothing is read or written earlier, so only
- * launch latency overlaps (1 to 2 us of a small call). */
+ * launch latency overlaps (1 to 2 us of a small call).
+ * The kernel before may write what this one reads while this one is already
+ * resident, so no memory is read-only for as long as these kernels run: they
+ * load with coherent loads that stay behind the wait (ordinary ones, or those
+ * below), never through the non-coherent path, whose loads the wait does not
+ * cover and the compiler may move. */
 static __device__ __forceinline__ void ct_gqa_enter() {
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
+}
+/* Loads with a cache hint, in program order with the wait above, with barriers
+ * and with fences (the hinted intrinsics promise no order): values read once,
+ * and what another CTA of the same launch left in L2. */
+static __device__ __forceinline__ uint4 ct_gqa_load_once(const uint4 *p) {
+    uint4 v;
+    asm volatile("ld.global.cs.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+    return v;
+}
+static __device__ __forceinline__ float4 ct_gqa_load_l2(const float4 *p) {
+    float4 v;
+    asm volatile("ld.global.cg.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "l"(p) : "memory");
+    return v;
+}
+static __device__ __forceinline__ float2 ct_gqa_load_l2(const float2 *p) {
+    float2 v;
+    asm volatile("ld.global.cg.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "l"(p) : "memory");
+    return v;
 }
 template <class... P, class... A>
 static inline cudaError_t ct_gqa_launch(void (*k)(P...), dim3 grid, dim3 block, size_t smem, cudaStream_t st, uint32_t cluster,

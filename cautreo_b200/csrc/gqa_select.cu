@@ -89,7 +89,7 @@ __global__ void __launch_bounds__(kThreads, kResident<D>) k_gqa_select(const ct_
         #pragma unroll
         for (int t = 0; t < kTiles; t++) {
             const uint32_t p = p0 + t * 8 + g;
-            ph[t] = p < pe ? __ldg(table + p) : -1;
+            ph[t] = p < pe ? table[p] : -1;
         }
     };
     const uint32_t n_tiles = (a.group + 15) / 16;
@@ -138,8 +138,8 @@ __global__ void __launch_bounds__(kThreads, kResident<D>) k_gqa_select(const ct_
                 const size_t at = (size_t)(ok[t] ? ph[t] : 0) * a.n_kv_heads + head;
                 const uint4 *src = reinterpret_cast<const uint4 *>(a.bounds + at * 2 * D) + j;
                 #pragma unroll
-                for (int b = 0; b < D / 32; b++) w[t][b] = ok[t] ? __ldg(src + b * 4) : make_uint4(0u, 0u, 0u, 0u);
-                ps[t] = ok[t] ? __ldg(a.bound_scales + at) : 0.0f;
+                for (int b = 0; b < D / 32; b++) w[t][b] = ok[t] ? src[b * 4] : make_uint4(0u, 0u, 0u, 0u);
+                ps[t] = ok[t] ? a.bound_scales[at] : 0.0f;
             }
             numbers(p0 + kWarps * kStep);
             /* rows = pages p0 + g and p0 + 8 + g, columns = heads 2j, 2j + 1 of a

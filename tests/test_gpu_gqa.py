@@ -815,3 +815,58 @@ def test_decode_many_selected_pages(dtype, window):
     torch.cuda.synchronize()
     G.check_attention(out, lse, G.attend(q, pool, scales, table, lens, dtype, heads * group, MOD, window, pages=pages), dim,
                       max(lens), dtype)
+
+
+@pytest.mark.parametrize("dtype", [BF16, INT8, E4M3])
+def test_calls_in_a_row_see_what_the_one_before_wrote(dtype):
+    """Write, bounds, read back, selection, both decodes and a copy of the lengths, over the same buffers again and again
+    without a wait: the bits of the same calls with a wait after each."""
+    g = gen(91)
+    heads, group, dim, page, S, pick, steps = 2, 4, 64, 16, 6, 3, 60
+    hq, per, n_pages = heads * group, 12, 6 * 12
+    layout = ct.GqaLayout(heads, dim, page, dtype, n_pages, per)
+    plan = ct.GqaPlan(layout, S, hq)
+    n, width = S * page * 5, heads * dim
+    x = torch.randn(steps, n, 2 * width, generator=g, device="cuda").bfloat16()
+    q = torch.randn(steps, S, hq, dim, generator=g, device="cuda").bfloat16()
+    tables = torch.stack([torch.randperm(n_pages, generator=g, device="cuda").view(S, per) for _ in range(steps)]).to(torch.int32)
+    lens_bank = torch.randint(1, 5 * page + 1, (steps, S), generator=g, device="cuda").to(torch.int32)
+    t = torch.arange(page * 5, device="cuda")
+    slot_bank = (tables[:, :, t // page] * page + t % page).reshape(steps, n).contiguous()
+
+    def run(wait):
+        pool = torch.zeros(n_pages, 2, heads, page, dim, device="cuda",
+                           dtype={BF16: torch.bfloat16, INT8: torch.int8, E4M3: torch.uint8}[dtype])
+        scales = None if dtype == BF16 else torch.zeros(n_pages, 2, heads, page, device="cuda")
+        bounds = torch.zeros(n_pages, heads, 2, dim, dtype=torch.int8, device="cuda")
+        bs = torch.zeros(n_pages, heads, device="cuda")
+        pages = torch.arange(n_pages, dtype=torch.int32, device="cuda")
+        counts = torch.full((n_pages,), page, dtype=torch.int32, device="cuda")
+        slots, table, lens, picked = slot_bank[0].clone(), tables[0].clone(), lens_bank[0].clone(), torch.zeros(
+            S, heads, pick, dtype=torch.int32, device="cuda")
+        back = torch.zeros(steps, 2, n, width, device="cuda")
+        out = torch.zeros(steps, 2, S, hq, dim, device="cuda").bfloat16()
+        chosen = torch.zeros(steps, S, heads, pick, dtype=torch.int32, device="cuda")
+        torch.cuda.synchronize()
+        for i in range(steps):
+            def then():
+                if wait:
+                    torch.cuda.synchronize()
+            slots.copy_(slot_bank[i]); then()  # noqa: E702
+            ct.gqa_write_slots(layout, pool, scales, x[i], x[i, :, width:], slots, n, k_stride=2 * width, v_stride=2 * width,
+                               stream=stream()); then()  # noqa: E702
+            ct.gqa_page_bounds(layout, pool, scales, pages, counts, n_pages, bounds, bs, stream=stream()); then()  # noqa: E702
+            ct.gqa_read_slots(layout, pool, scales, slots, n, back[i, 0], back[i, 1], out_dtype=ct.CT_KV_F32,
+                              stream=stream()); then()  # noqa: E702
+            table.copy_(tables[i]); lens.copy_(lens_bank[i]); then()  # noqa: E702
+            plan.select(q[i], bounds, bs, table, lens, picked, pick, stream=stream()); then()  # noqa: E702
+            plan.decode_selected(q[i], pool, scales, table, lens, picked, pick, out[i, 0], stream=stream()); then()  # noqa: E702
+            plan.decode(q[i], pool, scales, table, lens, out[i, 1], stream=stream()); then()  # noqa: E702
+            chosen[i].copy_(picked); then()  # noqa: E702
+        torch.cuda.synchronize()
+        return back, out, chosen
+
+    want = run(True)
+    for _ in range(3):
+        for a, b in zip(run(False), want):
+            assert torch.equal(a, b)

@@ -1,5 +1,7 @@
 """CPU: what grouped-query caches refuse, and their tables without a device."""
 import ctypes as C
+import re
+from pathlib import Path
 
 import numpy as np
 import pytest
@@ -110,3 +112,13 @@ def test_plans_of_too_many_steps_refused():
             s.kv.max_pages_per_seq = 60000
         assert not ct.lib().ct_gqa_plan_create(C.byref(s), n_seq, 0)
         assert b"too many" in ct.lib().ct_hal_cuda_last_error()
+
+
+def test_kernels_launched_early_load_coherently():
+    """These kernels are resident while the one before them still writes what they read, so none of their loads may take the
+    non-coherent path, nor be an intrinsic that is free to move above the wait."""
+    csrc = Path(ct.__file__).resolve().parent / "csrc"
+    sources = sorted(csrc.glob("gqa_*"))
+    assert len(sources) >= 5
+    for f in sources:
+        assert not re.findall(r"__ldg\b|__ldc[agsv]\b|__ldlu\b|global\.nc\b|__restrict__", f.read_text()), f.name
