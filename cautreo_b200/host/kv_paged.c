@@ -669,13 +669,15 @@ int ct_kv_paged_fork(ct_kv_paged_t *h, uint32_t src, uint32_t dst, uint32_t n_to
     }
     int32_t copy_from = -1, copy_to = -1;
     if (!rc && rem) {                                 /* the partial page: dst's own copy */
+        copy_from = h->bt[(size_t)src * MP + full];
         if (h->heap_n == 0) {
+            h->refc[copy_from]++;                     /* as a shared page: no victim while it is to be read */
             int64_t c = lru_victim(h);
+            h->refc[copy_from]--;
             if (c < 0) { ct__set_error("fork: no evictable page"); rc = CT_ERR_FULL; }
             else rc = free_low_page(h, (uint32_t)c, 2);
         }
         if (!rc) {
-            copy_from = h->bt[(size_t)src * MP + full];
             copy_to = heap_pop(h);
             h->refc[copy_to] = 1;
             h->st.n_pages_live++;

@@ -197,7 +197,8 @@ int  ct_kv_paged_gather(ct_kv_paged_t *h, uint32_t seq, uint32_t start, uint32_t
  * Full pages are shared -- both block tables map them and a page returns to
  * the free set only when no sequence maps it -- and a partial last page is
  * copied into a page of dst's own, so appends never write a shared page.
- * Shared pages are not LRU victims; a sequence's window releases its
+ * Shared pages are not LRU victims, nor is the page being copied (CT_ERR_FULL
+ * if no page is free and there is no other); a sequence's window releases its
  * references; compaction keeps them shared.  CT_ERR_UNMAPPED if the window
  * already dropped part of src's prefix. */
 int      ct_kv_paged_fork(ct_kv_paged_t *h, uint32_t src, uint32_t dst, uint32_t n_tokens);

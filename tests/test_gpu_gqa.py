@@ -870,3 +870,22 @@ def test_calls_in_a_row_see_what_the_one_before_wrote(dtype):
     for _ in range(3):
         for a, b in zip(run(False), want):
             assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("dtype", [BF16, INT8])
+def test_fork_from_a_full_pool_keeps_the_source(dtype):
+    """No page is free: another sequence gives one up, the fork reads what its source reads, and the source keeps its tokens."""
+    heads, dim, page = 2, 64, 16
+    g = gen(92)
+    kv = ct.GqaKV(3, 8, 4, heads, dim, page, dtype=dtype, keep_bounds=True, stream=stream())
+    x = rows(64, heads, dim, g)
+    kv.append_kv([0, 2], [32, 32], x[0], x[1])
+    kv.fork(0, 1, 5)
+    got = torch.empty(2, 37, heads * dim, device="cuda")
+    kv.gather_kv([0, 1], [0, 0], [32, 5], got[0], got[1], ct.CT_KV_F32)
+    torch.cuda.synchronize()
+    for i in range(2):
+        want = stored_as(x[i], dtype, heads, dim)
+        assert torch.equal(got[i], torch.cat((want[:32], want[:5])))
+    assert ct.lib().ct_kv_paged_gather(kv.h, 2, 0, 1, got.data_ptr(), BF16) == ct.CT_ERR_UNMAPPED
+    check_bounds(kv, heads, dim, page, dtype)

@@ -461,3 +461,32 @@ def test_token_ids_prefix_match_fork_and_checkpoint(tmp_path):
     assert np.array_equal(g1.block_table(), h.block_table()) and len(g1.tokens(0)) == 0
     g1.close()
     h.close()
+
+
+@pytest.mark.parametrize("gqa", [False, True])
+def test_fork_does_not_evict_the_page_it_copies(gqa):
+    """Less than a page is forked and no page is free: the source's only candidate page is the one to be copied, so another
+    sequence gives one up, or the fork is refused and changes nothing."""
+    def handle(n_pages):
+        return ct.GqaKV(3, 8, n_pages, 2, 64, 16, device=-1) if gqa else ct.PagedKV(3, 8, n_pages, 16, 64, device=-1)
+
+    h = handle(3)
+    h.append([0], [48])
+    before = h.block_table()
+    assert ct.lib().ct_kv_paged_fork(h.h, 0, 1, 5) == ct.CT_ERR_FULL
+    assert np.array_equal(h.block_table(), before) and h.seq_lens().tolist() == [48, 0, 0]
+    assert h.stats().n_evict_lru == 0 and h.stats().n_pages_live == 3
+    assert [ct.lib().ct_kv_paged_page_refs(h.h, p) for p in range(3)] == [1, 1, 1]
+
+    h = handle(4)                                     # the source is the least recently used one of two
+    h.append([0], [32])
+    h.append([2], [32])
+    h.fork(0, 1, 5)
+    t = h.block_table()
+    assert t[0, :2].tolist() == before[0, :2].tolist()                # the source keeps its prefix
+    assert t[2, 0] == -1 and t[1, 0] >= 0 and t[1, 0] not in t[0].tolist()
+    assert h.seq_lens().tolist() == [32, 5, 32]
+    assert [ct.lib().ct_kv_paged_page_refs(h.h, p) for p in range(4)] == [1, 1, 1, 1]
+    h.append([1], [3])                                # and both go on
+    h.append([0], [1])
+    assert h.block_table()[0, 0] == -1                # now it is the source's turn: no longer kept out
