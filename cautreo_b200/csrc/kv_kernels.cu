@@ -866,8 +866,9 @@ __global__ void __launch_bounds__(256) k_move_pages(const uint4 *src, const floa
         __stcs(d + i, a); __stcs(d + i + 256, b); __stcs(d + i + 512, c); __stcs(d + i + 768, e);
     }
     for (; i < vec_per_page; i += 256) __stcs(d + i, __ldcs(s + i));
-    if (src_sc && threadIdx.x < page_tokens)
-        dst_sc[(size_t)blockIdx.x * page_tokens + threadIdx.x] = src_sc[from * page_tokens + threadIdx.x];
+    if (src_sc)
+        for (uint32_t t = threadIdx.x; t < page_tokens; t += 256)
+            dst_sc[(size_t)blockIdx.x * page_tokens + t] = src_sc[from * page_tokens + t];
 }
 
 /* ct_kv_compress: row j of the kept set is row j*step (per layer), copied
@@ -992,7 +993,7 @@ extern "C" int ct_kv_paged_write_slots(void *pool, float *scales, uint32_t pool_
 extern "C" int ct_kv_paged_move_pages(const void *src_pool, const float *src_scales, void *dst_pool,
                                       float *dst_scales, const int32_t *map, uint32_t n_pages,
                                       size_t page_bytes, uint32_t page_tokens, void *stream) {
-    if (!src_pool || !dst_pool || !map || page_bytes % 16 != 0 || page_tokens > 256) return CT_ERR_ARG;
+    if (!src_pool || !dst_pool || !map || page_bytes % 16 != 0) return CT_ERR_ARG;
     if ((src_scales == NULL) != (dst_scales == NULL)) return CT_ERR_ARG;
     if (n_pages == 0) return CT_OK;
     k_move_pages<<<n_pages, 256, 0, (cudaStream_t)stream>>>(

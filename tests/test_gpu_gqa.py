@@ -889,3 +889,51 @@ def test_fork_from_a_full_pool_keeps_the_source(dtype):
         assert torch.equal(got[i], torch.cat((want[:32], want[:5])))
     assert ct.lib().ct_kv_paged_gather(kv.h, 2, 0, 1, got.data_ptr(), BF16) == ct.CT_ERR_UNMAPPED
     check_bounds(kv, heads, dim, page, dtype)
+
+
+@pytest.mark.parametrize("dtype,page", [(BF16, 272), (INT8, 272), (INT8, 512), (E4M3, 512), (BF16, 512)])
+def test_large_pages_append_compact_checkpoint_and_decode(dtype, page, tmp_path):
+    heads, group, dim = 2, 4, 64
+    hq = heads * group
+    g = gen(page + dtype)
+    kv = ct.GqaKV(3, 6, 12, heads, dim, page, dtype=dtype, keep_bounds=True, stream=stream())
+    kv.set_free_order(np.random.default_rng(6).permutation(12))
+    lens = [3 * page + 7, 1, 2 * page]
+    x = rows(sum(lens), heads, dim, g)
+    kv.append_kv([0, 1, 2], lens, x[0], x[1])
+    wk, wv = stored_as(x[0], dtype, heads, dim), stored_as(x[1], dtype, heads, dim)
+
+    def same(h):
+        k, v = (torch.empty(sum(lens), heads * dim, device="cuda") for _ in range(2))
+        h.gather_kv(range(3), [0] * 3, lens, k, v, ct.CT_KV_F32)
+        torch.cuda.synchronize()
+        assert torch.equal(k, wk) and torch.equal(v, wv)
+        check_bounds(h, heads, dim, page, dtype)
+        q = torch.randn(3, hq, dim, generator=g, device="cuda").bfloat16()
+        plan = ct.GqaPlan(h.layout, 3, hq)
+        out, sel = (torch.empty(3, hq, dim, device="cuda").bfloat16() for _ in range(2))
+        picked = torch.empty(3, heads, 2, dtype=torch.int32, device="cuda")
+        plan.decode(q, h.pool, h.scales, h.block_table_dev, h.seq_lens_dev, out, stream=stream())
+        plan.select(q, h.bounds, h.bound_scales, h.block_table_dev, h.seq_lens_dev, picked, 2, 1, 0, stream=stream())
+        plan.decode_selected(q, h.pool, h.scales, h.block_table_dev, h.seq_lens_dev, picked, 2, sel, stream=stream())
+        torch.cuda.synchronize()
+        NP, tb = h.layout.n_pages, torch.from_numpy(h.block_table()).cuda()
+        shape = (NP, 2, heads, page, dim)
+        pool = dev_copy(h.pool, shape, {BF16: torch.bfloat16, INT8: torch.int8, E4M3: torch.uint8}[dtype])
+        scales = None if dtype == BF16 else dev_copy(h.scales, shape[:4], torch.float32)
+        bounds = dev_copy(h.bounds, (NP, heads, 2, dim), torch.int8).cpu().numpy()
+        bs = dev_copy(h.bound_scales, (NP, heads), torch.float32).cpu().numpy()
+        want = G.select(q.float().cpu().numpy(), bounds, bs, tb.cpu().numpy(), lens, NP, page, hq, MOD, 2, 1, 0)
+        assert np.array_equal(picked.cpu().numpy(), want)
+        G.check_attention(out, None, G.attend(q, pool, scales, tb, lens, dtype, hq, MOD), dim, max(lens), dtype)
+        G.check_attention(sel, None, G.attend(q, pool, scales, tb, lens, dtype, hq, MOD, pages=want), dim, max(lens), dtype)
+
+    same(kv)
+    kv.compact()
+    assert sorted(kv.block_table()[kv.block_table() >= 0].tolist()) == list(range(7))
+    same(kv)
+    kv.save(tmp_path / "p.bin")
+    back = ct.GqaKV.load(tmp_path / "p.bin", stream=stream())
+    same(back)
+    back.compact()
+    same(back)

@@ -122,3 +122,13 @@ def test_kernels_launched_early_load_coherently():
     assert len(sources) >= 5
     for f in sources:
         assert not re.findall(r"__ldg\b|__ldc[agsv]\b|__ldlu\b|global\.nc\b|__restrict__", f.read_text()), f.name
+
+
+def test_pages_of_every_size_may_move():
+    """A cache takes pages of up to 512 tokens here (latent caches any number), so its compaction has to move them."""
+    L, a = ct.lib(), 4096
+    for tokens in (16, 256, 272, 512, 4096):
+        assert L.ct_kv_paged_move_pages(a, a, a, a, a, 0, 16, tokens, None) == ct.CT_OK, tokens
+        assert L.ct_kv_paged_move_pages(a, None, a, None, a, 0, 16, tokens, None) == ct.CT_OK, tokens
+    assert L.ct_kv_paged_move_pages(a, None, a, a, a, 0, 16, 64, None) == ct.CT_ERR_ARG
+    assert L.ct_kv_paged_move_pages(a, None, a, None, a, 0, 24, 64, None) == ct.CT_ERR_ARG
