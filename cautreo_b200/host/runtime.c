@@ -19,6 +19,7 @@ int ct__cuda_status(int code, const char *where) {
     if (code == 0) return CT_OK;
     snprintf(g_last_error, sizeof g_last_error, "%s: %s (%d)", where ? where : "cuda",
              cudaGetErrorString((cudaError_t)code), code);
+    cudaGetLastError();                               /* reported here: the next launch must not find it again */
     return CT_ERR_CUDA;
 }
 

@@ -1,0 +1,117 @@
+"""CPU: the host layer of the paged caches and the grouped-query plans over a device made of host memory, which can be made to
+fail at any call (tests/fake_cuda.c)."""
+import ctypes as C
+import shutil
+import subprocess
+from pathlib import Path
+
+import numpy as np
+import pytest
+
+import cautreo_b200 as ct
+from cautreo_b200 import build as B
+
+ROOT = Path(__file__).resolve().parent.parent
+
+
+@pytest.fixture(scope="module")
+def fake(tmp_path_factory):
+    """The host sources linked with the fake device, the package's signatures declared on it."""
+    so = tmp_path_factory.mktemp("fake") / "libfake.so"
+    host = ROOT / "cautreo_b200" / "host"
+    cc = shutil.which("gcc") or "gcc"
+    r = subprocess.run([cc, *B.CC_FLAGS, "-Wno-sign-compare", "-shared", "-o", str(so), str(ROOT / "tests" / "fake_cuda.c"),
+                        *(str(host / f) for f in ("kv_paged.c", "gqa.c", "runtime.c")), "-lm", "-lpthread"],
+                       capture_output=True, text=True)
+    assert r.returncode == 0, r.stderr
+    L = C.CDLL(str(so))
+    for name, (res, args) in ct.SIGNATURES.items():
+        if hasattr(L, name):
+            f = getattr(L, name)
+            f.restype, f.argtypes = res, args
+    L.fake_fail.argtypes = [C.c_long]
+    L.fake_pending.restype = L.fake_live.restype = C.c_long
+    return L
+
+
+class Handle:
+    """A handle of the fake device: 4 sequences of 8 pages of 16 tokens, bf16, 2 heads of 32 (or entries of 128 values)."""
+    S, MP, NP, P, H, D = 4, 8, 20, 16, 2, 32
+    W = H * D
+
+    def __init__(self, L, gqa, bounds=True, n_pages=None):
+        self.L, self.gqa = L, gqa
+        cfg = ct.PagedConfig(self.S, self.MP, n_pages or self.NP, self.P, 2 * self.W, 0, ct.CT_KV_BF16, 0)
+        self.h = (L.ct_kv_paged_create_gqa(C.byref(cfg), self.H, self.D, int(bounds)) if gqa else L.ct_kv_paged_create(C.byref(cfg)))
+        self.np = n_pages or self.NP
+        self.rng = np.random.default_rng(7)
+        self.rows = [np.zeros((0, 2 * self.W), np.uint16) for _ in range(self.S)]
+
+    def append(self, seqs, counts):
+        x = self.rng.integers(0, 1 << 16, (sum(counts), 2 * self.W), dtype=np.uint16)
+        s, c = np.array(seqs, np.uint32), np.array(counts, np.uint32)
+        aligned = C.create_string_buffer(x.nbytes + 32)
+        at = (C.addressof(aligned) + 31) // 16 * 16
+        C.memmove(at, x.ctypes.data, x.nbytes)
+        rc = self.L.ct_kv_paged_append(self.h, s.ctypes.data, c.ctypes.data, len(s), at, ct.CT_KV_BF16)
+        if rc == 0:
+            o = 0
+            for q, n in zip(seqs, counts):
+                self.rows[q] = np.concatenate((self.rows[q], x[o:o + n]))
+                o += n
+        return rc
+
+    def fork(self, src, dst, n):
+        rc = self.L.ct_kv_paged_fork(self.h, src, dst, n)
+        if rc == 0:
+            self.rows[dst] = self.rows[src][:n].copy()
+        return rc
+
+    def table(self):
+        t = np.zeros((self.S, self.MP), np.int32)
+        self.L.ct_kv_paged_block_table(self.h, t.ctypes.data)
+        return t
+
+    def check(self):
+        """Host and device tables agree, every token reads back, references and free pages add up, bounds follow."""
+        t = self.table()
+        dev = np.ctypeslib.as_array(C.cast(self.L.ct_kv_paged_block_table_dev(self.h), C.POINTER(C.c_int32)), t.shape)
+        assert np.array_equal(dev, t)
+        lens = np.ctypeslib.as_array(C.cast(self.L.ct_kv_paged_seq_lens_dev(self.h), C.POINTER(C.c_int32)), (self.S,))
+        assert lens.tolist() == [len(r) for r in self.rows]
+        out = C.create_string_buffer(2 * 2 * self.W * self.P * self.MP + 32)
+        at = (C.addressof(out) + 31) // 16 * 16
+        for s, r in enumerate(self.rows):
+            if len(r) == 0:
+                continue
+            assert self.L.ct_kv_paged_gather(self.h, s, 0, len(r), at, ct.CT_KV_BF16) == 0
+            got = np.frombuffer((C.c_char * r.nbytes).from_address(at), np.uint16).reshape(r.shape)
+            assert np.array_equal(got, r), s
+        ids, n = np.unique(t[t >= 0], return_counts=True)
+        assert [self.L.ct_kv_paged_page_refs(self.h, int(p)) for p in ids] == n.tolist()
+        st = self.L.ct_kv_paged_stats(self.h)
+        assert st.n_pages_live == len(ids) and st.n_pages_free == self.np - len(ids)
+        if self.gqa and self.L.ct_kv_paged_bound_scales(self.h):
+            bs = np.ctypeslib.as_array(C.cast(self.L.ct_kv_paged_bound_scales(self.h), C.POINTER(C.c_float)), (self.np, self.H))
+            for s, r in enumerate(self.rows):
+                for lp in range(-(-len(r) // self.P)):
+                    assert (bs[t[s, lp]] == min(self.P, len(r) - lp * self.P)).all()
+
+    def close(self):
+        self.L.ct_kv_paged_destroy(self.h)
+
+
+def test_an_error_is_reported_once(fake):
+    """A call that failed (here a plan whose scratch does not fit) does not make the next call, which works, fail as well."""
+    h = Handle(fake, True)
+    assert h.append([0, 1], [20, 3]) == 0
+    lay = ct.GqaLayout()
+    assert fake.ct_kv_paged_gqa_layout(h.h, C.byref(lay)) == 0
+    shape = ct.GqaShape(lay, 4, 0, 0, 0.0)
+    for k in (1, 2, 3):                               # the scratch, its stream, its zeroes
+        fake.fake_fail(k)
+        assert not fake.ct_gqa_plan_create(C.byref(shape), 2, 0) and fake.fake_pending() < 0
+        assert b"gqa scratch" in fake.ct_hal_cuda_last_error()
+        assert h.append([0, 1], [1, 1]) == 0
+        h.check()
+    h.close()
