@@ -16,11 +16,12 @@ ROOT = Path(__file__).resolve().parent.parent
 
 @pytest.fixture(scope="module")
 def fake(tmp_path_factory):
-    """The host sources linked with the fake device, the package's signatures declared on it."""
+    """The host sources linked with the fake device (-Bsymbolic: also where a CUDA runtime is loaded), the package's signatures
+    declared on it."""
     so = tmp_path_factory.mktemp("fake") / "libfake.so"
     host = ROOT / "cautreo_b200" / "host"
     cc = shutil.which("gcc") or "gcc"
-    r = subprocess.run([cc, *B.CC_FLAGS, "-Wno-sign-compare", "-shared", "-o", str(so), str(ROOT / "tests" / "fake_cuda.c"),
+    r = subprocess.run([cc, *B.CC_FLAGS, "-Wno-sign-compare", "-shared", "-Wl,-Bsymbolic", "-o", str(so), str(ROOT / "tests" / "fake_cuda.c"),
                         *(str(host / f) for f in ("kv_paged.c", "gqa.c", "runtime.c")), "-lm", "-lpthread"],
                        capture_output=True, text=True)
     assert r.returncode == 0, r.stderr
