@@ -774,101 +774,98 @@ int ct_kv_paged_match_prefix(const ct_kv_paged_t *h, const int32_t *ids, uint32_
 
 /* ---- compaction ----------------------------------------------------------- */
 
+/* The tables change only after every device step has succeeded: a compaction
+ * that fails leaves the handle as it was. */
 int ct_kv_paged_compact(ct_kv_paged_t *h) {
     if (!h) return CT_ERR_ARG;
     const uint32_t S = h->cfg.n_seqs, MP = h->cfg.max_pages_per_seq, NP = h->cfg.n_pages, P = h->cfg.page_tokens;
-    int32_t *map;
-    int rc = CT_OK;
-    if (h->host_only) {
-        map = h->heap;                            /* scratch: rebuilt below */
-    } else {
-        rc = stage_reserve(h, (size_t)S * MP + NP + 64);
-        if (rc) return rc;
-        map = h->stage_host;                      /* [n_live] new -> old, then the bt image */
-    }
+    const size_t bt_n = (size_t)S * MP;
+    int rc = h->host_only ? CT_OK : stage_reserve(h, bt_n + NP + 64);
+    if (rc) return rc;
     /* a page shared by several sequences gets one new id, at its first use */
     int32_t *new_id = (int32_t *)malloc((size_t)NP * sizeof(int32_t));
+    int32_t *map = (int32_t *)malloc((size_t)NP * sizeof(int32_t));                /* [n_live] new -> old */
     uint32_t *refc2 = (uint32_t *)calloc(NP, sizeof(uint32_t));
-    if (!new_id || !refc2) { free(new_id); free(refc2); return CT_ERR_NOMEM; }
+    if (!new_id || !map || !refc2) { free(new_id); free(map); free(refc2); return CT_ERR_NOMEM; }
     for (uint32_t p = 0; p < NP; p++) new_id[p] = -1;
     uint32_t n_live = 0;
     for (uint32_t s = 0; s < S; s++)
         for (uint32_t lp = h->lo[s]; lp < h->hi[s]; lp++) {
-            int32_t *e = h->bt + (size_t)s * MP + lp;
-            if (new_id[*e] < 0) {
-                new_id[*e] = (int32_t)n_live;
-                refc2[n_live] = h->refc[*e];
-                map[n_live++] = *e;
-            }
-            *e = new_id[*e];
+            const int32_t old = h->bt[(size_t)s * MP + lp];
+            if (new_id[old] >= 0) continue;
+            new_id[old] = (int32_t)n_live;
+            refc2[n_live] = h->refc[old];
+            map[n_live++] = old;
         }
-    memcpy(h->refc, refc2, (size_t)NP * sizeof(uint32_t));
-    free(new_id);
-    free(refc2);
-    if (h->host_only) goto renumbered;
-    void *new_pool = NULL;
-    float *new_scales = NULL, *new_bscales = NULL;
-    int8_t *new_bounds = NULL;
-    const size_t sc_row = (size_t)P * h->scale_rows;  /* scales of a page */
-    const size_t b_page = (size_t)h->gqa_heads * 2 * h->gqa_dim;
-    /* stream-ordered allocations: after the first compaction the pool's
-     * memory comes back from the driver's cache without a device sync */
-    rc = ct__cuda_status(cudaMallocAsync(&new_pool, (size_t)NP * h->page_bytes, h->stream), "compact pool");
-    if (!rc && h->scales)
-        rc = ct__cuda_status(cudaMallocAsync((void **)&new_scales, (size_t)NP * sc_row * sizeof(float), h->stream),
-                             "compact scales");
-    if (!rc && new_scales) rc = ct__cuda_status(cudaMemsetAsync(new_scales, 0, (size_t)NP * sc_row * sizeof(float), h->stream), "compact");
-    if (!rc && h->bounds) {
-        rc = ct__cuda_status(cudaMallocAsync((void **)&new_bounds, (size_t)NP * b_page, h->stream), "compact bounds");
-        if (!rc)
-            rc = ct__cuda_status(cudaMallocAsync((void **)&new_bscales, (size_t)NP * h->gqa_heads * sizeof(float), h->stream),
-                                 "compact bounds");
-    }
-    /* bt image follows the map in the staging buffer */
-    memcpy(map + n_live, h->bt, (size_t)S * MP * sizeof(int32_t));
-    if (!rc) rc = ct__cuda_status(cudaMemcpyAsync(h->stage_dev, map, ((size_t)n_live + (size_t)S * MP) * sizeof(int32_t),
-                                                  cudaMemcpyHostToDevice, h->stream), "compact upload");
-    if (!rc && !h->gqa_heads)
-        rc = ct_kv_paged_move_pages(h->pool, h->scales, new_pool, new_scales, h->stage_dev, n_live, h->page_bytes, P, h->stream);
-    if (!rc && h->gqa_heads) {                        /* a page's scales and bounds are byte runs of their own */
-        rc = ct_kv_paged_move_pages(h->pool, NULL, new_pool, NULL, h->stage_dev, n_live, h->page_bytes, P, h->stream);
+    if (!h->host_only) {
+        void *new_pool = NULL;
+        float *new_scales = NULL, *new_bscales = NULL;
+        int8_t *new_bounds = NULL;
+        const size_t sc_row = (size_t)P * h->scale_rows;  /* scales of a page */
+        const size_t b_page = (size_t)h->gqa_heads * 2 * h->gqa_dim;
+        /* stream-ordered allocations: after the first compaction the pool's
+         * memory comes back from the driver's cache without a device sync */
+        rc = ct__cuda_status(cudaMallocAsync(&new_pool, (size_t)NP * h->page_bytes, h->stream), "compact pool");
         if (!rc && h->scales)
-            rc = ct_kv_paged_move_pages(h->scales, NULL, new_scales, NULL, h->stage_dev, n_live, sc_row * sizeof(float), P,
-                                        h->stream);
-        if (!rc && h->bounds)
-            rc = ct_kv_paged_move_pages(h->bounds, h->bound_scales, new_bounds, new_bscales, h->stage_dev, n_live, b_page,
-                                        h->gqa_heads, h->stream);
+            rc = ct__cuda_status(cudaMallocAsync((void **)&new_scales, (size_t)NP * sc_row * sizeof(float), h->stream),
+                                 "compact scales");
+        if (!rc && new_scales)
+            rc = ct__cuda_status(cudaMemsetAsync(new_scales, 0, (size_t)NP * sc_row * sizeof(float), h->stream), "compact");
+        if (!rc && h->bounds) {
+            rc = ct__cuda_status(cudaMallocAsync((void **)&new_bounds, (size_t)NP * b_page, h->stream), "compact bounds");
+            if (!rc)
+                rc = ct__cuda_status(cudaMallocAsync((void **)&new_bscales, (size_t)NP * h->gqa_heads * sizeof(float), h->stream),
+                                     "compact bounds");
+        }
+        /* the new table follows the map in the staging buffer */
+        memcpy(h->stage_host, map, (size_t)n_live * sizeof(int32_t));
+        for (size_t i = 0; i < bt_n; i++) h->stage_host[n_live + i] = h->bt[i] < 0 ? -1 : new_id[h->bt[i]];
+        if (!rc) rc = ct__cuda_status(cudaMemcpyAsync(h->stage_dev, h->stage_host, ((size_t)n_live + bt_n) * sizeof(int32_t),
+                                                      cudaMemcpyHostToDevice, h->stream), "compact upload");
+        if (!rc && !h->gqa_heads)
+            rc = ct_kv_paged_move_pages(h->pool, h->scales, new_pool, new_scales, h->stage_dev, n_live, h->page_bytes, P, h->stream);
+        if (!rc && h->gqa_heads) {                    /* a page's scales and bounds are byte runs of their own */
+            rc = ct_kv_paged_move_pages(h->pool, NULL, new_pool, NULL, h->stage_dev, n_live, h->page_bytes, P, h->stream);
+            if (!rc && h->scales)
+                rc = ct_kv_paged_move_pages(h->scales, NULL, new_scales, NULL, h->stage_dev, n_live, sc_row * sizeof(float), P,
+                                            h->stream);
+            if (!rc && h->bounds)
+                rc = ct_kv_paged_move_pages(h->bounds, h->bound_scales, new_bounds, new_bscales, h->stage_dev, n_live, b_page,
+                                            h->gqa_heads, h->stream);
+        }
+        if (!rc) rc = ct__cuda_status(cudaMemcpyAsync(h->bt_dev, h->stage_dev + n_live, bt_n * sizeof(int32_t),
+                                                      cudaMemcpyDeviceToDevice, h->stream), "compact bt");
+        /* the staging buffer is reused by the next call on the host */
+        const int synced = ct__cuda_status(cudaStreamSynchronize(h->stream), "compact sync");
+        if (!rc) rc = synced;
+        if (rc) {
+            if (new_pool) cudaFreeAsync(new_pool, h->stream);
+            if (new_scales) cudaFreeAsync(new_scales, h->stream);
+            if (new_bounds) cudaFreeAsync(new_bounds, h->stream);
+            if (new_bscales) cudaFreeAsync(new_bscales, h->stream);
+            free(new_id); free(map); free(refc2);
+            return rc;
+        }
+        if (h->pool_async) {                          /* from an earlier compaction: back to the cache */
+            cudaFreeAsync(h->pool, h->stream);
+            if (h->scales) cudaFreeAsync(h->scales, h->stream);
+            if (h->bounds) { cudaFreeAsync(h->bounds, h->stream); cudaFreeAsync(h->bound_scales, h->stream); }
+        } else {                                      /* the create-time buffers */
+            cudaFree(h->pool);
+            cudaFree(h->scales);
+            cudaFree(h->bounds);
+            cudaFree(h->bound_scales);
+        }
+        h->pool_async = 1;
+        h->pool = new_pool;
+        h->scales = new_scales;
+        h->bounds = new_bounds;
+        h->bound_scales = new_bscales;
     }
-    if (!rc) rc = ct__cuda_status(cudaMemcpyAsync(h->bt_dev, h->stage_dev + n_live, (size_t)S * MP * sizeof(int32_t),
-                                                  cudaMemcpyDeviceToDevice, h->stream), "compact bt");
-    if (rc) {
-        if (new_pool) cudaFreeAsync(new_pool, h->stream);
-        if (new_scales) cudaFreeAsync(new_scales, h->stream);
-        if (new_bounds) cudaFreeAsync(new_bounds, h->stream);
-        if (new_bscales) cudaFreeAsync(new_bscales, h->stream);
-        cudaStreamSynchronize(h->stream);
-        return rc;
-    }
-    if (h->pool_async) {                          /* from an earlier compaction: back to the cache */
-        cudaFreeAsync(h->pool, h->stream);
-        if (h->scales) cudaFreeAsync(h->scales, h->stream);
-        if (h->bounds) { cudaFreeAsync(h->bounds, h->stream); cudaFreeAsync(h->bound_scales, h->stream); }
-    }
-    /* the staging buffer is reused by the next call on the host */
-    rc = ct__cuda_status(cudaStreamSynchronize(h->stream), "compact sync");
-    if (rc) return rc;
-    if (!h->pool_async) {                         /* the create-time buffers */
-        cudaFree(h->pool);
-        cudaFree(h->scales);
-        cudaFree(h->bounds);
-        cudaFree(h->bound_scales);
-    }
-    h->pool_async = 1;
-    h->pool = new_pool;
-    h->scales = new_scales;
-    h->bounds = new_bounds;
-    h->bound_scales = new_bscales;
-renumbered:
+    for (size_t i = 0; i < bt_n; i++)
+        if (h->bt[i] >= 0) h->bt[i] = new_id[h->bt[i]];
+    memcpy(h->refc, refc2, (size_t)NP * sizeof(uint32_t));
+    free(new_id); free(map); free(refc2);
     /* Free pages are now n_live..NP-1, handed out in ascending order. */
     for (uint32_t p = 0; p < NP; p++) h->rank[p] = p;
     h->heap_n = 0;

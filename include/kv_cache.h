@@ -183,7 +183,8 @@ int  ct_kv_paged_free_seq(ct_kv_paged_t *h, uint32_t seq);
 /* Frees up to n pages by LRU order; returns the number freed (>= 0). */
 int  ct_kv_paged_evict_lru(ct_kv_paged_t *h, uint32_t n);
 /* Renumbers live pages to 0..n_live-1 in (seq, lpage) order and moves their
- * bytes to match (device gather into a fresh pool). */
+ * bytes to match (device gather into a fresh pool).  On an error (no room for
+ * that pool, say) the handle stays as it was. */
 int  ct_kv_paged_compact(ct_kv_paged_t *h);
 
 /* Copies n tokens [start, start+n) of a sequence to out (device) as

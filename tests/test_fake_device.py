@@ -116,3 +116,41 @@ def test_an_error_is_reported_once(fake):
         assert h.append([0, 1], [1, 1]) == 0
         h.check()
     h.close()
+
+
+@pytest.mark.parametrize("gqa", [False, True])
+@pytest.mark.parametrize("again", [False, True])
+def test_a_compaction_that_fails_changes_nothing(fake, gqa, again):
+    """Each device call of a compaction fails once; afterwards the handle reads, appends and compacts as if it had not begun."""
+    for k in range(1, 40):
+        live = fake.fake_live()
+        h = Handle(fake, gqa)
+        order = np.random.default_rng(k).permutation(h.NP).astype(np.int32)
+        assert fake.ct_kv_paged_set_free_order(h.h, order.ctypes.data) == 0
+        assert h.append([0, 1, 2], [40, 17, 64]) == 0 and h.fork(2, 3, 37) == 0
+        if again:                                     # buffers of an earlier compaction
+            assert fake.ct_kv_paged_compact(h.h) == 0
+            assert fake.ct_kv_paged_free_seq(h.h, 1) == 0
+            h.rows[1] = h.rows[1][:0]
+        h.check()
+        held, before = fake.fake_live(), h.table()
+        fake.fake_fail(k)
+        rc = fake.ct_kv_paged_compact(h.h)
+        failed = fake.fake_pending() < 0
+        fake.fake_fail(-1)
+        assert (rc != 0) == failed
+        if failed:
+            assert rc == ct.CT_ERR_CUDA and np.array_equal(h.table(), before) and fake.fake_live() <= held
+            assert fake.ct_kv_paged_stats(h.h).n_compactions == again
+        h.check()
+        assert h.append([1, 3], [20, 30]) == 0
+        h.check()
+        assert fake.ct_kv_paged_compact(h.h) == 0
+        h.check()
+        t = h.table()
+        assert sorted(set(t[t >= 0].tolist())) == list(range(len(set(t[t >= 0].tolist()))))
+        h.close()
+        assert fake.fake_live() == live
+        if not failed:
+            break
+    assert not failed and k > 4
