@@ -28,6 +28,9 @@ struct ct_gqa_plan {
 
 static int misaligned(const void *p, uintptr_t n) { return ((uintptr_t)p & (n - 1)) != 0; }
 
+/* The kernels count a row's entries in 32 bits, a block of threads at a time. */
+static const uint32_t kMostSelected = 0x7FFFFFFFu;
+
 static int bad(const char *msg) {
     ct__set_error(msg);
     return CT_ERR_ARG;
@@ -259,7 +262,7 @@ int ct_attn_gqa_decode_selected(ct_gqa_plan_t *plan, const void *q, uint64_t q_s
                                 const int32_t *block_table, const int32_t *seq_lens, const int32_t *pages, uint32_t n_select,
                                 void *out, float *lse, void *stream) {
     if (!plan) return bad("gqa: no plan");
-    if (!pages || n_select == 0) return bad("gqa: no page list");
+    if (!pages || n_select == 0 || n_select > kMostSelected) return bad("gqa: no page list, or one too long");
     return decode(plan, q, q_stride, pool, scales, block_table, seq_lens, pages, n_select, out, lse, stream);
 }
 
@@ -272,6 +275,7 @@ int ct_attn_gqa_select_pages(ct_gqa_plan_t *plan, const void *q, uint64_t q_stri
     if (rc) return rc;
     if (!bounds || misaligned(bounds, 16) || !bound_scales || !block_table || !seq_lens || !pages_out)
         return bad("gqa: bounds (16-byte aligned), table, lengths or pages");
+    if (n_select > kMostSelected) return bad("gqa: n_select (at most 2^31 - 1)");
     if (n_select == 0 || (uint64_t)n_first + n_last > n_select) return bad("gqa: n_first + n_last > n_select, or nothing to select");
     if (l->max_pages_per_seq > ct__gqa_select_max_pages()) {
         ct__set_error("gqa: max_pages_per_seq is beyond the page selection");

@@ -226,7 +226,7 @@ int ct_attn_gqa_decode_paged(ct_gqa_plan_t *plan, const void *q, uint64_t q_stri
  *   e = max|q| / 127,  c = rint(q / e),  hi, lo, s: the page's bounds,
  * whole-number sums and single fp32 roundings, so the choice is the same on
  * every run.  A score that is not a number counts as infinity.  n_first +
- * n_last <= n_select; max_pages_per_seq at most 49152 (else
+ * n_last <= n_select < 2^31; max_pages_per_seq at most 49152 (else
  * CT_ERR_UNSUPPORTED). */
 int ct_attn_gqa_select_pages(ct_gqa_plan_t *plan, const void *q, uint64_t q_stride, const int8_t *bounds,
                              const float *bound_scales, const int32_t *block_table, const int32_t *seq_lens, uint32_t n_select,

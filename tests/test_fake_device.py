@@ -154,3 +154,17 @@ def test_a_compaction_that_fails_changes_nothing(fake, gqa, again):
         if not failed:
             break
     assert not failed and k > 4
+
+
+def test_page_lists_of_any_length_are_refused_or_end(fake):
+    """Entries of a row are counted in 32 bits by 256 threads, so lists that long are refused, not written without an end."""
+    lay = ct.GqaLayout(1, 32, 16, ct.CT_KV_BF16, 4, 4)
+    shape = ct.GqaShape(lay, 1, 0, 0, 0.0)
+    plan = fake.ct_gqa_plan_create(C.byref(shape), 1, 0)
+    a = 4096                                          # never read: the fake device computes nothing
+    for n, rc in ((1, 0), (1 << 20, 0), (0x7FFFFFFF, 0), (0x80000000, ct.CT_ERR_ARG), (0xFFFFFFFF, ct.CT_ERR_ARG)):
+        runs = fake.fake_runs()
+        assert fake.ct_attn_gqa_select_pages(plan, a, 0, a, a, a, a, n, 0, 0, a, None) == rc, n
+        assert fake.ct_attn_gqa_decode_selected(plan, a, 0, a, None, a, a, a, n, a, None, None) == rc, n
+        assert fake.fake_runs() == runs + (2 if rc == 0 else 0)
+    fake.ct_gqa_plan_destroy(plan)
