@@ -1284,14 +1284,26 @@ ct_kv_paged_t *ct_kv_paged_load(const char *path, int device) {
             free(len32);
         }
     }
-    if (!bad && h->bounds) {                           /* the bounds of every mapped page */
+    if (!bad && h->bounds) {                           /* the bounds of every mapped page, once: a shared one is full */
         uint32_t *all = (uint32_t *)malloc((size_t)S * 4), *from = (uint32_t *)calloc(S, 4);
-        touched_t tp;
+        uint8_t *listed = (uint8_t *)calloc(NP, 1);
+        touched_t tp = {NULL, NULL, 0};
         int32_t *mem = NULL;
         for (uint32_t i = 0; all && i < S; i++) all[i] = i;
-        bad = !all || !from || touched_pages(h, all, from, S, &tp, &mem) != CT_OK ||
-              flush_all(h, NULL, 0, NULL, 0, NULL, NULL, &tp) != CT_OK;
-        free(all); free(from); free(mem);
+        bad = !all || !from || !listed || touched_pages(h, all, from, S, &tp, &mem) != CT_OK;
+        if (!bad) {
+            int32_t *counts = mem + (tp.counts - tp.pages);
+            uint32_t n = 0;
+            for (uint32_t i = 0; i < tp.n; i++) {
+                if (listed[mem[i]]) continue;
+                listed[mem[i]] = 1;
+                mem[n] = mem[i];
+                counts[n++] = counts[i];
+            }
+            tp.n = n;
+            bad = flush_all(h, NULL, 0, NULL, 0, NULL, NULL, &tp) != CT_OK;
+        }
+        free(all); free(from); free(listed); free(mem);
     }
     if (bad) { ct_kv_paged_destroy(h); return NULL; }
     return h;

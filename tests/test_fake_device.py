@@ -168,3 +168,20 @@ def test_page_lists_of_any_length_are_refused_or_end(fake):
         assert fake.ct_attn_gqa_decode_selected(plan, a, 0, a, None, a, a, a, n, a, None, None) == rc, n
         assert fake.fake_runs() == runs + (2 if rc == 0 else 0)
     fake.ct_gqa_plan_destroy(plan)
+
+
+def test_a_shared_page_gets_its_bounds_once_when_loaded(fake, tmp_path):
+    """A checkpoint of forked sequences: every mapped page once in the call that makes the bounds, however many sequences map it
+    (one block a listed page and head: entries of all tables would pass what a launch takes)."""
+    h = Handle(fake, True)
+    assert h.append([0], [7 * h.P + 3]) == 0
+    for s in (1, 2, 3):
+        assert h.fork(0, s, 7 * h.P + s - 1) == 0
+    assert fake.ct_kv_paged_save(h.h, str(tmp_path / "f.bin").encode()) == 0
+    back = Handle(fake, True)
+    back.close()
+    back.h, back.rows = fake.ct_kv_paged_load(str(tmp_path / "f.bin").encode(), 0), h.rows
+    back.check()
+    assert fake.fake_listed() == len(set(back.table()[back.table() >= 0].tolist())) == 10 and fake.fake_listed_twice() == 0
+    back.close()
+    h.close()
