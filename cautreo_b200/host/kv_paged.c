@@ -276,6 +276,8 @@ static ct_kv_paged_t *create_impl(const ct_kv_paged_config_t *cfg, uint32_t gqa_
     if (!rc && h->scales)
         rc = ct__cuda_status(cudaMemset(h->scales, 0, (size_t)NP * P * h->scale_rows * sizeof(float)), "ct_kv_paged_create");
     if (!rc) rc = ct__cuda_status(cudaEventCreateWithFlags(&h->stage_ev, cudaEventDisableTiming), "ct_kv_paged_create");
+    /* the stream that the handle is given next need not wait for the default one */
+    if (!rc) rc = ct__cuda_status(cudaStreamSynchronize(NULL), "ct_kv_paged_create");
     if (rc) { ct_kv_paged_destroy(h); return NULL; }
     return h;
 }
@@ -1305,6 +1307,7 @@ ct_kv_paged_t *ct_kv_paged_load(const char *path, int device) {
         }
         free(all); free(from); free(listed); free(mem);
     }
+    if (!bad && !h->host_only) bad = ct__cuda_status(cudaStreamSynchronize(h->stream), "ct_kv_paged_load") != CT_OK;
     if (bad) { ct_kv_paged_destroy(h); return NULL; }
     return h;
 }

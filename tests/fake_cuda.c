@@ -16,12 +16,14 @@
 #include "../include/hal.h"
 #include "../include/kv_cache.h"
 
-static long g_countdown = -1, g_live;
+static long g_countdown = -1, g_live, g_unfinished;
 static cudaError_t g_last;
 
 void fake_fail(long n) { g_countdown = n; }
 long fake_pending(void) { return g_countdown; }
 long fake_live(void) { return g_live; }
+/* Device work since the last wait for the device: on a GPU it may still be running. */
+long fake_unfinished(void) { return g_unfinished; }
 
 static cudaError_t step(void) {
     if (g_countdown > 0 && --g_countdown == 0) { g_countdown = -1; return g_last = cudaErrorMemoryAllocation; }
@@ -50,7 +52,7 @@ cudaError_t cudaGetDevice(int *d) { *d = 0; return cudaSuccess; }
 cudaError_t cudaSetDevice(int d) { return d == 0 ? cudaSuccess : (g_last = cudaErrorInvalidDevice); }
 cudaError_t cudaGetDeviceProperties_v2(struct cudaDeviceProp *p, int d) { memset(p, 0, sizeof *p); return cudaSuccess; }
 cudaError_t cudaDeviceGetAttribute(int *v, enum cudaDeviceAttr a, int d) { *v = 148; return cudaSuccess; }
-cudaError_t cudaDeviceSynchronize(void) { return cudaSuccess; }
+cudaError_t cudaDeviceSynchronize(void) { g_unfinished = 0; return cudaSuccess; }
 cudaError_t cudaMalloc(void **p, size_t n) { return take(p, n); }
 cudaError_t cudaMallocHost(void **p, size_t n) { return take(p, n); }
 cudaError_t cudaMallocAsync(void **p, size_t n, cudaStream_t s) { return take(p, n); }
@@ -63,6 +65,7 @@ cudaError_t cudaMemPoolDestroy(cudaMemPool_t m) { return cudaSuccess; }
 cudaError_t cudaMemPoolSetAttribute(cudaMemPool_t m, enum cudaMemPoolAttr a, void *v) { return cudaSuccess; }
 cudaError_t cudaMemcpy(void *d, const void *s, size_t n, enum cudaMemcpyKind k) {
     const cudaError_t e = step();
+    g_unfinished++;
     if (!e) memcpy(d, s, n);
     return e;
 }
@@ -74,13 +77,14 @@ cudaError_t cudaMemcpy2DAsync(void *d, size_t dp, const void *s, size_t sp, size
 }
 cudaError_t cudaMemset(void *d, int v, size_t n) {
     const cudaError_t e = step();
+    g_unfinished++;
     if (!e) memset(d, v, n);
     return e;
 }
 cudaError_t cudaMemsetAsync(void *d, int v, size_t n, cudaStream_t st) { return cudaMemset(d, v, n); }
 cudaError_t cudaStreamCreateWithFlags(cudaStream_t *s, unsigned f) { *s = NULL; return step(); }
 cudaError_t cudaStreamDestroy(cudaStream_t s) { return cudaSuccess; }
-cudaError_t cudaStreamSynchronize(cudaStream_t s) { return cudaSuccess; }
+cudaError_t cudaStreamSynchronize(cudaStream_t s) { g_unfinished = 0; return cudaSuccess; }
 cudaError_t cudaEventCreate(cudaEvent_t *e) { *e = NULL; return cudaSuccess; }
 cudaError_t cudaEventCreateWithFlags(cudaEvent_t *e, unsigned f) { *e = NULL; return step(); }
 cudaError_t cudaEventDestroy(cudaEvent_t e) { return cudaSuccess; }
@@ -92,6 +96,7 @@ cudaError_t cudaEventElapsedTime(float *ms, cudaEvent_t a, cudaEvent_t b) { *ms 
 
 static int launched(void) {
     step();
+    g_unfinished++;
     return ct__cuda_status(cudaGetLastError(), "launch");
 }
 

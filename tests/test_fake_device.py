@@ -31,7 +31,7 @@ def fake(tmp_path_factory):
             f = getattr(L, name)
             f.restype, f.argtypes = res, args
     L.fake_fail.argtypes = [C.c_long]
-    L.fake_pending.restype = L.fake_live.restype = C.c_long
+    L.fake_pending.restype = L.fake_live.restype = L.fake_unfinished.restype = C.c_long
     return L
 
 
@@ -184,4 +184,19 @@ def test_a_shared_page_gets_its_bounds_once_when_loaded(fake, tmp_path):
     back.check()
     assert fake.fake_listed() == len(set(back.table()[back.table() >= 0].tolist())) == 10 and fake.fake_listed_twice() == 0
     back.close()
+    h.close()
+
+
+@pytest.mark.parametrize("gqa", [False, True])
+def test_a_new_handle_leaves_nothing_running(fake, gqa, tmp_path):
+    """Creating and loading work on the default stream, which the stream that the handle is given next need not wait for: what
+    they set (zeroes, tables, bounds) is there when they return."""
+    h = Handle(fake, gqa)
+    assert fake.fake_unfinished() == 0
+    assert h.append([0, 1], [40, 17]) == 0 and fake.fake_unfinished() > 0
+    assert fake.ct_kv_paged_save(h.h, str(tmp_path / "f.bin").encode()) == 0
+    h.close()
+    h.h = fake.ct_kv_paged_load(str(tmp_path / "f.bin").encode(), 0)
+    assert fake.fake_unfinished() == 0
+    h.check()
     h.close()
