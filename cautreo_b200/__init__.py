@@ -533,7 +533,7 @@ class GqaKV(PagedKV):
 
 
 def gqa_write_slots(layout, pool, scales, k, v, dest_slot, n, src_dtype=CT_KV_BF16, k_stride=0, v_stride=0, stream=None):
-    """Write n tokens' K and V rows into a grouped-query pool (ct_kv_gqa_write_slots)."""
+    """Write n tokens' K and V rows into a grouped-query pool, each slot at most once (ct_kv_gqa_write_slots)."""
     rc = lib().ct_kv_gqa_write_slots(layout, _addr(pool), _addr(scales), _addr(k), _addr(v), k_stride, v_stride, src_dtype,
                                      _addr(dest_slot), n, stream)
     if rc:

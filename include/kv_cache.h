@@ -305,8 +305,11 @@ typedef struct {
 } ct_kv_gqa_layout_t;
 
 /* Writes K and V of n tokens to dest_slot[i] = page * page_tokens + slot
- * (device int32; outside the pool skips the token; a slot given twice gets
- * either token), converting / quantising.  Token i's K is k[i * k_stride]
+ * (device int32; outside the pool skips the token), converting / quantising.
+ * A slot of the pool is given at most once a call: its K and V heads, codes
+ * and scales are stored apart, so two tokens on one slot may leave a row that
+ * is neither's.  (ct_kv_paged_append_kv keeps the last token of a slot by
+ * itself.)  Token i's K is k[i * k_stride]
  * onwards, n_kv_heads x head_dim values of src_dtype (CT_KV_BF16 or
  * CT_KV_F32), its V at v[i * v_stride]; a stride (in values) of 0 selects
  * n_kv_heads x head_dim, so K and V may be columns of a fused projection.

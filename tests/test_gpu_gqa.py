@@ -937,3 +937,23 @@ def test_large_pages_append_compact_checkpoint_and_decode(dtype, page, tmp_path)
     same(back)
     back.compact()
     same(back)
+
+
+@pytest.mark.parametrize("dtype", [BF16, INT8, E4M3])
+def test_one_append_that_uses_pages_again_keeps_the_last_tokens(dtype):
+    """A call longer than the window frees pages and takes them again: a slot is written by its last token alone, K and V, codes
+    and scales."""
+    heads, dim, page, window = 3, 64, 16, 40
+    g = gen(93)
+    kv = ct.GqaKV(2, 64, 9, heads, dim, page, window_tokens=window, dtype=dtype, keep_bounds=True, stream=stream())
+    n = [700, 333]
+    x = rows(sum(n), heads, dim, g)
+    kv.append_kv([0, 1], n, x[0], x[1])
+    kept = [c - (c - window) // page * page for c in n]               # tokens of the pages that the window reaches
+    k, v = (torch.empty(sum(kept), heads * dim, device="cuda") for _ in range(2))
+    kv.gather_kv([0, 1], [c - m for c, m in zip(n, kept)], kept, k, v, ct.CT_KV_F32)
+    torch.cuda.synchronize()
+    for got, src in ((k, x[0]), (v, x[1])):
+        want = torch.cat((src[n[0] - kept[0]:n[0]], src[n[0] + n[1] - kept[1]:]))
+        assert torch.equal(got, stored_as(want, dtype, heads, dim))
+    check_bounds(kv, heads, dim, page, dtype)
