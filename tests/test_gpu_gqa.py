@@ -832,7 +832,7 @@ def test_calls_in_a_row_see_what_the_one_before_wrote(dtype):
     tables = torch.stack([torch.randperm(n_pages, generator=g, device="cuda").view(S, per) for _ in range(steps)]).to(torch.int32)
     lens_bank = torch.randint(1, 5 * page + 1, (steps, S), generator=g, device="cuda").to(torch.int32)
     t = torch.arange(page * 5, device="cuda")
-    slot_bank = (tables[:, :, t // page] * page + t % page).reshape(steps, n).contiguous()
+    slot_bank = (tables[:, :, t // page] * page + t % page).reshape(steps, n).to(torch.int32).contiguous()
 
     def run(wait):
         pool = torch.zeros(n_pages, 2, heads, page, dim, device="cuda",
