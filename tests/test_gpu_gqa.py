@@ -957,3 +957,112 @@ def test_one_append_that_uses_pages_again_keeps_the_last_tokens(dtype):
         want = torch.cat((src[n[0] - kept[0]:n[0]], src[n[0] + n[1] - kept[1]:]))
         assert torch.equal(got, stored_as(want, dtype, heads, dim))
     check_bounds(kv, heads, dim, page, dtype)
+
+
+# ---- what page bounds and scores are for ---------------------------------------------------------------------------------
+
+def rounded_queries(q):
+    """Whole-number codes of query heads [..., dim] and their steps, single 32-bit roundings; in 64 bits."""
+    x = q.float()
+    e = x.abs().amax(-1) / torch.full_like(x[..., 0], 127.0)
+    c = torch.where(e[..., None] > 0, torch.round(x / e[..., None]), torch.zeros_like(x)).clamp(-127, 127)
+    return c.double(), e.double()
+
+
+@pytest.mark.parametrize("dtype", [BF16, INT8, E4M3])
+@pytest.mark.parametrize("dim,page,group", [(32, 16, 1), (96, 48, 3), (128, 64, 4), (256, 128, 17)])
+def test_a_page_scores_no_less_than_any_of_its_keys(dim, page, group, dtype):
+    """The score of a page, from its stored bounds, against the product of the rounded query with every key of the page, and the
+    pages left out against those chosen.
+
+    s and y = b / s are single roundings, and codes are clamped only where |b| is the page's largest value, so a bound times s
+    falls short of its b by at most (2^-24 + 2^-24) times that largest value `top`, and a product of `dim` terms by that times
+    sum |c| e; twice as much is allowed.  The kernel's score rounds twice more: 2^-23 of it, twice that allowed."""
+    g = gen(dim + group + dtype)
+    heads, n_pages, pick = 2, 40, 9
+    hq, width = heads * group, heads * dim
+    layout = ct.GqaLayout(heads, dim, page, dtype, n_pages, n_pages)
+    pool, scales = G.make_pool(n_pages, heads, page, dim, dtype, g)
+    n = n_pages * page - 5
+    x = torch.randn(n, 2 * width, generator=g, device="cuda")
+    x[:, :width] = x[:, :width] * (torch.rand(width, generator=g, device="cuda") * 3 + 0.1) + torch.randn(width, generator=g, device="cuda")
+    x[torch.rand(n, generator=g, device="cuda") < 0.02] *= 20.0
+    x = x.bfloat16()
+    table = torch.randperm(n_pages, generator=g, device="cuda").to(torch.int32).view(1, n_pages)
+    t = torch.arange(n, device="cuda")
+    slots = (table[0, t // page] * page + t % page).to(torch.int32)
+    ct.gqa_write_slots(layout, pool, scales, x, x[:, width:], slots, n, k_stride=2 * width, v_stride=2 * width, stream=stream())
+    bounds = torch.zeros(n_pages, heads, 2, dim, dtype=torch.int8, device="cuda")
+    bs = torch.zeros(n_pages, heads, device="cuda")
+    counts = torch.full((n_pages,), page, dtype=torch.int32, device="cuda")
+    counts[-1] = page - 5
+    ct.gqa_page_bounds(layout, pool, scales, table, counts, n_pages, bounds, bs, stream=stream())
+    q = torch.randn(1, hq, dim, generator=g, device="cuda").bfloat16()
+    plan = ct.GqaPlan(layout, 1, hq, head_order=BLK)
+    picked = torch.zeros(1, heads, pick, dtype=torch.int32, device="cuda")
+    lens = torch.tensor([n], dtype=torch.int32, device="cuda")
+    plan.select(q, bounds, bs, table, lens, picked, pick, 1, 1, stream=stream())
+    torch.cuda.synchronize()
+    code, e = rounded_queries(q.view(heads, group, dim))
+    for h in range(heads):
+        at = table[0].long()
+        keys = G.values(pool[at, 0, h], None if scales is None else scales[at, 0, h], dtype)          # [page][slot][dim]
+        live = (torch.arange(page, device="cuda")[None] < counts[:, None])
+        keys = torch.where(live[..., None], keys, torch.zeros_like(keys))
+        product = torch.einsum("gd,ptd->gpt", code[h] * e[h][:, None], keys).masked_fill(~live[None], float("-inf"))
+        hi, lo = bounds[at, h, 0].double(), bounds[at, h, 1].double()
+        score = (code[h].clamp(min=0) @ hi.T + code[h].clamp(max=0) @ lo.T) * e[h][:, None] * bs[at, h].double()[None]
+        top = keys.abs().amax((1, 2))
+        short = 2.0 ** -22 * top[None] * (code[h].abs().sum(-1) * e[h])[:, None]
+        assert (product.amax(-1) <= score + short).all()
+        best = score.amax(0)
+        chosen = torch.zeros(n_pages, dtype=torch.bool, device="cuda")
+        chosen[picked[0, h].long()] = True
+        free = chosen.clone()
+        free[0] = free[-1] = False
+        assert int(chosen.sum()) == pick and bool(chosen[0]) and bool(chosen[-1])
+        least = best[free].min()
+        assert (best[~chosen] <= least + 2.0 ** -22 * best.abs().max()).all()
+        limit = least + 2.0 ** -22 * best.abs().max() + short.amax(0)[~chosen]
+        assert (product.amax(-1).amax(0)[~chosen] <= limit).all()
+
+
+@pytest.mark.parametrize("dtype", [BF16, INT8, E4M3])
+def test_chosen_pages_hold_the_weight(dtype):
+    """Three keys a query head point along it, in pages anywhere; the other 3188 are short.  With logits of 3 |q|^2 / sqrt(128)
+    (at least 18 where |q|^2 >= 68, five deviations below its mean) against others whose exponentials sum to less than 2^13,
+    the pages left out hold less than 2^13 e^-18 < 2^-12 of the softmax; the decode over the chosen ones then differs from the
+    whole by at most twice that of the values, besides each one's own rounding."""
+    g = gen(95)
+    heads, group, dim, page, n_pages, pick = 2, 4, 128, 16, 200, 16
+    hq, width, n = heads * group, heads * dim, 200 * 16
+    q = torch.randn(1, hq, dim, generator=g, device="cuda").bfloat16()
+    assert float(q.float().square().sum(-1).min()) >= 68
+    x = torch.randn(2, n, heads, dim, generator=g, device="cuda") * 0.3
+    where = torch.randperm(n, generator=g, device="cuda")[:3 * group * heads].view(heads, group, 3)
+    for h in range(heads):
+        for i in range(group):
+            x[0, where[h, i], h] = 3.0 * q[0, i * heads + h].float()
+    x = x.view(2, n, width).bfloat16()
+    kv = ct.GqaKV(1, n_pages, n_pages, heads, dim, page, dtype=dtype, keep_bounds=True, stream=stream())
+    kv.set_free_order(np.random.default_rng(8).permutation(n_pages))
+    kv.append_kv([0], [n], x[0], x[1])
+    plan = ct.GqaPlan(kv.layout, 1, hq)
+    picked = torch.zeros(1, heads, pick, dtype=torch.int32, device="cuda")
+    out, sel = (torch.empty(1, hq, dim, device="cuda").bfloat16() for _ in range(2))
+    plan.select(q, kv.bounds, kv.bound_scales, kv.block_table_dev, kv.seq_lens_dev, picked, pick, stream=stream())
+    plan.decode(q, kv.pool, kv.scales, kv.block_table_dev, kv.seq_lens_dev, out, stream=stream())
+    plan.decode_selected(q, kv.pool, kv.scales, kv.block_table_dev, kv.seq_lens_dev, picked, pick, sel, stream=stream())
+    k = torch.empty(2, n, width, device="cuda")
+    kv.gather_kv([0], [0], [n], k[0], k[1], ct.CT_KV_F32)
+    torch.cuda.synchronize()
+    k = k.double().view(2, n, heads, dim)
+    for h in range(heads):
+        pages = picked[0, h].long()
+        assert set((where[h] // page).flatten().tolist()) <= set(pages.tolist())
+        held = torch.isin(torch.arange(n, device="cuda") // page, pages)
+        for i in range(group):
+            p = torch.softmax(k[0, :, h] @ q[0, i * heads + h].double() / dim ** 0.5, 0)
+            assert float(p[~held].sum()) <= 2.0 ** -12
+    gap = (out.double() - sel.double()).abs()
+    assert (gap <= 2 * 2.0 ** -12 * k[1].abs().max() + 3 * 2.0 ** -8 * out.double().abs().clamp(min=2.0 ** -4)).all()
