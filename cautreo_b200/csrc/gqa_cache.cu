@@ -25,7 +25,8 @@ namespace {
 
 constexpr int kThreads = 256;
 
-/* Lanes that share a row, 8 values each: the power of two >= D / 8. */
+/* Lanes that share a row, 8 values each: the power of two >= D / 8, so that a
+ * row's maximum is reduced by shuffles (a quarter of them idle at 96 and 192). */
 __host__ __device__ constexpr int lanes_of(int D) { return D <= 32 ? 4 : D <= 64 ? 8 : D <= 128 ? 16 : 32; }
 
 CT_DEV uint32_t pack2_bf16(float lo, float hi) {
@@ -38,9 +39,9 @@ CT_DEV uint32_t pack2_bf16(float lo, float hi) {
  * consecutive slots as one contiguous run.  A thread moves 8 values of T
  * tokens; all its loads are in flight before the first is used, and the lanes
  * of a row find the tokens' rows once between them.  Bound by HBM in large
- * calls (16384 tokens, 8 heads of 128, bf16 -> int8 18.5 us, 5.5 TB/s of bytes
- * read and written; read back at once, the pool still in L2, 12), by the
- * launch in small ones (64 tokens with their pages' bounds 4.5 to 5 us). */
+ * calls (16384 tokens, 8 heads of 128, bf16 -> int8 18.2 us, 5.6 TB/s of bytes
+ * read and written; read back 18.7, at once, the pool still in L2, 11.5), by
+ * the launch in small ones (64 tokens with their pages' bounds 5 us). */
 
 /* Row of the pool for a token's slot, or kNoRow. */
 constexpr size_t kNoRow = ~(size_t)0;
@@ -420,9 +421,12 @@ __global__ void __launch_bounds__(kBoundThreads) k_gqa_bounds(const void *pool, 
         default: return CT_ERR_UNSUPPORTED;        \
     }
 
-/* Tokens a thread moves: 4 when the call fills the GPU with them, else 1 (8
- * heads of 128, bf16 -> int8: 64 tokens in ones 1.7 us, in fours 2.4; 2048
- * 4.5, 5.0; 4096 8.0, 6.9; 16384 27.6, 20.7). */
+/* Tokens a thread moves: 4 when the call fills the GPU with them, else 1.
+ * Write, read back in us, in ones and in fours: 8 heads of 128, bf16 -> int8,
+ * 64 tokens 1.4, 1.5 and 1.9, 1.8; 2048 4.2, 3.4 and 4.2, 3.3; 4096 7.1, 5.7
+ * and 6.1, 4.5; 16384 24.7, 24.1 and 18.2, 18.4; 5 heads of 96, fp32 <-> e4m3,
+ * 2560 tokens 3.6, 3.4 and 3.6, 4.7; 4096 5.4, 4.7 and 5.2, 6.3; 16384 16.7,
+ * 18.8 and 15.0, 17.0.  The limit lies between 4096 x 5 and 4096 x 8. */
 inline bool many(uint32_t n, uint32_t heads) { return (uint64_t)n * heads >= 24576; }
 
 struct WriteCall {

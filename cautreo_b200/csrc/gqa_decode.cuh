@@ -9,9 +9,9 @@
  * domain; a maximum is only followed when it grows by more than 2^3, so the
  * accumulators are rescaled a few times per sequence.
  *
- * Bound: HBM.  A token of a head is 4 D bytes (bf16) for 4 G D flops, G <= 16
- * query heads sharing it: 16 flops a byte at most, a fourteenth of the
- * ridge of the tensor cores.  So K and V go through cp.async into shared
+ * Bound: HBM.  A token of a head is 4 D bytes (bf16; 2 (D + 4) in 8 bits) for
+ * 4 G D flops, G <= 16 query heads sharing it: at most 16 flops a byte (31 in
+ * 8 bits), a sixteenth (an eighth) of the ridge of the tensor cores.  So K and V go through cp.async into shared
  * memory and ldmatrix into mma.sync m16n8k16 with 16 tokens (for the scores)
  * or 16 values of a head (for the output) as the rows and 8 query heads of
  * the group as the columns: a group of up to 8 heads wastes nothing on rows,
@@ -19,9 +19,9 @@
  * further items.  Scores come out as [token][head] and are needed as
  * [token][head] operands: two movmatrix per 16 tokens.
  * Measured, 8 kv heads of 4 query heads, 128 values: 32 sequences of 4096
- * tokens, bf16 94 us (5.7 TB/s), int8 54 us (5.1 TB/s); 64 of 8192 bf16 341 us
- * (6.3 TB/s); one of 777 tokens 8.2 us, most of it the launch, the dependent
- * loads up to the first tokens and the join.
+ * tokens, bf16 95 us (5.6 TB/s), int8 54 us (5.1 TB/s); 64 of 8192 bf16 350 us
+ * (6.1 TB/s), int8 193 (5.7); one of 777 tokens 8.1 us, of 64 (which no two
+ * CTAs share) 4.4, of none 4.1.
  *
  * bf16 pools: probabilities enter as two bf16 digits (one would add an error
  * as large as the rounding of the output).  8-bit pools: codes are widened to

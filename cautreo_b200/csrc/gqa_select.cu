@@ -11,9 +11,11 @@
  * single fp32 roundings, so the chosen pages do not depend on how the sums
  * are split (ties go to the lowest page).
  *
- * Bound: HBM, 2 D + 4 bytes a page and head, while the scores are made (up to
- * 1024 pages of 64 sequences, 8 heads of 128: 11 of 26.8 us at 6.4 TB/s);
- * latency of the rounding, the select and the launch for the rest.  A CTA per
+ * Bound: HBM, 2 D + 4 bytes a page and head, while the scores are made, and
+ * latency of the launch, the rounding and the select: 64 sequences of 16 to
+ * 1024 pages, 8 heads of 128, take 27 us, 10.7 of them for the bytes, 3 what a
+ * call costs that has nothing to choose, 6 for rows of unequal length (21 us
+ * for as many pages in rows of 512).  A CTA per
  * (sequence, kv head), or a cluster of up to 8 when the batch has few: its
  * warps take 16 pages at a time, as the rows of mma.sync m16n8k32 (int8), 8
  * heads of the group being the columns, with the next pages' numbers loaded
@@ -52,7 +54,9 @@ CT_DEV uint32_t key_of(float x) {
     return (u >> 31) ? ~u : u | 0x80000000u;
 }
 
-template <int D> constexpr uint32_t kResident = D <= 128 ? 4 : 2;         /* CTAs an SM holds */
+/* CTAs an SM holds; four leave 64 registers a thread, which spills 32 bytes at
+ * D = 128 (8 at 96, 4 at 64). */
+template <int D> constexpr uint32_t kResident = D <= 128 ? 4 : 2;
 
 template <int D>
 __global__ void __launch_bounds__(kThreads, kResident<D>) k_gqa_select(const ct_gqa_select_args_t a) {
