@@ -213,7 +213,10 @@ size_t         ct_gqa_plan_scratch_bytes(const ct_gqa_plan_t *p);
  * seq_lens: device [n_seq].  out: device bf16 [n_seq][n_q_heads][head_dim],
  * 8-byte aligned; lse (optional, device fp32 [n_seq][n_q_heads]): the
  * natural-log softmax normaliser.  A sequence without tokens gives 0 and
- * -inf.  Slots behind a sequence's end may hold anything. */
+ * -inf.  Slots behind a sequence's end may hold anything.  8-bit pools: the
+ * weights of the likeliest tokens keep 11 bits where their V scales are 2^-25
+ * of the largest of the sequence and head or more (fewer below), query values
+ * all of theirs where they are 2^-29 of their head's largest or more. */
 int ct_attn_gqa_decode_paged(ct_gqa_plan_t *plan, const void *q, uint64_t q_stride, const void *pool, const float *scales,
                              const int32_t *block_table, const int32_t *seq_lens, void *out, float *lse, void *stream);
 

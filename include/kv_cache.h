@@ -330,7 +330,7 @@ int ct_kv_gqa_read_slots(const ct_kv_gqa_layout_t *layout, const void *pool, con
  * hi_d / lo_d = the largest / smallest k_d, s = max(|hi|, |lo|) / 127, codes
  * ceil(hi / s) and floor(lo / s).  A NaN or an infinity among the keys gives
  * scale NaN (such a page counts as the highest score), no token scale 0.  A
- * page listed twice has one count. */
+ * page listed twice has to have the same count both times. */
 int ct_kv_gqa_page_bounds(const ct_kv_gqa_layout_t *layout, const void *pool, const float *scales, const int32_t *pages,
                           const int32_t *counts, uint32_t n, int8_t *bounds, float *bound_scales, void *stream);
 
