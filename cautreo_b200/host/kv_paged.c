@@ -81,7 +81,7 @@ struct ct_kv_paged {
     int32_t **tok;
     uint32_t *tok_n, *tok_cap;
     /* pending device updates of this call */
-    int32_t *pairs;             /* (index, value) for bt_dev then len_dev */
+    int32_t *pairs;             /* (index, value before) for bt_dev, then indices for len_dev */
     uint32_t n_bt_pairs, n_len_pairs, pairs_cap;
 };
 
@@ -132,14 +132,14 @@ static int pairs_reserve(ct_kv_paged_t *h, uint32_t extra) {
     return CT_OK;
 }
 
-/* bt pairs are stored from the front, len pairs are appended after the call
- * by flush (lengths are final only then). */
+/* bt pairs (index, value before) are stored from the front, len pairs are
+ * appended after the call by flush (lengths are final only then). */
 static int set_bt(ct_kv_paged_t *h, uint32_t s, uint32_t lp, int32_t v) {
     size_t idx = (size_t)s * h->cfg.max_pages_per_seq + lp;
-    h->bt[idx] = v;
     if (pairs_reserve(h, 1)) return CT_ERR_NOMEM;
     h->pairs[2 * h->n_bt_pairs] = (int32_t)idx;
-    h->pairs[2 * h->n_bt_pairs + 1] = v;
+    h->pairs[2 * h->n_bt_pairs + 1] = h->bt[idx];
+    h->bt[idx] = v;
     h->n_bt_pairs++;
     return CT_OK;
 }
@@ -378,9 +378,10 @@ typedef struct {
 /* Uploads n_dest token slots plus the pending bt / len (index, value) pairs
  * in one pinned staging copy, then runs the scatters and the token writes
  * (entries copied, or projected when pj is set, or K and V of kv), and makes
- * the bounds of the touched pages. */
+ * the bounds of the touched pages.  *wrote (may be NULL): whether the token
+ * writes are on their way. */
 static int flush_all(ct_kv_paged_t *h, const int32_t *dest, uint32_t n_dest, const void *entries, uint32_t src_dtype,
-                     const proj_args_t *pj, const kv_args_t *kv, const touched_t *tp) {
+                     const proj_args_t *pj, const kv_args_t *kv, const touched_t *tp, int *wrote) {
     const size_t n_pairs = (size_t)h->n_bt_pairs + h->n_len_pairs;
     const size_t n_tp = tp && h->bounds ? tp->n : 0;
     const size_t total = n_dest + 2 * n_pairs + 2 * n_tp;
@@ -426,6 +427,7 @@ static int flush_all(ct_kv_paged_t *h, const int32_t *dest, uint32_t n_dest, con
     else if (!rc && entries && n_dest)
         rc = ct_kv_paged_write_slots(h->pool, h->scales, h->cfg.dtype, entries, src_dtype, h->stage_dev, n_dest,
                                      h->cfg.entry_dim, h->stream);
+    if (wrote) *wrote = !rc && n_dest;
     if (!rc && n_tp)
         rc = ct__launch_gqa_bounds(h->pool, h->scales, h->cfg.dtype, h->gqa_heads, h->gqa_dim, h->cfg.page_tokens,
                                    h->cfg.n_pages, h->stage_dev + tp_at, h->stage_dev + tp_at + n_tp, (uint32_t)n_tp, h->bounds,
@@ -436,14 +438,13 @@ static int flush_all(ct_kv_paged_t *h, const int32_t *dest, uint32_t n_dest, con
 
 static int flush(ct_kv_paged_t *h, const int32_t *dest, uint32_t n_dest, const void *entries, uint32_t src_dtype,
                  const proj_args_t *pj) {
-    return flush_all(h, dest, n_dest, entries, src_dtype, pj, NULL, NULL);
+    return flush_all(h, dest, n_dest, entries, src_dtype, pj, NULL, NULL, NULL);
 }
 
 static int push_len(ct_kv_paged_t *h, uint32_t s) {
     if (pairs_reserve(h, 1)) return CT_ERR_NOMEM;
     uint32_t i = h->n_bt_pairs + h->n_len_pairs;
     h->pairs[2 * i] = (int32_t)s;
-    h->pairs[2 * i + 1] = (int32_t)h->len[s];
     h->n_len_pairs++;
     return CT_OK;
 }
@@ -476,6 +477,45 @@ static int touched_pages(const ct_kv_paged_t *h, const uint32_t *seq_ids, const 
     return CT_OK;
 }
 
+/* What an append that fails is taken back to; the table's entries are in the
+ * pending pairs, references and free pages follow from the table. */
+typedef struct {
+    uint64_t *last_access;      /* one allocation of all three */
+    uint32_t *lo, *hi;
+    ct_kv_paged_stats_t st;
+    uint32_t log_n;
+} saved_t;
+
+static int save_tables(const ct_kv_paged_t *h, saved_t *sv) {
+    const size_t S = h->cfg.n_seqs;
+    sv->last_access = (uint64_t *)malloc(S * 16);
+    if (!sv->last_access) return CT_ERR_NOMEM;
+    sv->lo = (uint32_t *)(sv->last_access + S);
+    sv->hi = sv->lo + S;
+    memcpy(sv->last_access, h->last_access, S * 8);
+    memcpy(sv->lo, h->lo, S * 4);
+    memcpy(sv->hi, h->hi, S * 4);
+    sv->st = h->st;
+    sv->log_n = h->log_n;
+    return CT_OK;
+}
+
+static void restore_tables(ct_kv_paged_t *h, const saved_t *sv, const uint32_t *seq_ids, const uint32_t *from, uint32_t n,
+                           uint32_t n_bt_pairs) {
+    const size_t S = h->cfg.n_seqs, bt_n = S * h->cfg.max_pages_per_seq;
+    for (uint32_t i = n_bt_pairs; i-- > 0;) h->bt[h->pairs[2 * i]] = h->pairs[2 * i + 1];
+    for (uint32_t i = 0; i < n; i++) h->len[seq_ids[i]] = from[i];
+    memcpy(h->last_access, sv->last_access, S * 8);
+    memcpy(h->lo, sv->lo, S * 4);
+    memcpy(h->hi, sv->hi, S * 4);
+    h->st = sv->st;
+    h->log_n = sv->log_n;
+    memset(h->refc, 0, (size_t)h->cfg.n_pages * sizeof(uint32_t));
+    for (size_t i = 0; i < bt_n; i++) if (h->bt[i] >= 0) h->refc[h->bt[i]]++;
+    h->heap_n = 0;
+    for (uint32_t p = 0; p < h->cfg.n_pages; p++) if (h->refc[p] == 0) heap_push(h, (int32_t)p);
+}
+
 static int append_impl(ct_kv_paged_t *h, const uint32_t *seq_ids, const uint32_t *counts, uint32_t n,
                        const void *entries, uint32_t src_dtype, const proj_args_t *pj, const kv_args_t *kv) {
     if (!h || (n && (!seq_ids || !counts))) return CT_ERR_ARG;
@@ -503,7 +543,8 @@ static int append_impl(ct_kv_paged_t *h, const uint32_t *seq_ids, const uint32_t
     size_t *off = (size_t *)malloc((n ? n : 1) * sizeof(size_t));
     int32_t *dest = (int32_t *)malloc((total ? total : 1) * sizeof(int32_t));
     uint32_t *from = (uint32_t *)malloc((n ? n : 1) * sizeof(uint32_t));
-    if (!off || !dest || !from) { free(off); free(dest); free(from); return CT_ERR_NOMEM; }
+    saved_t sv = {NULL, NULL, NULL, h->st, 0};
+    if (!off || !dest || !from || save_tables(h, &sv)) { free(off); free(dest); free(from); return CT_ERR_NOMEM; }
     for (uint32_t i = 0, acc = 0; i < n; i++) { off[i] = acc; acc += counts[i]; from[i] = h->len[seq_ids[i]]; }
     h->n_bt_pairs = h->n_len_pairs = 0;
 
@@ -566,23 +607,31 @@ static int append_impl(ct_kv_paged_t *h, const uint32_t *seq_ids, const uint32_t
         for (uint32_t i = 0; i < n; i++) if ((rc = push_len(h, seq_ids[i]))) break;
     free(off);
     h->st.n_pages_free = h->heap_n;
-    if (rc != CT_OK) {
-        /* Host state already advanced: publish what changed so the device
-         * mirrors stay consistent, but write no token data. */
-        flush(h, NULL, 0, NULL, 0, NULL);
-        free(dest);
-        free(from);
-        return rc;
-    }
     touched_t tp = {NULL, NULL, 0};
     int32_t *tp_mem = NULL;
-    if (kv && h->bounds) rc = touched_pages(h, seq_ids, from, n, &tp, &tp_mem);
-    /* Without entries only the tables change: the slots need not travel. */
-    const int rc2 = flush_all(h, dest, !rc && (entries || pj || kv) ? (uint32_t)total : 0u, entries, src_dtype, pj, kv, &tp);
+    if (!rc && kv && h->bounds) rc = touched_pages(h, seq_ids, from, n, &tp, &tp_mem);
+    const uint32_t n_bt = h->n_bt_pairs;
+    int wrote = 0, sent = 0;
+    if (!rc) {
+        /* Without entries only the tables change: the slots need not travel. */
+        rc = flush_all(h, dest, entries || pj || kv ? (uint32_t)total : 0u, entries, src_dtype, pj, kv, &tp, &wrote);
+        sent = 1;
+    }
+    if (rc && !wrote) {
+        /* No token was written, pages given up in the call among them: all is
+         * taken back, and published once more if some of it was sent. */
+        restore_tables(h, &sv, seq_ids, from, n, n_bt);
+        h->n_bt_pairs = sent ? n_bt : 0;
+        h->n_len_pairs = 0;
+        for (uint32_t i = 0; i < n && sent && push_len(h, seq_ids[i]) == CT_OK; i++) {}
+        if (sent) flush(h, NULL, 0, NULL, 0, NULL);
+        h->n_bt_pairs = h->n_len_pairs = 0;
+    }
     free(tp_mem);
     free(dest);
     free(from);
-    return rc ? rc : rc2;
+    free(sv.last_access);
+    return rc;
 }
 
 int ct_kv_paged_append(ct_kv_paged_t *h, const uint32_t *seq_ids, const uint32_t *counts, uint32_t n,
@@ -721,7 +770,7 @@ int ct_kv_paged_fork(ct_kv_paged_t *h, uint32_t src, uint32_t dst, uint32_t n_to
         if (rc) return rc;
         const int32_t count = (int32_t)rem;
         const touched_t tp = {&copy_to, &count, 1};
-        return flush_all(h, NULL, 0, NULL, 0, NULL, NULL, &tp);
+        return flush_all(h, NULL, 0, NULL, 0, NULL, NULL, &tp, NULL);
     }
     if (!h->host_only && copy_to >= 0) {             /* first rem slots of the page, and their scales */
         const size_t tok_bytes = h->page_bytes / P;
@@ -1303,7 +1352,7 @@ ct_kv_paged_t *ct_kv_paged_load(const char *path, int device) {
                 counts[n++] = counts[i];
             }
             tp.n = n;
-            bad = flush_all(h, NULL, 0, NULL, 0, NULL, NULL, &tp) != CT_OK;
+            bad = flush_all(h, NULL, 0, NULL, 0, NULL, NULL, &tp, NULL) != CT_OK;
         }
         free(all); free(from); free(listed); free(mem);
     }

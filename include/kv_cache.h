@@ -166,7 +166,10 @@ int  ct_kv_paged_set_free_order(ct_kv_paged_t *h, const int32_t *order_host);
  *   5. pages wholly outside the sliding window are freed.
  * entries: device [sum(counts)][entry_dim] in src_dtype (CT_KV_BF16 or
  * CT_KV_F32), ordered sequence by sequence (all tokens of seq_ids[0] first);
- * NULL reserves the slots and writes nothing. */
+ * NULL reserves the slots and writes nothing.  On an error (CT_ERR_FULL: no
+ * page can be freed, or a sequence's row is full) the call changes nothing,
+ * evictions on its way included; only the launch that makes the bounds of a
+ * grouped-query cache comes after the tokens are written. */
 int  ct_kv_paged_append(ct_kv_paged_t *h, const uint32_t *seq_ids, const uint32_t *counts,
                         uint32_t n, const void *entries, uint32_t src_dtype);
 

@@ -37,12 +37,12 @@ def fake(tmp_path_factory):
 
 class Handle:
     """A handle of the fake device: 4 sequences of 8 pages of 16 tokens, bf16, 2 heads of 32 (or entries of 128 values)."""
-    S, MP, NP, P, H, D = 4, 8, 20, 16, 2, 32
+    S, NP, P, H, D = 4, 20, 16, 2, 32
     W = H * D
 
-    def __init__(self, L, gqa, bounds=True, n_pages=None):
-        self.L, self.gqa = L, gqa
-        cfg = ct.PagedConfig(self.S, self.MP, n_pages or self.NP, self.P, 2 * self.W, 0, ct.CT_KV_BF16, 0)
+    def __init__(self, L, gqa, bounds=True, n_pages=None, window=0, pages_per_seq=8):
+        self.L, self.gqa, self.MP = L, gqa, pages_per_seq
+        cfg = ct.PagedConfig(self.S, self.MP, n_pages or self.NP, self.P, 2 * self.W, window, ct.CT_KV_BF16, 0)
         self.h = (L.ct_kv_paged_create_gqa(C.byref(cfg), self.H, self.D, int(bounds)) if gqa else L.ct_kv_paged_create(C.byref(cfg)))
         self.np = n_pages or self.NP
         self.rng = np.random.default_rng(7)
@@ -73,8 +73,9 @@ class Handle:
         self.L.ct_kv_paged_block_table(self.h, t.ctypes.data)
         return t
 
-    def check(self):
-        """Host and device tables agree, every token reads back, references and free pages add up, bounds follow."""
+    def check(self, mapped_only=False):
+        """Host and device tables agree, every token (that is still mapped) reads back, references and free pages add up, bounds
+        follow."""
         t = self.table()
         dev = np.ctypeslib.as_array(C.cast(self.L.ct_kv_paged_block_table_dev(self.h), C.POINTER(C.c_int32)), t.shape)
         assert np.array_equal(dev, t)
@@ -83,9 +84,11 @@ class Handle:
         out = C.create_string_buffer(2 * 2 * self.W * self.P * self.MP + 32)
         at = (C.addressof(out) + 31) // 16 * 16
         for s, r in enumerate(self.rows):
-            if len(r) == 0:
+            first = int(np.argmax(t[s] >= 0)) * self.P if mapped_only and (t[s] >= 0).any() else 0
+            r = r[first:]
+            if len(r) == 0 or (mapped_only and not (t[s] >= 0).any()):
                 continue
-            assert self.L.ct_kv_paged_gather(self.h, s, 0, len(r), at, ct.CT_KV_BF16) == 0
+            assert self.L.ct_kv_paged_gather(self.h, s, first, len(r), at, ct.CT_KV_BF16) == 0
             got = np.frombuffer((C.c_char * r.nbytes).from_address(at), np.uint16).reshape(r.shape)
             assert np.array_equal(got, r), s
         ids, n = np.unique(t[t >= 0], return_counts=True)
@@ -96,6 +99,8 @@ class Handle:
             bs = np.ctypeslib.as_array(C.cast(self.L.ct_kv_paged_bound_scales(self.h), C.POINTER(C.c_float)), (self.np, self.H))
             for s, r in enumerate(self.rows):
                 for lp in range(-(-len(r) // self.P)):
+                    if mapped_only and t[s, lp] < 0:
+                        continue
                     assert (bs[t[s, lp]] == min(self.P, len(r) - lp * self.P)).all()
 
     def close(self):
@@ -200,3 +205,66 @@ def test_a_new_handle_leaves_nothing_running(fake, gqa, tmp_path):
     assert fake.fake_unfinished() == 0
     h.check()
     h.close()
+
+
+def state(h):
+    """Everything of a handle that a call can change on the host."""
+    L = h.L
+    st = L.ct_kv_paged_stats(h.h)
+    last = np.zeros(h.S, np.uint64)
+    lens = np.zeros(h.S, np.uint32)
+    L.ct_kv_paged_last_access(h.h, last.ctypes.data)
+    L.ct_kv_paged_seq_lens(h.h, lens.ctypes.data)
+    return (h.table().tolist(), lens.tolist(), last.tolist(), [getattr(st, n) for n, _ in st._fields_],
+            [L.ct_kv_paged_page_refs(h.h, p) for p in range(h.np)], L.ct_kv_paged_evict_log(h.h, None, 0))
+
+
+@pytest.mark.parametrize("gqa", [False, True])
+@pytest.mark.parametrize("window", [0, 40])
+def test_an_append_without_room_changes_nothing(fake, gqa, window):
+    """The pool or a table row is full in the middle of the call, pages evicted and used again before that among them: the call
+    is refused as a whole, and works when there is room."""
+    h = Handle(fake, gqa, n_pages=11, window=window)
+    assert h.append([0, 1, 2], [33, 20, 16]) == 0
+    h.fork(0, 3, 20)
+    for seqs, counts in (([0, 1], [100, 3]), ([3, 0], [1, 129]), ([2, 2], [60, 60]), ([1, 0, 3], [30, 126, 30])):
+        before = state(h)
+        assert h.append(seqs, counts) == ct.CT_ERR_FULL, (seqs, counts)
+        assert state(h) == before
+        h.check(mapped_only=True)
+    assert fake.ct_kv_paged_free_seq(h.h, 2) == 0
+    h.rows[2] = h.rows[2][:0]
+    assert h.append([1, 2], [5, 17]) == 0
+    h.check(mapped_only=True)
+    h.close()
+
+
+@pytest.mark.parametrize("gqa", [False, True])
+def test_an_append_that_fails_on_the_device_changes_nothing(fake, gqa):
+    """Each device call of an append fails once (the staging buffers grow in it).  Up to the launch that writes the tokens the
+    handle stays as it was, on the host and on the device; the launch of the bounds comes after that, and the tokens are there."""
+    last = 0
+    for k in range(1, 40):
+        h = Handle(fake, gqa, n_pages=300, pages_per_seq=200)
+        assert h.append([0, 1], [40, 17]) == 0 and h.fork(0, 2, 21) == 0
+        before = state(h)
+        fake.fake_fail(k)
+        rows = [r.copy() for r in h.rows]
+        rc = h.append([0, 1, 3], [2000, 9, 2500])
+        failed = fake.fake_pending() < 0
+        fake.fake_fail(-1)
+        assert (rc != 0) == failed
+        if failed and state(h) != before:             # only the bounds are missing
+            assert gqa and k == last + 1
+            h.close()
+            break
+        if failed:
+            last = k
+            assert all(np.array_equal(a, b) for a, b in zip(h.rows, rows))
+            h.check()
+            assert h.append([0, 1, 3], [2000, 9, 2500]) == 0
+        h.check()
+        h.close()
+        if not failed:
+            break
+    assert last >= 5
